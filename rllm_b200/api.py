@@ -69,11 +69,12 @@ class LLM:
     def __init__(self, model: str | dict, dtype="bfloat16", device="cuda:0", seed: int = 0,
                  page_size: int = 16, num_pages: int | None = None, max_active: int = 64,
                  max_tokens_per_step: int = 2048, max_chunk: int | None = None,
-                 weight_std: float = 0.02, norm_std: float = 0.0):
+                 weight_std: float = 0.02, norm_std: float = 0.0, kv_quant: str = "none", weight_quant: str = "none"):
         """`model`: a folder with config.json + model.safetensors, or a raw config dict, which
-        gets random weights from `seed`."""
+        gets random weights from `seed`. `kv_quant` "int4": keys and values are held in 4 bits (4.5 with their scales);
+        `weight_quant` "int8": the layers' matrices in 8 bits, quantised at load, their inputs per token."""
         kw = dict(dtype=parse_dtype(dtype), device=device, page_size=page_size, num_pages=num_pages,
-                  max_requests=max_active)
+                  max_requests=max_active, kv_quant=kv_quant, weight_quant=weight_quant)
         if isinstance(model, dict):
             self.engine = random_engine(model, seed, std=weight_std, norm_std=norm_std, **kw)
             self.model_dir = None

@@ -1,8 +1,8 @@
 """Command line in the reference's manner: `rllm run`, `rllm batch`, `rllm bench`, with the
 reference's option names, meanings and defaults (src/commands/mod.rs:75-131, run.rs:20-22,
 batch.rs:21-23, bench.rs:37-39). Options of parts that are not built (--chat, --system, --tp,
---stream-experts, --image, --kv-quant other than none) are accepted and refused with a
-clear message. Added here: --prompt-ids (token ids instead of text), --dtype, --seed,
+--stream-experts, --image, --kv-quant other than none and int4) are accepted and refused with a
+clear message. Added here: --weight-quant (the reference quantises offline, src/commands/quantize.rs), --prompt-ids (token ids instead of text), --dtype, --seed,
 --page-size, --kv-pages, --random-weights (a configuration folder without weights).
 """
 from __future__ import annotations
@@ -28,7 +28,9 @@ def _model_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--tp", type=int, default=0, help="Tensor parallelism; this engine runs on one GPU (0 or 1).")
     p.add_argument("--stream-experts", action="store_true", help="(not built) MoE expert streaming")
     p.add_argument("--image", default=None, help="(not built) image input")
-    p.add_argument("--kv-quant", default="none", help='KV cache quantization; only "none" is built.')
+    p.add_argument("--kv-quant", default="none", help='KV cache quantization: "none" or "int4" (4 bits, a scale per 32 numbers).')
+    p.add_argument("--weight-quant", default="none", choices=["none", "int8"],
+                   help="Layers' matrices in 8 bits with a scale per output channel, quantised at load.")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     p.add_argument("--seed", type=int, default=None, help="Seed of the sampling random numbers.")
     p.add_argument("--page-size", type=int, default=16, help="Positions per cache page (reference: 16).")
@@ -47,8 +49,8 @@ def _refuse_unbuilt(a) -> None:
         bad.append("--stream-experts")
     if a.image:
         bad.append("--image")
-    if a.kv_quant != "none":
-        bad.append(f"--kv-quant {a.kv_quant} (only 'none')")
+    if a.kv_quant not in ("none", "int4"):
+        bad.append(f"--kv-quant {a.kv_quant} (only 'none' and 'int4')")
     if bad:
         sys.exit("rllm: not built in this engine: " + "; ".join(bad))
 
@@ -61,7 +63,7 @@ def _load(a, max_active: int):
             model = json.load(f)
     t0 = time.time()
     llm = LLM(model, dtype=a.dtype, seed=a.random_weights or 0, page_size=a.page_size,
-              num_pages=a.kv_pages, max_active=max_active)
+              num_pages=a.kv_pages, max_active=max_active, kv_quant=a.kv_quant, weight_quant=a.weight_quant)
     if a.random_weights is None:
         llm.model_dir = a.model
     llm.warm_up()          # modules loaded, a first graph captured: the first request is not the slow one

@@ -1,0 +1,197 @@
+// The cache held in 4 bits: new keys and values stored, stored ones read back (layout and formulas: quant.cuh).
+//
+// Both kernels are a read and a write with little between. Eight lanes share the 64 dimensions of a row's block, four numbers of
+// each of its two groups a lane: the groups' largest numbers meet in three shuffles, a lane's eight codes are one word,
+// and the block's 32 bytes and its two scales leave as whole pieces.
+#include "quant.cuh"
+
+using namespace rllm;
+
+namespace {
+
+constexpr int THREADS = 256;
+
+struct Pages {                       // one layer's tensors
+  uint8_t* k4; uint8_t* v4; bf16* ks; bf16* vs;
+  int nkv, page_size, hd;
+};
+
+template <typename T> __device__ __forceinline__ void load4(const T* p, bool vec, float (&v)[4]) {
+  if (sizeof(T) == 2 && vec) {
+    const uint2 a = __ldcg(reinterpret_cast<const uint2*>(p));
+    v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
+  } else if (sizeof(T) == 4 && vec) {
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = to_f32(p[i]);
+  }
+}
+
+// The codes (as nibbles from bit `shift` of `word` on) and the scale of a group, four numbers of it in each of eight lanes.
+__device__ __forceinline__ bf16 quantize_group(const float (&v)[4], int shift, uint32_t& word) {
+  float hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+  float bad = fmaf(v[0], 0.f, fmaf(v[1], 0.f, fmaf(v[2], 0.f, v[3] * 0.f)));      // 0, or NaN where a number is not finite
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    bad += __shfl_xor_sync(0xffffffffu, bad, o);
+  }
+  bf16 d = __float2bfloat16_rn((hi >= -lo ? hi : lo) * -0.125f);
+  if (bad != 0.f) d = __ushort_as_bfloat16((unsigned short)0x7fc0);
+  const float df = __bfloat162float(d);
+  const float inv = 1.f / df;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int c = 0;
+    if (df != 0.f && bad == 0.f) {
+      // (1 / d leaves the float range where |d| is below 2^-126: the division itself then)
+      const float r = fabsf(df) >= 1.17549435e-38f ? round_quotient(v[i], df, inv) : rintf(__fdiv_rn(v[i], df));
+      c = (int)fminf(fmaxf(r, -8.f), 7.f);
+    }
+    word |= (uint32_t)(c + 8) << (shift + 4 * i);
+  }
+  return d;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+kv4_store_kernel(const T* __restrict__ k, const T* __restrict__ v, long long ldk, long long ldv, bool vec,
+                 const int* __restrict__ slots, long long num_slots, Pages c, long long units) {
+  pdl_launch();
+  pdl_wait();
+  const long long idx = (long long)blockIdx.x * THREADS + threadIdx.x;
+  const int w = (int)(idx & 7);
+  long long u = idx >> 3;                                // (token, keys or values, head, block of 64)
+  const bool live = u < units;                           // (the lanes of a warp stay together for the shuffles)
+  if (!live) u = units - 1;
+  const int blocks = c.hd >> 6;
+  const int b = (int)(u % blocks);
+  const int h = (int)(u / blocks % c.nkv);
+  const long long tv = u / ((long long)blocks * c.nkv);
+  const bool is_v = tv & 1;
+  const long long t = tv >> 1;
+  const int slot = slots[t];
+  const T* src = (is_v ? v + t * ldv : k + t * ldk) + (size_t)h * c.hd + 64 * b + 4 * w;
+  float x0[4], x1[4];
+  load4<T>(src, vec, x0);
+  load4<T>(src + 32, vec, x1);
+  uint32_t word = 0u;
+  const bf16 d0 = quantize_group(x0, 0, word), d1 = quantize_group(x1, 16, word);
+  if (!live || slot < 0 || slot >= num_slots) return;    // a slot of -1: the layer must not write this token
+  const size_t row = ((size_t)(slot / c.page_size) * c.nkv + h) * c.page_size + slot % c.page_size;
+  reinterpret_cast<uint32_t*>((is_v ? c.v4 : c.k4) + row * (c.hd >> 1))[8 * b + w] = word;
+  if (w == 0) {
+    const uint32_t two = (uint32_t)__bfloat16_as_ushort(d0) | (uint32_t)__bfloat16_as_ushort(d1) << 16;
+    reinterpret_cast<uint32_t*>((is_v ? c.vs : c.ks) + row * (c.hd >> 5))[b] = two;
+  }
+}
+
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// Page i of sequence s goes to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind the
+// sequence's last token are zeros, and so are pages it does not hold. With `cu_q` (attention of portions) pages that no query
+// of the step sees are left out; table_out says which are there, cu_out counts the portions' rows from zero.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+kv4_read_kernel(Pages c, long long num_pages, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ kv_lens,
+                const int* __restrict__ cu_q, int window, int num_seqs, int width, T* __restrict__ k, T* __restrict__ v,
+                int* __restrict__ table_out, int* __restrict__ cu_out) {
+  pdl_launch();
+  pdl_wait();
+  const int i = blockIdx.x, s = blockIdx.y;
+  const int n = kv_lens[s];
+  int first = 0;                                         // the first position that a query sees
+  if (cu_q != nullptr && window > 0) first = max(0, n - (cu_q[s + 1] - cu_q[s]) - window + 1);
+  const int page = i * c.page_size < n ? block_table[(size_t)s * bt_stride + i] : -1;
+  const bool held = page >= 0 && page < num_pages;
+  const bool left_out = table_out != nullptr && (!held || (i + 1) * c.page_size <= first);
+  if (threadIdx.x == 0) {
+    if (table_out != nullptr && blockIdx.z == 0) table_out[(size_t)s * width + i] = left_out ? -1 : s * width + i;
+    if (cu_out != nullptr && i == 0 && blockIdx.z == 0) { cu_out[s] = cu_q[s] - cu_q[0]; if (s == num_seqs - 1) cu_out[s + 1] = cu_q[s + 1] - cu_q[0]; }
+  }
+  if (left_out) return;
+  const int blocks = c.hd >> 6, w = threadIdx.x & 7;
+  const int rows = c.nkv * c.page_size;                  // a page's rows, in the order in which they lie
+  const bool is_v = blockIdx.z;
+  const uint8_t* src = is_v ? c.v4 : c.k4;
+  const bf16* sc = is_v ? c.vs : c.ks;
+  T* dst = is_v ? v : k;
+  for (int u = threadIdx.x >> 3; u < rows * blocks; u += THREADS / 8) {
+    const int r = u / blocks, b = u - r * blocks;
+    const bool there = held && i * c.page_size + r % c.page_size < n;
+    float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
+    if (there) {
+      const size_t row = (size_t)page * rows + r;
+      const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(src + row * (c.hd >> 1)) + 8 * b + w);
+      const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(sc + row * (c.hd >> 5)) + b);
+      const float d0 = bf16_lo(two), d1 = bf16_hi(two);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { x0[e] = (float)code4(word, e) * d0; x1[e] = (float)code4(word, 4 + e) * d1; }
+    }
+    T* o = dst + (((size_t)s * width + i) * rows + r) * c.hd + 64 * b + 4 * w;
+    store4(o, x0);
+    store4(o + 32, x1);
+  }
+}
+
+int make_pages(Pages& c, void* k4, void* ks, void* v4, void* vs, int nkv, int page_size, int hd) {
+  if (nkv <= 0 || page_size <= 0 || (hd != 64 && hd != 128 && hd != 192 && hd != 256)) return ERR_BAD_SIZE;
+  if (((uintptr_t)k4 | (uintptr_t)v4 | (uintptr_t)ks | (uintptr_t)vs) & 15) return ERR_BAD_ALIGN;
+  c.k4 = (uint8_t*)k4; c.v4 = (uint8_t*)v4; c.ks = (bf16*)ks; c.vs = (bf16*)vs; c.nkv = nkv; c.page_size = page_size; c.hd = hd;
+  return 0;
+}
+
+}  // namespace
+
+// k, v [T, nkv * hd] float or bf16 with row strides ldk, ldv; slots int32 [T]: page * page_size + offset, -1 (or beyond the
+// num_pages pages): not stored. No slot twice in a call.
+RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk, long long ldv, const int* slots, void* k4, void* ks,
+                            void* v4, void* vs, long long num_pages, int T, int nkv, int page_size, int hd, void* stream) {
+  if (T <= 0) return 0;
+  Pages c;
+  const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
+  if (rc) return rc;
+  const long long units = (long long)T * 2 * nkv * (hd >> 6);
+  const long long blocks = (units * 8 + THREADS - 1) / THREADS;
+  if (blocks > 2147483647LL) return ERR_TOO_LARGE;
+  const uintptr_t piece = dt == DT_F32 ? 15 : 7;
+  const bool vec = ldk % 4 == 0 && ldv % 4 == 0 && !(((uintptr_t)k | (uintptr_t)v) & piece);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dt == DT_F32)
+    return launch_ex(kv4_store_kernel<float>, dim3((unsigned)blocks), dim3(THREADS), 0, s, 1, (const float*)k, (const float*)v, ldk, ldv,
+                     vec, slots, num_pages * page_size, c, units);
+  if (dt == DT_BF16)
+    return launch_ex(kv4_store_kernel<bf16>, dim3((unsigned)blocks), dim3(THREADS), 0, s, 1, (const bf16*)k, (const bf16*)v, ldk, ldv,
+                     vec, slots, num_pages * page_size, c, units);
+  return ERR_BAD_DTYPE;
+}
+
+// The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, page_size, hd] float or bf16 (rounded once). kv_lens int32
+// [num_seqs], block_table int32 with bt_stride >= width. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
+// [num_seqs + 1] for attention of portions, or null.
+RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
+                           const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, void* k, void* v,
+                           int* table_out, int* cu_out, int nkv, int page_size, int hd, void* stream) {
+  if (num_seqs <= 0 || width <= 0) return 0;
+  Pages c;
+  const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
+  if (rc) return rc;
+  if (num_seqs > 65535 || (cu_out != nullptr && cu_q == nullptr) || (long long)num_seqs * width > 2147483647LL) return ERR_TOO_LARGE;
+  if (((uintptr_t)k | (uintptr_t)v) & 15) return ERR_BAD_ALIGN;
+  cudaStream_t s = (cudaStream_t)stream;
+  const dim3 grid(width, num_seqs, 2);
+  if (dt == DT_F32)
+    return launch_ex(kv4_read_kernel<float>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
+                     num_seqs, width, (float*)k, (float*)v, table_out, cu_out);
+  if (dt == DT_BF16)
+    return launch_ex(kv4_read_kernel<bf16>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
+                     num_seqs, width, (bf16*)k, (bf16*)v, table_out, cu_out);
+  return ERR_BAD_DTYPE;
+}

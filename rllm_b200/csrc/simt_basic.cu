@@ -278,7 +278,7 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, const int* __restrict__ p
                                   const float* __restrict__ inv_freq, const float2* __restrict__ cos_sin,
                                   const int* __restrict__ slots,
                                   T* __restrict__ kcache, T* __restrict__ vcache, int nh, int nkv,
-                                  int hd, int page_size, int rot_dim) {
+                                  int hd, int page_size, int rot_dim, int keys_too) {
   pdl_launch();
   pdl_wait();
   const int t = blockIdx.x;
@@ -304,9 +304,8 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, const int* __restrict__ p
       ra = a * cs - b * sn;
       rb = a * sn + b * cs;
     }
-    if (head < nh) {
-      if (i < rh) { hp[ia] = from_f32<T>(ra); hp[ib] = from_f32<T>(rb); }
-    } else if (slot >= 0) {
+    if ((head < nh || keys_too) && i < rh) { hp[ia] = from_f32<T>(ra); hp[ib] = from_f32<T>(rb); }
+    if (head >= nh && slot >= 0) {
       const int kvh = head - nh;
       T* dst = kcache + (((size_t)page * nkv + kvh) * page_size + off) * hd;
       dst[ia] = from_f32<T>(ra);
@@ -326,7 +325,7 @@ __global__ void rope_cache_kernel(T* __restrict__ qkv, const int* __restrict__ p
 // step's table of angles: eight pairs per thread, 16-byte loads and stores.
 __global__ void rope_cache_vec_kernel(bf16* __restrict__ qkv, const float2* __restrict__ cos_sin,
                                       const int* __restrict__ slots, bf16* __restrict__ kcache,
-                                      bf16* __restrict__ vcache, int nh, int nkv, int hd, int page_size) {
+                                      bf16* __restrict__ vcache, int nh, int nkv, int hd, int page_size, int keys_too) {
   pdl_launch();
   pdl_wait();
   const int t = blockIdx.x;
@@ -355,10 +354,11 @@ __global__ void rope_cache_vec_kernel(bf16* __restrict__ qkv, const float2* __re
       oa32[e] = *reinterpret_cast<const uint32_t*>(&na);
       ob32[e] = *reinterpret_cast<const uint32_t*>(&nb);
     }
-    if (head < nh) {
+    if (head < nh || keys_too) {
       *reinterpret_cast<uint4*>(hp) = oa;
       *reinterpret_cast<uint4*>(hp + half) = ob;
-    } else if (slot >= 0) {
+    }
+    if (head >= nh && slot >= 0) {
       bf16* dst = kcache + (((size_t)page * nkv + (head - nh)) * page_size + off) * hd + 8 * c;
       *reinterpret_cast<uint4*>(dst) = oa;
       *reinterpret_cast<uint4*>(dst + half) = ob;
@@ -375,10 +375,11 @@ __global__ void rope_cache_vec_kernel(bf16* __restrict__ qkv, const float2* __re
   }
 }
 
+// keys_too: the rotated keys go back into qkv as well (a cache that is written from there).
 // cos_sin: the table of rllm_rope_table for these positions ([T][rot_dim / 2] float2), or null.
 RLLM_API int rllm_rope_cache_write(void* qkv, int dt, const int* positions, const float* inv_freq,
                                    const void* cos_sin, const int* slots, void* kcache, void* vcache, int T, int nh,
-                                   int nkv, int hd, int page_size, int rot_dim, void* stream) {
+                                   int nkv, int hd, int page_size, int rot_dim, int keys_too, void* stream) {
   if (T <= 0) return 0;
   if (hd % 2 || rot_dim % 2 || rot_dim > hd || rot_dim < 0) return ERR_BAD_SIZE;
   cudaStream_t s = (cudaStream_t)stream;
@@ -389,15 +390,15 @@ RLLM_API int rllm_rope_cache_write(void* qkv, int dt, const int* positions, cons
                        (!slots || (((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0);
   if (dt == DT_BF16 && cos_sin && rot_dim == hd && hd % 16 == 0 && aligned)
     return launch_ex(rope_cache_vec_kernel, dim3(T), dim3(128), 0, s, 1, (bf16*)qkv, (const float2*)cos_sin, slots,
-                     (bf16*)kcache, (bf16*)vcache, nh, nkv, hd, page_size);
+                     (bf16*)kcache, (bf16*)vcache, nh, nkv, hd, page_size, keys_too);
   if (dt == DT_F32)
     rc = launch_ex(rope_cache_kernel<float>, dim3(T), dim3(threads), 0, s, 1, (float*)qkv, positions, inv_freq, (const float2*)cos_sin, slots,
                                                    (float*)kcache, (float*)vcache, nh, nkv, hd,
-                                                   page_size, rot_dim);
+                                                   page_size, rot_dim, keys_too);
   else if (dt == DT_BF16)
     rc = launch_ex(rope_cache_kernel<bf16>, dim3(T), dim3(threads), 0, s, 1, (bf16*)qkv, positions, inv_freq, (const float2*)cos_sin, slots,
                                                   (bf16*)kcache, (bf16*)vcache, nh, nkv, hd,
-                                                  page_size, rot_dim);
+                                                  page_size, rot_dim, keys_too);
   else return ERR_BAD_DTYPE;
   return rc;
 }

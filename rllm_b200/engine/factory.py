@@ -8,6 +8,7 @@ import torch
 from ..cache import CacheManager, pages_for
 from ..config import config_from_dict, load_config
 from ..kernels.backend import Backend
+from ..parts.base import KV4CacheSpec, cache_kind_of
 from ..weights import init_random_weights, load_weights
 from .step import Engine
 
@@ -24,6 +25,49 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype must be one of {sorted(_DTYPES)}, got {name!r}") from None
 
 
+KV_QUANT = ("none", "int4")
+WEIGHT_QUANT = ("none", "int8")
+
+
+def set_kv_quant(model, kv_quant: str) -> None:
+    """"int4": every layer's keys and values are held in 4 bits (`KV4CacheSpec`); a model with another paged cache is refused.
+    Before the cache is made."""
+    if kv_quant not in KV_QUANT:
+        raise ValueError(f"kv_quant must be one of {KV_QUANT}, got {kv_quant!r}")
+    if kv_quant == "none":
+        return
+    specs = [s for s in model.cache_specs() if s is not None and cache_kind_of(s).paged]
+    able = [p for p in model.parts() if hasattr(p, "use_kv4")]
+    if not able:
+        raise ValueError(f"kv_quant {kv_quant!r}: this model has no cache of keys and values that can be held in 4 bits"
+                         + (f" (it has {sorted({type(s).__name__ for s in specs})})" if specs else ""))
+    for p in able:
+        p.use_kv4()
+    left = sorted({type(s).__name__ for s in model.cache_specs()
+                   if s is not None and cache_kind_of(s).paged and not isinstance(s, KV4CacheSpec)})
+    if left:
+        raise ValueError(f"kv_quant {kv_quant!r}: layers with {left} cannot be held in 4 bits")
+
+
+def set_weight_quant(model, weight_quant: str) -> None:
+    """"int8": the matrices that the parts declare (`Part.int8_params`) are held in 8 bits with a scale per output channel, and their
+    inputs are quantised per token. Embedding and output head stay as they are. After the weights are bound."""
+    if weight_quant not in WEIGHT_QUANT:
+        raise ValueError(f"weight_quant must be one of {WEIGHT_QUANT}, got {weight_quant!r}")
+    if weight_quant == "none":
+        return
+    from ..kernels import quant
+    seen = False
+    for p in model.parts():
+        for name in p.int8_params:
+            w = getattr(p, name)
+            with torch.cuda.device(w.device):
+                setattr(p, name, quant.quantize_matrix(w))
+            seen = True
+    if not seen:
+        raise ValueError(f"weight_quant {weight_quant!r}: no part of this model has matrices that can be held in 8 bits")
+
+
 def default_num_pages(model, page_size: int, dtype: torch.dtype, device, weights_bytes: int = 0,
                       fraction: float = 0.75) -> int:
     """Pages that fit in `fraction` of the free device memory (the reference takes 75 % of
@@ -37,9 +81,12 @@ def default_num_pages(model, page_size: int, dtype: torch.dtype, device, weights
 
 
 def make_engine(model, dtype, device="cuda:0", page_size: int = 16, num_pages: int | None = None,
-                max_tokens: int | None = None, max_requests: int = 256) -> Engine:
+                max_tokens: int | None = None, max_requests: int = 256, kv_quant: str = "none",
+                weight_quant: str = "none") -> Engine:
     """`model` must already hold its weights on `device`."""
     dtype = parse_dtype(dtype)
+    set_kv_quant(model, kv_quant)
+    set_weight_quant(model, weight_quant)
     backend = Backend(dtype, device)
     if num_pages is None:
         if max_tokens is not None:

@@ -67,7 +67,10 @@ class Engine:
         self.vocab = model.vocab_size
         # device words: [0] a kernel's bounded wait ran out, [1] a token id outside the table,
         # [2] checked runs: a page number or cache slot outside the pool, [3] spare
-        if backend.fast:
+        # products in 8 bits wait with the same bound in either run type
+        self._waits = backend.fast or any(hasattr(getattr(p, n, None), "codes") for p in (model.parts() if hasattr(model, "parts") else ())
+                                          for n in getattr(p, "int8_params", ()))
+        if self._waits:
             from ..kernels import sm100
             self.error_words = sm100.init(self.device).err
         else:
@@ -119,7 +122,7 @@ class Engine:
             self.error_words[2:3].zero_()
             what = f"slot of token {page & 0x3fffffff}" if page & 0x40000000 else f"block-table entry {page - 1}"
             raise StepError(f"checked run: a {what} named a page outside the pool (the access was skipped)")
-        if wait and self.backend.fast:
+        if wait and self._waits:
             from ..kernels import sm100
             sm100.check_error(self.device)
 

@@ -10,6 +10,7 @@ Both are hand-written CUDA; there is nothing else to fall back to.
 from __future__ import annotations
 
 import os
+from dataclasses import replace
 
 import torch
 
@@ -149,8 +150,26 @@ class Backend:
         # weights whose height is no multiple of 4 (a gate row per head, say) stay on the CUDA cores
         return self._sm100 is not None and w.shape[0] % 4 == 0 and self._sm100.gemm_supported(x, w)
 
+    @property
+    def _quant(self):
+        from . import quant
+        return quant
+
+    def quantize_weight(self, w):
+        """A weight [N, K] in 8 bits with a scale per output channel; the products below take it in place of the tensor."""
+        return self._quant.quantize_matrix(w)
+
+    def _int8(self, x, w, epilogue, out=None):
+        """The product with a weight in 8 bits: the rows are quantised first, a norm in front in the same kernel."""
+        q = self._quant
+        rows = q.quantize_rows(x.h, (x.weight, x.eps), x.rows) if isinstance(x, Normed) else q.quantize_rows(x)
+        return q.linear_int8(rows, w, epilogue, out, self.dtype)
+
     def linear(self, x, w, bias=None, tag=None):
         # `tag` names the product for per-operation timing (kernels/profile.py); it changes nothing here
+        if not isinstance(w, torch.Tensor):
+            y = self._int8(x, w, ops.EPI_STORE)
+            return y if bias is None else ops.add_bias(y, bias)
         if bias is None and self._fused_norm(x, w):
             return self._sm100.gemm_norm(x.h, x.weight, x.eps, w, ops.EPI_STORE, rows=x.rows, w_fixed=True)
         x = x.tensor() if isinstance(x, Normed) else x
@@ -161,6 +180,8 @@ class Backend:
         return ops.gemm_simt(x, w, ops.EPI_STORE, bias=bias)
 
     def linear_f32(self, x, w, tag=None):
+        if not isinstance(w, torch.Tensor):
+            return self._int8(x, w, ops.EPI_STORE_F32)
         if w.shape[0] <= ops.SKINNY_MAX:         # a gate row, a handful of heads: a warp a token
             return ops.gemm_skinny(x.tensor() if isinstance(x, Normed) else x, w)
         if self._fused_norm(x, w):
@@ -172,6 +193,8 @@ class Backend:
 
     def linear_residual(self, x, w, residual):
         """residual (float32, in place) += x W^T"""
+        if not isinstance(w, torch.Tensor):
+            return self._int8(x, w, ops.EPI_ACCUM_F32, residual)
         x = x.tensor() if isinstance(x, Normed) else x
         if self._tc(x, w):
             return self._sm100.product(x, w, ops.EPI_ACCUM_F32, out=residual)
@@ -179,6 +202,8 @@ class Backend:
 
     def linear_swiglu(self, x, w_gate_up):
         """silu(x Wg^T) * (x Wu^T) with w_gate_up = [Wg; Wu]"""
+        if not isinstance(w_gate_up, torch.Tensor):
+            return self._int8(x, w_gate_up, ops.EPI_SWIGLU)
         if self._fused_norm(x, w_gate_up, gate_up=True):
             return self._sm100.gemm_norm(x.h, x.weight, x.eps, w_gate_up, ops.EPI_SWIGLU, rows=x.rows, w_fixed=True)
         x = x.tensor() if isinstance(x, Normed) else x
@@ -200,10 +225,21 @@ class Backend:
         return t
 
     def qkv_rope_cache_write(self, x, w_qkv, bias, positions, inv_freq, cache, nh, nkv, hd, rot_dim=None,
-                             ctx=None, key=None):
+                             ctx=None, key=None, keys_too=False):
         """qkv = x w_qkv^T (+ bias), q and k rotated, k and v written to the cache. One kernel when
-        the tensor-core product takes the sizes, else the product followed by the rotation kernel."""
+        the tensor-core product takes the sizes, else the product followed by the rotation kernel. `keys_too`: the
+        caller reads the rotated keys from qkv."""
         rot_dim = hd if rot_dim is None else rot_dim
+        if "k4" in cache.tensors:
+            # the rotated keys are rounded to the run's type, as a cache of whole numbers holds them, then quantised
+            qkv = self.qkv_rope_cache_write(x, w_qkv, bias, positions, inv_freq, replace(cache, writes=False, tensors={}), nh, nkv, hd,
+                                            rot_dim, ctx, key, keys_too=True)
+            self._store_kv4(qkv, cache, nh, nkv, hd)
+            return qkv
+        if not isinstance(w_qkv, torch.Tensor):
+            qkv = self.linear(x, w_qkv, bias=bias)
+            self.rope_cache_write(qkv, positions, inv_freq, cache, nh, nkv, hd, rot_dim, ctx=ctx, key=key, keys_too=keys_too)
+            return qkv
         table = self.rope_table(ctx, positions, inv_freq, rot_dim, key)
         kc = cache.k if cache.writes else None
         if bias is None and self._fused_norm(x, w_qkv) and x.rows is None and 128 % hd == 0 and \
@@ -220,18 +256,37 @@ class Backend:
                                              cache.k if writes else None, cache.v if writes else None,
                                              nh, nkv, hd, cache.page_size, rot_dim, table=table, asked=True, w_fixed=True)
         qkv = self.linear(x, w_qkv, bias=bias)
-        self.rope_cache_write(qkv, positions, inv_freq, cache, nh, nkv, hd, rot_dim, ctx=ctx, key=key)
+        self.rope_cache_write(qkv, positions, inv_freq, cache, nh, nkv, hd, rot_dim, ctx=ctx, key=key, keys_too=keys_too)
         return qkv
 
-    def rope_cache_write(self, qkv, positions, inv_freq, cache, nh, nkv, hd, rot_dim=None, ctx=None, key=None):
+    def rope_cache_write(self, qkv, positions, inv_freq, cache, nh, nkv, hd, rot_dim=None, ctx=None, key=None, keys_too=False):
+        if "k4" in cache.tensors:
+            self.rope_cache_write(qkv, positions, inv_freq, replace(cache, writes=False, tensors={}), nh, nkv, hd, rot_dim, ctx, key, True)
+            self._store_kv4(qkv, cache, nh, nkv, hd)
+            return
         writes = cache.writes
         rot_dim = hd if rot_dim is None else rot_dim
         table = self.rope_table(ctx, positions, inv_freq, rot_dim, key)
         ops.rope_cache_write(qkv, positions, inv_freq, cache.slots if writes else None,
                              cache.k if writes else None, cache.v if writes else None,
-                             nh, nkv, hd, cache.page_size, rot_dim, table=table)
+                             nh, nkv, hd, cache.page_size, rot_dim, table=table, keys_too=keys_too)
+
+    def _store_kv4(self, qkv, cache, nh, nkv, hd):
+        if cache.writes:
+            self.kv4_store(qkv[:, nh * hd: (nh + nkv) * hd], qkv[:, (nh + nkv) * hd:], cache)
+
+    def kv4_store(self, k, v, cache):
+        """Keys and values [T, kv heads * head size] of the step's tokens into a cache layer held in 4 bits, at its slots."""
+        self._quant.kv4_store(k, v, cache.tensors, cache.slots)
+
+    def kv4_read(self, cache, ctx, dtype=None):
+        """(k, v) [sequences, pages, kv heads, page size, head size]: what a cache layer held in 4 bits stands for, in the run's
+        type or dtype; zeros behind a sequence's last token."""
+        return self._quant.kv4_read(cache.tensors, cache.block_table, ctx.kv_lens, ctx.max_kv_len, dtype or self.dtype)
 
     def attention(self, q, cache, ctx, nh, scale, window):
+        if "k4" in cache.tensors:
+            return self._quant.attention_kv4_simt(q, cache.tensors, ctx.token_seq, ctx.positions, cache.block_table, nh, scale, window)
         if self._sm100 is not None:
             out = self._sm100.attention(q, cache, ctx, nh, scale, window)
             if out is not None:

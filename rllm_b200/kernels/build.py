@@ -31,6 +31,7 @@ CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
 # sink, output gate and block mask plus the row-wise work of layers that norm after the sum; all in both
 # precisions, each built only when a model uses it; "recurrent" recurrent mixers with a short convolution (a state-space
 # and a delta-rule recurrence); "rows" the row-wise work of layers whose sublayers run side by side;
+# "quant" products in 8-bit integers and the cache held in 4 bits;
 # "hybrid" a gated recurrence whose gates read only the current token, attention whose heads' weights are mixed, and
 # sublayers gated into the stream.
 LIBRARIES: dict[str, list[str]] = {
@@ -41,6 +42,7 @@ LIBRARIES: dict[str, list[str]] = {
     "sink": ["sink_attention.cu", "stream_ops.cu"],
     "recurrent": ["recurrent.cu"],
     "rows": ["row_mix.cu"],
+    "quant": ["quant_rows.cu", "int8_gemm.cu", "kv4_cache.cu", "kv4_attention.cu"],
     "hybrid": ["talk_attention.cu", "gated_ops.cu"],
     "host": ["host_runtime.cpp"],          # no CUDA: the cache manager's bookkeeping and metadata writer
 }

@@ -36,7 +36,7 @@ _SIGS = {
         "rllm_rmsnorm": [_P, _P, _P, c_int, _P, c_int, c_int, c_int, c_float, _P],
         "rllm_rope_table": [_P, _P, _P, c_int, c_int, c_float, _P],
         "rllm_rope_cache_write": [_P, c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
-                                  c_int, _P],
+                                  c_int, c_int, _P],
         "rllm_gather_rows": [_P, _P, _P, c_int, c_int, _P],
         "rllm_step_meta": [_P, _P, c_int, _P, c_int, _P],
         "rllm_add_into": [_P, _P, c_int, c_longlong, _P],
@@ -193,8 +193,8 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, T: int, mag: flo
 def rope_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                      slots: torch.Tensor | None, kcache: torch.Tensor | None,
                      vcache: torch.Tensor | None, nh: int, nkv: int, hd: int, page_size: int,
-                     rot_dim: int | None = None, table: torch.Tensor | None = None) -> None:
-    """Rotate q and k of `qkv` [T, (nh+2nkv)*hd] (q in place) and write k, v to the cache.
+                     rot_dim: int | None = None, table: torch.Tensor | None = None, keys_too: bool = False) -> None:
+    """Rotate q and k of `qkv` [T, (nh+2nkv)*hd] (q in place, with `keys_too` k as well) and write k, v to the cache.
     `table`: `rope_table(positions, inv_freq[:rot_dim // 2], T)`, else the angles are computed here."""
     _cuda(qkv, "qkv")
     T = qkv.shape[0]
@@ -217,7 +217,7 @@ def rope_cache_write(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch
         raise KernelError(f"rope table must be contiguous float32 [{T}, {rot_dim // 2}, 2]")
     _check(_fn("simt", "rllm_rope_cache_write")(
         qkv.data_ptr(), _dt(qkv, "qkv"), positions.data_ptr(), inv_freq.data_ptr(), _ptr(table), _ptr(slots),
-        _ptr(kcache), _ptr(vcache), T, nh, nkv, hd, page_size, rot_dim, _stream()), "rope_cache_write")
+        _ptr(kcache), _ptr(vcache), T, nh, nkv, hd, page_size, rot_dim, int(keys_too), _stream()), "rope_cache_write")
 
 
 def gather_rows(x: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:

@@ -40,7 +40,7 @@ def _peaks() -> tuple[float, float]:
 
 
 def _nbytes(*tensors) -> int:
-    return sum(t.numel() * t.element_size() for t in tensors if isinstance(t, torch.Tensor))
+    return sum(getattr(t, "nbytes", 0) for t in tensors)
 
 
 def _visible(q: int, n: int, window: int | None) -> int:
@@ -142,13 +142,14 @@ class OpProfile:
 
     def attention(self, q, cache, ctx, nh, scale, window):
         hd = q.shape[1] // nh
-        nkv = cache.k.shape[1] if cache.k is not None else nh
+        four = "k4" in cache.tensors
+        nkv = cache.tensors["k4"].shape[1] if four else cache.k.shape[1]
         lens, qs = ctx.kv_lens_host, ctx.q_lens_host
         if lens is None:
             lens, qs = [ctx.max_kv_len] * ctx.num_seqs, [1] * ctx.num_seqs
         seen = [min(L, window + q - 1) if window else L for L, q in zip(lens, qs)]
         pairs = sum(q * (s - q) + q * (q + 1) // 2 for s, q in zip(seen, qs))
-        nbytes = sum(seen) * nkv * hd * 2 * cache.k.element_size() + 2 * _nbytes(q)
+        nbytes = sum(seen) * nkv * hd * 2 * (9 / 16 if four else cache.k.element_size()) + 2 * _nbytes(q)
         return self._timed("attention", nbytes, 4 * nh * hd * pairs, self._be.attention, q, cache, ctx, nh, scale, window)
 
     # ---- mixers with latents or a recurrent state, routed feed-forwards

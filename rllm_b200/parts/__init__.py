@@ -1,4 +1,4 @@
-from .base import (CacheKind, KVCacheSpec, LayerCache, NormedSum, Param, Part, ScaledSum, Source, StateSpec, Summands, cache_kind_of,
+from .base import (CacheKind, KV4CacheSpec, KVCacheSpec, LayerCache, NormedSum, Param, Part, ScaledSum, Source, StateSpec, Summands, cache_kind_of,
                    make_part, register_cache_kind, register_part, registered_parts)
 from .rope_rules import register_rope_rule, registered_rope_rules
 from .norm import RMSNorm
@@ -13,7 +13,7 @@ from .recurrent import DeltaRuleMixer, MinGRUMixer, SideBySideMixer, StateSpaceM
 from .embedding import Embedding, OutputHead, PairEmbedding
 
 __all__ = ["CacheKind", "cache_kind_of", "register_cache_kind", "register_rope_rule", "registered_rope_rules",
-           "KVCacheSpec", "LayerCache", "Param", "Part", "Source", "StateSpec", "make_part",
+           "KVCacheSpec", "KV4CacheSpec", "LayerCache", "Param", "Part", "Source", "StateSpec", "make_part",
            "register_part", "registered_parts", "RMSNorm", "RotaryEmbedding",
            "inverse_frequencies", "GQAttention", "SwiGLU", "PreNormBlock", "Embedding",
            "OutputHead", "InterleavedRotary", "SandwichBlock", "LoopStep", "LatentAttention",

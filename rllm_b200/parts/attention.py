@@ -9,12 +9,14 @@ A `window` limits each query to the last `window` keys
 """
 from __future__ import annotations
 
-from .base import KVCacheSpec, Param, Part, Source, register_part
+from .base import KV4CacheSpec, KVCacheSpec, Param, Part, Source, register_part
 
 
 class GQAttention(Part):
     graph_safe = True
     takes_deferred = True      # x goes to the backend's products as it comes
+    int8_params = ("w_qkv", "w_o")
+    kv4 = False                # keys and values held in 4 bits
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, position: Part,
                  window: int | None = None, bias: bool = False, scale: float | None = None):
@@ -50,8 +52,16 @@ class GQAttention(Part):
                                       Source("v_proj.bias", (KV,)))))
         return ps
 
+    def use_kv4(self):
+        """Hold this layer's keys and values in 4 bits (before the cache is made)."""
+        if self.head_dim % 64:
+            raise ValueError(f"a cache held in 4 bits needs heads of 64, 128, 192 or 256, not {self.head_dim}")
+        if not getattr(self.position, "stores_kv4", False):
+            raise ValueError(f"{type(self.position).__name__} does not write a cache held in 4 bits")
+        self.kv4 = True
+
     def cache_spec(self):
-        return KVCacheSpec(self.kv_heads, self.head_dim, self.window)
+        return (KV4CacheSpec if self.kv4 else KVCacheSpec)(self.kv_heads, self.head_dim, self.window)
 
     def forward(self, x, ctx, cache, residual):
         """x: normalised activations [T, hidden]; adds the mixer's output into `residual`."""

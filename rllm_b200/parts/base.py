@@ -63,6 +63,15 @@ class KVCacheSpec:
 
 
 @dataclass(frozen=True)
+class KV4CacheSpec:
+    """Paged keys and values held in 4 bits: per token and kv head `head_dim` codes (a multiple of 64, two a byte) and a
+    bfloat16 scale for each group of 32 of them, 4.5 bits a number. `window` as for `KVCacheSpec`."""
+    kv_heads: int
+    head_dim: int
+    window: int | None = None
+
+
+@dataclass(frozen=True)
 class StateSpec:
     """Fixed-size per-request state: name -> (shape, dtype). Zeroed when a request opens."""
     tensors: tuple[tuple[str, tuple[int, ...], torch.dtype], ...]
@@ -75,6 +84,9 @@ class Part:
     # True when `forward` reads nothing of the step on the host (no `*_host` mirror of the
     # context, no device-to-host copy): only then can a decode step be captured in a CUDA graph
     graph_safe: bool = False
+    # matrices of the part that may be held in 8 bits: the part hands them to the backend's `linear`, `linear_f32`,
+    # `linear_residual`, `linear_swiglu` or `qkv_rope_cache_write` and reads nothing else of them
+    int8_params: tuple[str, ...] = ()
 
     def params(self) -> list[Param]:
         return []
@@ -147,6 +159,12 @@ def _kv_allocate(spec, num_pages, page_size, dtype, device):
     return {"k": torch.zeros(shape, dtype=dtype, device=device), "v": torch.zeros(vshape, dtype=dtype, device=device)}
 
 
+def _kv4_allocate(spec, num_pages, page_size, _dtype, device):
+    shape = (num_pages, spec.kv_heads, page_size)
+    make = lambda n, dt: torch.zeros(shape + (spec.head_dim // n,), dtype=dt, device=device)
+    return {"k4": make(2, torch.uint8), "ks": make(32, torch.bfloat16), "v4": make(2, torch.uint8), "vs": make(32, torch.bfloat16)}
+
+
 def _state_allocate(spec, max_requests, _page_size, _dtype, device):
     return {name: torch.zeros((max_requests,) + tuple(shape), dtype=dt, device=device)
             for name, shape, dt in spec.tensors}
@@ -156,6 +174,9 @@ register_cache_kind(KVCacheSpec, CacheKind(
     paged=True, allocate=_kv_allocate, window=lambda spec: spec.window, chunk=lambda spec: spec.chunk,
     keep_first=lambda spec: spec.keep_first, page_bytes=lambda spec, page_size, dtype: spec.kv_heads * (spec.head_dim + (spec.v_dim or spec.head_dim)) * page_size
     * torch.empty((), dtype=dtype).element_size()))
+register_cache_kind(KV4CacheSpec, CacheKind(
+    paged=True, allocate=_kv4_allocate, window=lambda spec: spec.window,
+    page_bytes=lambda spec, page_size, dtype: 2 * spec.kv_heads * page_size * (spec.head_dim // 2 + spec.head_dim // 16)))
 register_cache_kind(StateSpec, CacheKind(paged=False, allocate=_state_allocate))
 
 
@@ -216,7 +237,7 @@ class LayerCache:
     """What a mixer gets for its cache layer in one step.
 
     Paged layers: `tensors[name]` with the page first (keys and values: `k`, `v`
-    [pages, kv_heads, page_size, head_dim]); `slots` [T] (page*page_size + offset of each new
+    [pages, kv_heads, page_size, head_dim]; held in 4 bits: `k4`, `ks`, `v4`, `vs`); `slots` [T] (page*page_size + offset of each new
     token, -1 where the layer must not write); `block_table` [sequences, pages] (-1 where a page was
     given back). Slot layers: `state[name]` [slots, *shape]; the request's slot is
     `ctx.state_slots[seq]`."""

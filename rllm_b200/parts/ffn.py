@@ -12,6 +12,7 @@ class SwiGLU(Part):
     graph_safe = True
     takes_deferred = True      # x goes to the backend's products as it comes
     returns_output = True
+    int8_params = ("w_gate_up", "w_down")
 
     def __init__(self, hidden: int, intermediate: int,
                  names=("gate_proj.weight", "up_proj.weight", "down_proj.weight")):

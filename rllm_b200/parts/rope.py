@@ -38,6 +38,7 @@ def inverse_frequencies(rot_dim: int, theta: float, scaling=None) -> list[float]
 class RotaryEmbedding(Part):
     """Rotates pairs (i, i + rot_dim/2) of each head by position * f_i."""
     graph_safe = True
+    stores_kv4 = True          # leaves the write to the backend, which knows caches held in 4 bits
     interleaved = False
 
     def __init__(self, head_dim: int, theta: float, scaling=None, rot_dim: int | None = None):
