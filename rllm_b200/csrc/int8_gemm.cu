@@ -1,49 +1,314 @@
 // Products in 8-bit integers: Y[t, n] = (sum_k X[t, k] W[n, k]) * sx[t] * sw[n], codes with one scale a row on both sides. The sum of
-// code products is exact in 32 bits up to K = 131,072 (127^2 K < 2^31).
+// code products is exact in 32 bits up to K = 131,072 (127^2 K < 2^31), so it does not matter how it is cut; the two scales and
+// the rounding to the output's type follow in float.
 //
-// One thread an output, four products an instruction.
+// Two kernels. Few tokens (`streams`): the weights' stream, with the tokens quantised on the way. More: tcgen05.mma.kind::i8, the codes of both sides brought
+// in by TMA, accumulators in TMEM.
 #include "quant.cuh"
+#include "sm100.cuh"
 
 using namespace rllm;
+using namespace sm100;
 
 namespace {
 
 enum : int { EPI_STORE = 0, EPI_STORE_F32 = 1, EPI_ACCUM_F32 = 2, EPI_SWIGLU = 3 };
 
 struct Int8Params {
-  const int8_t* x; const float* sx;
-  const int8_t* w; const float* sw;
+  const float* sx; const float* sw;
   void* y; long long ldy;
+  int vec;                           // rows of y start on 16 bytes
   int T, N, K;                       // N: outputs (of one half with SwiGLU); K: bytes a row, a multiple of 16
+  int box;                           // token rows a copy brings
+  int* err;
 };
 
-__device__ __forceinline__ float silu_gate(float g, float u) { return g / (1.f + expf(-g)) * u; }
+__device__ __forceinline__ float silu_gate(float g, float u, bool precise) {
+  return precise ? g / (1.f + expf(-g)) * u : __fdividef(g, 1.f + __expf(-g)) * u;
+}
 
-template <int EPI, typename OUT>
-__global__ void __launch_bounds__(256)
-int8_simple_kernel(const Int8Params p) {
-  pdl_launch();
-  pdl_wait();
-  const int n = blockIdx.x * 32 + (threadIdx.x & 31), t = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (n >= p.N || t >= p.T) return;
-  float v[2];
+// D (+)= A B with 8-bit signed operands and 32-bit sums.
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// s8 x s8 -> s32, A and B K-major, M x N tile.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+constexpr int BM = 128, BK = 128, UMMA_K = 32;      // token rows a tile, bytes of K a stage and an MMA
+constexpr int THREADS_TC = 320;
+
+template <int BN> struct TcCfg {                      // BN: weight rows a tile (gate and up rows together)
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES_RAW = 208 * 1024 / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN <= 64 ? 64 : 2 * BN;
+};
+
+// CH neighbouring outputs of one token.
+template <int EPI, typename OUT, int CH>
+__device__ __forceinline__ void emit_row(const Int8Params& p, int t, int n, const float (&v)[CH]) {
+  if (EPI == EPI_ACCUM_F32) {
+    float* y = (float*)p.y + (size_t)t * p.ldy + n;
+    if (p.vec && n + CH <= p.N) {
 #pragma unroll
-  for (int half = 0; half < (EPI == EPI_SWIGLU ? 2 : 1); ++half) {
-    const int row = n + half * p.N;
-    const int* x = reinterpret_cast<const int*>(p.x + (size_t)t * p.K);
-    const int* w = reinterpret_cast<const int*>(p.w + (size_t)row * p.K);
-    int acc = 0;
-    for (int k = 0; k < p.K / 4; ++k) acc = __dp4a(x[k], w[k], acc);
-    v[half] = (float)acc * p.sx[t] * p.sw[row];
+      for (int i = 0; i < CH; i += 4)
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) if (n + i < p.N) atomicAdd(y + i, v[i]);
+    }
+    return;
   }
-  const size_t o = (size_t)t * p.ldy + n;
-  if (EPI == EPI_ACCUM_F32) ((float*)p.y)[o] += v[0];
-  else ((OUT*)p.y)[o] = from_f32<OUT>(EPI == EPI_SWIGLU ? silu_gate(v[0], v[1]) : v[0]);
+  OUT* y = (OUT*)p.y + (size_t)t * p.ldy + n;
+  if (p.vec && n + CH <= p.N) {
+    if (sizeof(OUT) == 4) {
+#pragma unroll
+      for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(y + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * e], v[i + 2 * e + 1]);
+          w[e] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(y + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) if (n + i < p.N) y[i] = from_f32<OUT>(v[i]);
+  }
+}
+
+template <int CH> __device__ __forceinline__ void tmem_cols(uint32_t taddr, uint32_t (&r)[CH]) {
+  if constexpr (CH == 16) tmem_ld16(taddr, r); else tmem_ld32(taddr, r);
+}
+
+// One tile's accumulator from TMEM to the output, by eight warps: a thread's row is a token; the two warps of a quarter of the lanes take
+// half of the features each.
+template <int BN, int EPI, typename OUT>
+__device__ __forceinline__ void tile_out(const Int8Params& p, uint32_t taddr, int t0, int n0, int warp, int lane) {
+  constexpr bool DUAL = EPI == EPI_SWIGLU;
+  constexpr int F = DUAL ? BN / 2 : BN;                // features a tile
+  constexpr int CH = F / 2 >= 32 ? 32 : 16;
+  static_assert(F / 2 >= 16, "a warp takes 16 features or more");
+  const int t_warp = t0 + (warp & 3) * 32, t = t_warp + lane;
+  if (t_warp >= p.T) return;
+  const float sx = t < p.T ? p.sx[t] : 0.f;
+  const int grp = (warp - 2) >> 2;
+#pragma unroll 1
+  for (int c = grp * (F / 2); c < (grp + 1) * (F / 2); c += CH) {
+    const int n = n0 + c;
+    if (n >= p.N) break;
+    uint32_t a[CH], b[DUAL ? CH : 1];
+    tmem_cols<CH>(taddr + c, a);
+    if constexpr (DUAL) tmem_cols<CH>(taddr + F + c, b);
+    tmem_ld_wait();
+    float v[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int ni = min(n + i, p.N - 1);
+      v[i] = (float)(int)a[i] * sx * __ldg(p.sw + ni);
+      if constexpr (DUAL) v[i] = silu_gate(v[i], (float)(int)b[i] * sx * __ldg(p.sw + p.N + ni), sizeof(OUT) == 4);
+    }
+    if (t < p.T) emit_row<EPI, OUT, CH>(p, t, n, v);
+  }
+}
+
+// Tokens on the accumulator's rows, a tile of 128 tokens x BN weight rows; one CTA an SM walks the tiles, token tiles fastest (a weight tile
+// is then read by neighbouring CTAs at once). Warp 0 issues the copies, warp 1 the MMAs, warps 2-9 take the finished
+// accumulator out of TMEM while the next tile's is made. Few tokens fill a part of the 128 rows: the copies bring their rows only
+// (`box`), the rows behind them hold whatever lay there, and their sums are not read.
+template <int BN, int EPI, typename OUT>
+__global__ void __launch_bounds__(THREADS_TC, 1)
+int8_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Int8Params p) {
+  constexpr bool DUAL = EPI == EPI_SWIGLU;
+  constexpr int F = DUAL ? BN / 2 : BN;
+  typedef TcCfg<BN> C;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+  __shared__ int never_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int t_tiles = (p.T + BM - 1) / BM, n_tiles = (p.N + F - 1) / F;
+  const int tiles = t_tiles * n_tiles;
+  const int n_kb = (p.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 8); }
+    abort_flag = 0;
+    never_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) { prefetch_tensormap(&tmap_w); prefetch_tensormap(&tmap_x); }
+  if (warp == 1) { tmem_alloc(&tmem_base_slot, C::TMEM_COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch();
+  const uint32_t tmem_base = tmem_base_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint64_t pol_x = policy_evict_last();    // the token tiles are read by every weight tile
+      const uint32_t bytes = (uint32_t)(C::B_BYTES + p.box * BK);
+      const uint32_t st0 = smem_u32(smem);
+      // the first stages' weights need not wait for the kernel in front: what writes a weight's codes lets no kernel start before it ends
+      const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * n_kb;
+      const int pre = min(mine, C::STAGES);
+      auto weights = [&](int s, int tile, int kb) {
+        const uint32_t dst = st0 + s * C::STAGE_BYTES + C::A_BYTES, full = smem_u32(&full_bar[s]);
+        const int n0 = tile / t_tiles * F;
+        tma_load_2d(dst, &tmap_w, full, kb * BK, n0);
+        if (DUAL) tma_load_2d(dst + F * BK, &tmap_w, full, kb * BK, p.N + n0);
+      };
+      auto tokens = [&](int s, int tile, int kb) {
+        tma_load_2d_hint(st0 + s * C::STAGE_BYTES, &tmap_x, smem_u32(&full_bar[s]), kb * BK, tile % t_tiles * BM, pol_x);
+      };
+      for (int i = 0; i < pre; ++i) {
+        mbar_expect_tx(&full_bar[i], bytes);
+        weights(i, blockIdx.x + i / n_kb * gridDim.x, i % n_kb);
+      }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) tokens(i, blockIdx.x + i / n_kb * gridDim.x, i % n_kb);
+      int it = pre, tile = blockIdx.x + pre / n_kb * gridDim.x, kb = pre % n_kb;
+      for (; it < mine; ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&empty_bar[s], (uint32_t)(it / C::STAGES - 1) & 1u, &abort_flag)) {
+          abort_flag = 1; record_failure(p.err, 5); break;
+        }
+        mbar_expect_tx(&full_bar[s], bytes);
+        weights(s, tile, kb);
+        tokens(s, tile, kb);
+        if (++kb == n_kb) { kb = 0; tile += gridDim.x; }
+      }
+      if (abort_flag)                                // let copies already issued land before the shared memory is given back
+        for (int i = max(0, it - C::STAGES); i < it; ++i)
+          mbar_wait(&full_bar[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, &never_flag, 200000000LL);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_i8(BM, BN);
+      const uint64_t d0 = umma_desc_sw128(smem_u32(smem));
+      int it = 0, ti = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++ti) {
+        const int buf = ti & 1, use = ti >> 1;
+        if (use > 0 && !mbar_wait(&acc_empty[buf], (uint32_t)(use - 1) & 1u, &abort_flag)) {
+          abort_flag = 1; record_failure(p.err, 6); ok = false; break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem_base + (uint32_t)(buf * BN);
+        for (int kb = 0; kb < n_kb; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&full_bar[s], (uint32_t)(it / C::STAGES) & 1u, &abort_flag)) { abort_flag = 1; record_failure(p.err, 2); ok = false; break; }
+          tc_fence_after();
+          const uint64_t da = d0 + (uint64_t)(s * (C::STAGE_BYTES >> 4)), db = da + (uint64_t)(C::A_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_i8(acc, da + (uint64_t)(k * UMMA_K / 16), db + (uint64_t)(k * UMMA_K / 16), idesc, kb > 0 || k > 0);
+          umma_commit(&empty_bar[s]);
+        }
+        if (ok) umma_commit(&acc_full[buf]);
+      }
+    }
+  } else {
+    pdl_wait();
+    int ti = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++ti) {
+      const int buf = ti & 1, use = ti >> 1;
+      bool got = mbar_wait(&acc_full[buf], (uint32_t)use & 1u, &abort_flag);
+      if (!got) { abort_flag = 1; record_failure(p.err, 3); }
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(buf * BN);
+      tile_out<BN, EPI, OUT>(p, taddr, tile % t_tiles * BM, tile / t_tiles * F, warp, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, C::TMEM_COLS); }
+}
+
+// ------------------------------------------------------------------------------------ host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+  static const EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return (EncodeTiledFn)f;
+  }();
+  return fn;
+}
+
+// codes [rows, K], a copy brings 128 bytes of `box` rows
+int make_map(CUtensorMap* m, const void* ptr, long long rows, int K, int box) {
+  const EncodeTiledFn enc = encoder();
+  if (!enc) return -5;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)K};
+  const cuuint32_t b[2] = {(cuuint32_t)BK, (cuuint32_t)box}, one[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -5;
+}
+
+template <int BN, int EPI, typename OUT>
+int launch_tc(const void* x, const void* w, Int8Params p, int sm_count, cudaStream_t s) {
+  typedef TcCfg<BN> C;
+  constexpr int F = EPI == EPI_SWIGLU ? BN / 2 : BN;
+  static bool configured[64] = {};
+  if (allow_dynamic_smem(int8_tc_kernel<BN, EPI, OUT>, C::SMEM_BYTES, configured)) return -5;
+  p.box = p.T >= BM ? BM : (p.T + 7) / 8 * 8;
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, x, p.T, p.K, p.box);
+  if (!rc) rc = make_map(&mw, w, EPI == EPI_SWIGLU ? 2ll * p.N : p.N, p.K, F);
+  if (rc) return rc;
+  const long long tiles = (long long)((p.T + BM - 1) / BM) * ((p.N + F - 1) / F);
+  if (tiles > 2147483647LL) return ERR_TOO_LARGE;
+  return launch_ex(int8_tc_kernel<BN, EPI, OUT>, dim3((unsigned)(tiles < sm_count ? tiles : sm_count)), dim3(THREADS_TC), C::SMEM_BYTES, s, 1, mx, mw, p);
+}
+
+// Weight rows a tile: the widest that still gives most SMs one, since a CTA reads its token tile again for every weight tile.
+int tile_rows(int T, int rows, int sm_count) {
+  const long long t_tiles = (T + BM - 1) / BM;
+  for (int bn = 256; bn > 64; bn >>= 1)
+    if (t_tiles * ((rows + bn - 1) / bn) * 4 >= 3ll * sm_count) return bn;
+  return 64;
 }
 
 template <int EPI, typename OUT>
-int launch_simple(const Int8Params& p, cudaStream_t s) {
-  return launch_ex(int8_simple_kernel<EPI, OUT>, dim3((p.N + 31) / 32, (p.T + 7) / 8), dim3(256), 0, s, 1, p);
+int launch_epi(const void* x, const void* w, const Int8Params& p, int sm_count, cudaStream_t s) {
+  switch (tile_rows(p.T, EPI == EPI_SWIGLU ? 2 * p.N : p.N, sm_count)) {
+    case 256: return launch_tc<256, EPI, OUT>(x, w, p, sm_count, s);
+    case 128: return launch_tc<128, EPI, OUT>(x, w, p, sm_count, s);
+    default: return launch_tc<64, EPI, OUT>(x, w, p, sm_count, s);
+  }
 }
 
 }  // namespace
@@ -53,14 +318,14 @@ int launch_simple(const Int8Params& p, cudaStream_t s) {
 RLLM_API int rllm_int8_gemm(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
                             int T, int N, int K, int* err, int sm_count, void* stream) {
   if (T <= 0 || N <= 0) return 0;
-  if (K <= 0 || K % 16 || K > 131072 || ldy < N || epi < 0 || epi > 3) return ERR_BAD_SIZE;
+  if (K <= 0 || K % 16 || K > 131072 || ldy < N || epi < 0 || epi > 3 || N > (1 << 30)) return ERR_BAD_SIZE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
   if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
-  (void)err; (void)sm_count;
-  const Int8Params p = {(const int8_t*)x, sx, (const int8_t*)w, sw, y, ldy, T, N, K};
+  const int size = epi == EPI_STORE_F32 || epi == EPI_ACCUM_F32 || out_dt == DT_F32 ? 4 : 2;
+  const Int8Params p = {sx, sw, y, ldy, !((uintptr_t)y & 15) && ldy * size % 16 == 0, T, N, K, 0, err};
   cudaStream_t s = (cudaStream_t)stream;
-  if (epi == EPI_STORE_F32) return launch_simple<EPI_STORE_F32, float>(p, s);
-  if (epi == EPI_ACCUM_F32) return launch_simple<EPI_ACCUM_F32, float>(p, s);
-  if (epi == EPI_STORE) return out_dt == DT_F32 ? launch_simple<EPI_STORE, float>(p, s) : launch_simple<EPI_STORE, bf16>(p, s);
-  return out_dt == DT_F32 ? launch_simple<EPI_SWIGLU, float>(p, s) : launch_simple<EPI_SWIGLU, bf16>(p, s);
+  if (epi == EPI_STORE_F32) return launch_epi<EPI_STORE_F32, float>(x, w, p, sm_count, s);
+  if (epi == EPI_ACCUM_F32) return launch_epi<EPI_ACCUM_F32, float>(x, w, p, sm_count, s);
+  if (epi == EPI_STORE) return out_dt == DT_F32 ? launch_epi<EPI_STORE, float>(x, w, p, sm_count, s) : launch_epi<EPI_STORE, bf16>(x, w, p, sm_count, s);
+  return out_dt == DT_F32 ? launch_epi<EPI_SWIGLU, float>(x, w, p, sm_count, s) : launch_epi<EPI_SWIGLU, bf16>(x, w, p, sm_count, s);
 }

@@ -33,13 +33,14 @@ struct RowArgs {
   const void* g; int g_is_bf16; float eps;      // norm weight, or null: no norm
   int8_t* codes; long long ldc; float* scales;
   int K;
+  int early;                       // the next kernel in the stream may begin before this one ends
 };
 
 // VPT: groups of 8 numbers a thread holds; 0: any K, two passes. VEC: rows and weight start on 16 (32) bytes, K is a multiple of 8.
 template <typename T, int VPT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 quantize_rows_kernel(const RowArgs a) {
-  pdl_launch();
+  if (a.early) pdl_launch();
   pdl_wait();
   __shared__ float red[32];
   const int t = blockIdx.x, K = a.K;
@@ -144,14 +145,15 @@ int launch_rows(const RowArgs& a, int T_, cudaStream_t s) {
 }  // namespace
 
 // x [*, K] float or bf16 with row stride ldx; rows int32 [T] or null; g norm weight [K] (g_dt) or null. codes int8 [T, ldc], ldc a
-// multiple of 16 that holds K, zeros behind K; scales float [T].
+// multiple of 16 that holds K, zeros behind K; scales float [T]. early 0 for a weight: the products read its codes before they wait for
+// the kernel in front of them.
 RLLM_API int rllm_quantize_rows(int dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
-                                void* codes, long long ldc, float* scales, int T, int K, void* stream) {
+                                void* codes, long long ldc, float* scales, int T, int K, int early, void* stream) {
   if (T <= 0) return 0;
   if (K <= 0 || ldc < K || ldc % 16 || ldc - K >= 16) return ERR_BAD_SIZE;
   if ((uintptr_t)codes & 15) return ERR_BAD_ALIGN;
   if (dt != DT_F32 && dt != DT_BF16) return ERR_BAD_DTYPE;
-  const RowArgs a = {x, ldx, rows, g, g_dt == DT_BF16, eps, (int8_t*)codes, ldc, scales, K};
+  const RowArgs a = {x, ldx, rows, g, g_dt == DT_BF16, eps, (int8_t*)codes, ldc, scales, K, early};
   const int unit = dt == DT_F32 ? 4 : 8;
   const bool vec = K % 8 == 0 && ldx % unit == 0 && !((uintptr_t)x & 15) && !((uintptr_t)g & 15);
   cudaStream_t s = (cudaStream_t)stream;

@@ -16,7 +16,7 @@ from . import ops, sm100
 
 _P = c_void_p
 ops.register_signatures("quant", {
-    "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, _P],
+    "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, c_int, _P],
     "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
     "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
@@ -88,7 +88,7 @@ def quantize_rows(x: torch.Tensor, norm: tuple | None = None, rows: torch.Tensor
     scales = torch.empty(T, dtype=torch.float32, device=x.device)
     ops._check(ops._fn("quant", "rllm_quantize_rows")(
         dt, x.data_ptr(), x.stride(0), ops._ptr(rows), ops._ptr(w), 0 if w is None else ops._dt(w, "norm weight"), float(eps),
-        codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, K, ops._stream()), "quantize_rows")
+        codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, K, int(cls is Int8Rows), ops._stream()), "quantize_rows")
     return cls(codes, scales, K)
 
 
