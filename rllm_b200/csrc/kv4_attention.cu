@@ -1,13 +1,32 @@
 // Attention over the paged cache held in 4 bits (layout: quant.cuh).
 //
+// Single tokens, heads of 64 and 128 in bfloat16 (kv4_decode_kernel): one pass over the codes, which stay codes until they are fragments of
+// mma.sync. A CTA has one (sequence, kv head, range of keys), a warp tiles of keys of its own, which per-lane
+// asynchronous copies bring into a ring; the ranges of a sequence form a cluster and meet in distributed shared memory.
+//   * S^T = K Q^T, keys on the rows (16 of them an instruction), the query heads of the kv head on the 8 columns: with the queries on the
+//     rows, 4 heads a kv head would fill a quarter of the instruction.
+//   * A number of the key fragment is bf16 128 + nibble, two of them by one AND-OR of a word; 136 sum(q) is what the products have too
+//     much, the accumulator starts at minus that. Codes and queries are exact in bfloat16, so a group's sum is as exact as float; it is
+//     multiplied by the group's scale as a float number. No dequantised key exists.
+//   * O^T = V^T P^T, dimensions on the rows: a value fragment pairs two keys' codes of one dimension, which is two words' halves put side by
+//     side. (128 + nibble) - 136 is exact here, where starting at a correction would not do: values cancel. The scale of a (key, group)
+//     goes onto the weight in float, before its one rounding to bfloat16; movmatrix turns the rounded weights from rows of keys into the
+//     columns that the second product takes.
+//   * Which key a row of the fragment stands for is free, as long as both products agree, and is chosen so that neither product's reads of
+//     shared memory meet a bank twice.
+//   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which float and bfloat16
+//     hold as well as 1, and the lanes' maxima meet once in a while instead of in every tile.
+//
 // On the CUDA cores, for any mix of prompt portions and single tokens, both run types and head sizes of 64, 128, 192 and 256: one
 // warp per (query token, query head), keys 32 at a time in position order with a running maximum and sum, all arithmetic in
 // float, as paged_attention_simt_kernel does over a cache of whole numbers. A lane scores one key: the key's codes times the
 // queries of a group of 32 are summed first and multiplied by the group's scale once. The weighted sum of the values takes one
 // byte of a row's block a lane, which is two neighbouring dimensions.
 #include "quant.cuh"
+#include "sm100.cuh"
 
 using namespace rllm;
+using namespace sm100;
 
 namespace {
 
@@ -21,6 +40,7 @@ struct Kv4Params {
   const int* block_table; int bt_stride;
   int rows, nh, nkv, page_size, window;
   float scale;
+  int page_shift, splits;
 };
 
 constexpr int WARPS = 4;
@@ -112,6 +132,355 @@ kv4_attention_simt_kernel(const Kv4Params p) {
   }
 }
 
+// ---------------------------------------------------------------------------- single tokens
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turn8x8(uint32_t v) {          // an 8 x 8 matrix of 16-bit numbers, rows to columns
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  const int n = there ? BYTES : 0;                                 // 0 bytes read: the place is filled with zeros
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float fast_exp2(float x) {              // exp2(-inf) = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+// Nibble i of both halves of a word as two bfloat16 numbers 128 + nibble.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t minus136(uint32_t v) {
+  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&v);
+  const uint32_t c = 0x43084308u;                                  // 136, 136
+  const __nv_bfloat162 r = __hsub2(a, *reinterpret_cast<const __nv_bfloat162*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A warp's tile is 4.5 KB whatever the head size, three of them a warp: 108 KB a CTA, two CTAs an SM.
+template <int HD> struct DecCfg {
+  static constexpr int NW = 8, D = 3, THREADS = NW * 32;
+  static constexpr int TILE = HD == 64 ? 64 : 32;                  // keys
+  static constexpr int CODES = TILE * HD / 2, SCALES = TILE * HD / 16;
+  static constexpr int STAGE = 2 * (CODES + SCALES);               // K codes, V codes, K scales, V scales
+  static constexpr int RING = NW * D * STAGE;
+  // the warps' parts lie over the ring once it is done with: [NW][queries][HD], then the CTA's [queries][HD], maxima and sums
+  static constexpr int parts(int nq) { return (NW + 1) * nq * HD * 4 + (NW + 1) * 16 * 8; }
+};
+static_assert(DecCfg<128>::RING >= DecCfg<128>::parts(16) && DecCfg<64>::RING >= DecCfg<64>::parts(16), "the parts fit the ring");
+
+// Where 16-byte piece `ch` of key row r lies in a tile of codes.
+template <int HD> __device__ __forceinline__ uint32_t code_off(int r, int ch) {
+  return HD == 128 ? (uint32_t)(r * 64 + ((ch ^ ((((r >> 1) ^ (r >> 2)) & 1) << 1)) << 4)) : (uint32_t)((r ^ (((r >> 2) & 1) << 1)) * 32 + (ch << 4));
+}
+
+// NQ: groups of 8 query heads a CTA
+template <int HD, int NQ>
+__global__ void __launch_bounds__(256, NQ == 1 ? 2 : 1)
+kv4_decode_kernel(const Kv4Params p) {
+  typedef DecCfg<HD> C;
+  constexpr int NW = C::NW, D = C::D, TILE = C::TILE, THREADS = C::THREADS;
+  constexpr int GR = HD / 32, BL = HD / 64;              // groups and blocks of a row
+  constexpr int CPR = HD / 32;                           // 16-byte pieces of a row's codes
+  extern __shared__ __align__(128) uint8_t ring_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, qi = lane & 3;
+  const int G = p.nh / p.nkv, qgroups = (G + 8 * NQ - 1) / (8 * NQ);
+  const int kvh = blockIdx.x / qgroups, seq = blockIdx.y;
+  const int h0 = kvh * G + blockIdx.x % qgroups * (8 * NQ);        // first query head
+  const int nq = min(8 * NQ, kvh * G + G - h0);
+  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+  pdl_launch();
+  pdl_wait();                                            // the kernel in front may have written any of the cache
+
+  const int pos = p.kv_lens[seq] - 1;
+  const int lo = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
+  const int tile_first = lo / TILE, tiles_total = pos >= 0 ? pos / TILE + 1 - tile_first : 0;
+  const int per = (tiles_total + p.splits - 1) / p.splits;
+  const int tb = tile_first + rank * per;
+  const int n_tiles = max(0, min(tile_first + tiles_total, tb + per) - tb);
+  const int* bt = p.block_table + (size_t)seq * p.bt_stride;
+  const uint32_t base = smem_u32(ring_raw), ring = base + (uint32_t)(warp * D) * C::STAGE;
+
+  // Starts the copies of this warp's tile i and closes a copy group, also when there is no such tile, so that the groups can be counted.
+  auto issue = [&](int i, int slot) {
+    if (i < n_tiles) {
+      const uint32_t st = ring + (uint32_t)slot * C::STAGE;
+      const int j0 = (tb + i) * TILE;
+      int row[TILE / 32];                                // a lane finds the rows of its keys, the others ask it
+#pragma unroll
+      for (int h = 0; h < TILE / 32; ++h) {
+        const int j = j0 + 32 * h + lane;
+        row[h] = -1;
+        if (j >= lo && j <= pos) {
+          const int pg = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
+          const int page = __ldcg(bt + pg);
+          if (page >= 0 && page < p.num_pages) row[h] = (page * p.nkv + kvh) * p.page_size + (j - pg * p.page_size);
+        }
+        const size_t r = row[h] < 0 ? 0 : row[h];
+        copy_async<HD / 16>(st + 2 * C::CODES + (32 * h + lane) * (HD / 16), p.ks + r * GR, row[h] >= 0);
+        copy_async<HD / 16>(st + 2 * C::CODES + C::SCALES + (32 * h + lane) * (HD / 16), p.vs + r * GR, row[h] >= 0);
+      }
+#pragma unroll
+      for (int c = 0; c < TILE * CPR / 32; ++c) {
+        const int key = (c * 32 + lane) / CPR, ch = lane % CPR;
+        const int r = __shfl_sync(0xffffffffu, row[c * 32 / CPR / 32], key & 31);
+        const size_t src = (size_t)(r < 0 ? 0 : r) * (HD / 2) + 16 * ch;
+        const uint32_t dst = st + code_off<HD>(key, ch);
+        copy_async<16>(dst, p.k4 + src, r >= 0);
+        copy_async<16>(dst + C::CODES, p.v4 + src, r >= 0);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) issue(warp + d * NW, d);
+
+  // the queries as fragments: lane (quad, qi) has numbers 8 qi .. 8 qi + 7 of each group of query `quad`; in a step of 16 numbers go
+  // number 2s of both its words (pairs i, i + 4), then 2s + 1
+  uint32_t qf[NQ][GR][2][2];
+  float qsum[NQ][GR][2];                                 // -136 sum(q) of queries 2 qi and 2 qi + 1
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const bool live = 8 * x + quad < nq;
+    const bf16* qp = (const bf16*)p.q + (size_t)seq * p.q_stride + (size_t)(h0 + (live ? 8 * x + quad : 0)) * HD + 8 * qi;
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      uint4 v = live ? __ldcg(reinterpret_cast<const uint4*>(qp + 32 * g)) : make_uint4(0u, 0u, 0u, 0u);
+      qf[x][g][0][0] = __byte_perm(v.x, v.z, 0x5410); qf[x][g][0][1] = __byte_perm(v.x, v.z, 0x7632);
+      qf[x][g][1][0] = __byte_perm(v.y, v.w, 0x5410); qf[x][g][1][1] = __byte_perm(v.y, v.w, 0x7632);
+      const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816(c, ones, qf[x][g][0][0], qf[x][g][0][1]);
+      mma16816(c, ones, qf[x][g][1][0], qf[x][g][1][1]);
+      qsum[x][g][0] = -136.f * c[0]; qsum[x][g][1] = -136.f * c[1];
+    }
+  }
+
+  float o[NQ][2 * GR][4];                                // rows: dimensions (see below), columns: queries 2 qi, 2 qi + 1
+  float m[NQ][2], l[NQ][2];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+#pragma unroll
+    for (int i = 0; i < 2 * GR; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+    m[x][0] = m[x][1] = -INFINITY;
+    l[x][0] = l[x][1] = 0.f;
+  }
+  const float sl = p.scale * 1.4426950408889634f;
+  // row r of a fragment is key (r & 7) / 2 + 4 (r & 1) + (r & 8)
+  const int krow = (quad >> 1) + 4 * (quad & 1);
+  int slot = 0;
+  for (int i = warp; i < n_tiles; i += NW) {
+    copy_wait<D - 1>();                                  // this warp's oldest group, tile i, has landed
+    __syncwarp();
+    const uint32_t st = ring + (uint32_t)slot * C::STAGE;
+    const int j0 = (tb + i) * TILE;
+    const bool edge = j0 < lo || j0 + TILE - 1 > pos;
+#pragma unroll 1
+    for (int sub = 0; sub < TILE / 16; ++sub) {
+      const int k0 = 16 * sub;
+      float s[NQ][4];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+      // ---- scores, group by group
+      uint32_t sc[2][BL];                                // the scales of rows quad and quad + 8
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
+#pragma unroll
+      for (int b = 0; b < BL; ++b) {
+        const uint2 wa = lds64(st + code_off<HD>(k0 + krow, 2 * b + (qi >> 1)) + 8 * (qi & 1));
+        const uint2 wb = lds64(st + code_off<HD>(k0 + krow + 8, 2 * b + (qi >> 1)) + 8 * (qi & 1));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t ta = __byte_perm(wa.x, wa.y, h ? 0x7632 : 0x5410), tb2 = __byte_perm(wb.x, wb.y, h ? 0x7632 : 0x5410);
+          const uint32_t a0[4] = {nibbles(ta, 0), nibbles(tb2, 0), nibbles(ta, 1), nibbles(tb2, 1)};
+          const uint32_t a1[4] = {nibbles(ta, 2), nibbles(tb2, 2), nibbles(ta, 3), nibbles(tb2, 3)};
+          const float d0 = h ? bf16_hi(sc[0][b]) : bf16_lo(sc[0][b]), d1 = h ? bf16_hi(sc[1][b]) : bf16_lo(sc[1][b]);
+#pragma unroll
+          for (int x = 0; x < NQ; ++x) {
+            const int g = 2 * b + h;
+            float c[4] = {qsum[x][g][0], qsum[x][g][1], qsum[x][g][0], qsum[x][g][1]};
+            mma16816(c, a0, qf[x][g][0][0], qf[x][g][0][1]);
+            mma16816(c, a1, qf[x][g][1][0], qf[x][g][1][1]);
+            s[x][0] = fmaf(d0, c[0], s[x][0]); s[x][1] = fmaf(d0, c[1], s[x][1]);
+            s[x][2] = fmaf(d1, c[2], s[x][2]); s[x][3] = fmaf(d1, c[3], s[x][3]);
+          }
+        }
+      }
+      if (edge) {
+        const int ja = j0 + k0 + krow, jb = ja + 8;
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if (ja < lo || ja > pos) s[x][0] = s[x][1] = -INFINITY;
+          if (jb < lo || jb > pos) s[x][2] = s[x][3] = -INFINITY;
+        }
+      }
+      // ---- weights
+      float pr[NQ][4];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        float mx0 = fmaxf(s[x][0], s[x][2]) * sl, mx1 = fmaxf(s[x][1], s[x][3]) * sl;
+        if (__any_sync(0xffffffffu, mx0 > m[x][0] + 8.f || mx1 > m[x][1] + 8.f)) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+          }
+          mx0 = fmaxf(mx0, m[x][0]); mx1 = fmaxf(mx1, m[x][1]);
+          const float c0 = m[x][0] == mx0 ? 1.f : fast_exp2(m[x][0] - mx0), c1 = m[x][1] == mx1 ? 1.f : fast_exp2(m[x][1] - mx1);
+          m[x][0] = mx0; m[x][1] = mx1;
+          l[x][0] *= c0; l[x][1] *= c1;
+#pragma unroll
+          for (int t = 0; t < 2 * GR; ++t) { o[x][t][0] *= c0; o[x][t][1] *= c1; o[x][t][2] *= c0; o[x][t][3] *= c1; }
+        }
+        const float u0 = m[x][0] == -INFINITY ? 0.f : m[x][0], u1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+        pr[x][0] = fast_exp2(fmaf(s[x][0], sl, -u0)); pr[x][1] = fast_exp2(fmaf(s[x][1], sl, -u1));
+        pr[x][2] = fast_exp2(fmaf(s[x][2], sl, -u0)); pr[x][3] = fast_exp2(fmaf(s[x][3], sl, -u1));
+        l[x][0] += pr[x][0] + pr[x][2];
+        l[x][1] += pr[x][1] + pr[x][3];
+      }
+      // ---- values: the keys of columns 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + C::SCALES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
+#pragma unroll
+      for (int b = 0; b < BL; ++b) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = lds32(st + C::CODES + code_off<HD>(k0 + qi + 4 * e, 2 * b + (quad >> 2)) + 4 * (quad & 3));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t ta = __byte_perm(w[0], w[1], h ? 0x7632 : 0x5410), tb2 = __byte_perm(w[2], w[3], h ? 0x7632 : 0x5410);
+          const int g = 2 * b + h;
+          const float d0 = h ? bf16_hi(sc[0][b]) : bf16_lo(sc[0][b]), d1 = h ? bf16_hi(sc[1][b]) : bf16_lo(sc[1][b]);
+          uint32_t b0[NQ], b1[NQ];
+#pragma unroll
+          for (int x = 0; x < NQ; ++x) {
+            b0[x] = turn8x8(pack2(pr[x][0] * d0, pr[x][1] * d0));
+            b1[x] = turn8x8(pack2(pr[x][2] * d1, pr[x][3] * d1));
+          }
+          // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the group
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t a[4] = {minus136(nibbles(ta, 2 * u)), minus136(nibbles(ta, 2 * u + 1)), minus136(nibbles(tb2, 2 * u)),
+                                   minus136(nibbles(tb2, 2 * u + 1))};
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) mma16816(o[x][2 * g + u], a, b0[x], b1[x]);
+          }
+        }
+      }
+    }
+    __syncwarp();                                        // every lane has read the stage
+    issue(i + D * NW, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
+  }
+  copy_wait<0>();
+  __syncthreads();                                       // the ring is done with: the parts go over it
+  float* w_o = reinterpret_cast<float*>(ring_raw);       // [NW][nq][HD]
+  float* c_o = w_o + NW * 8 * NQ * HD;                   // [nq][HD]
+  float* w_m = c_o + 8 * NQ * HD;                        // [NW][16]
+  float* w_l = w_m + NW * 16;
+  float* c_m = w_l + NW * 16;                            // [16]
+  float* c_l = c_m + 16;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      l[x][0] += __shfl_xor_sync(0xffffffffu, l[x][0], d);
+      l[x][1] += __shfl_xor_sync(0xffffffffu, l[x][1], d);
+    }
+    if (quad == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { w_m[warp * 16 + 8 * x + 2 * qi + e] = m[x][e]; w_l[warp * 16 + 8 * x + 2 * qi + e] = l[x][e]; }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int query = 8 * x + 2 * qi + e;
+      if (query < nq) {
+#pragma unroll
+        for (int t = 0; t < 2 * GR; ++t)
+          *reinterpret_cast<float2*>(w_o + ((size_t)warp * 8 * NQ + query) * HD + 32 * (t >> 1) + 4 * quad + 2 * (t & 1)) =
+              make_float2(o[x][t][e], o[x][t][2 + e]);
+      }
+    }
+  }
+  __syncthreads();
+  bf16* out = (bf16*)p.out + (size_t)seq * p.out_stride + (size_t)h0 * HD;
+  auto finish = [](float O, float L) { return L > 0.f ? O / L : (L == L ? 0.f : L); };     // no visible key: zeros; a NaN stays one
+  for (int idx = threadIdx.x; idx < nq * HD; idx += THREADS) {
+    const int r = idx / HD, d = idx % HD;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, w_m[w * 16 + r]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // a part whose scores were all NaN has a maximum of -inf and a sum of NaN
+      const float mw = w_m[w * 16 + r], f = mw == -INFINITY ? 1.f : exp2f(mw - M);
+      L += w_l[w * 16 + r] * f;
+      O += w_o[((size_t)w * 8 * NQ + r) * HD + d] * f;
+    }
+    if (p.splits == 1) out[idx] = __float2bfloat16_rn(finish(O, L));
+    else {
+      c_o[idx] = O;
+      if (d == 0) { c_m[r] = M; c_l[r] = L; }
+    }
+  }
+  if (p.splits > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    const uint32_t ao = smem_u32(c_o), am = smem_u32(c_m), al = smem_u32(c_l);
+    // number idx is finished by the rank of its place among the ranges
+    for (int idx = threadIdx.x + rank * THREADS; idx < nq * HD; idx += THREADS * p.splits) {
+      const int r = idx / HD;
+      float M = -INFINITY, L = 0.f, O = 0.f;
+      for (int z = 0; z < p.splits; ++z) M = fmaxf(M, ld_cluster_f32(map_to_rank(am, z) + 4 * r));
+      for (int z = 0; z < p.splits; ++z) {
+        const float mz = ld_cluster_f32(map_to_rank(am, z) + 4 * r), f = mz == -INFINITY ? 1.f : exp2f(mz - M);
+        L += ld_cluster_f32(map_to_rank(al, z) + 4 * r) * f;
+        O += ld_cluster_f32(map_to_rank(ao, z) + 4 * idx) * f;
+      }
+      out[idx] = __float2bfloat16_rn(finish(O, L));
+    }
+    __syncwarp();
+    cluster_sync_all();                                  // nobody leaves while its shared memory is still read
+  }
+}
+
+template <int HD, int NQ>
+int launch_decode(const Kv4Params& p, cudaStream_t s) {
+  typedef DecCfg<HD> C;
+  static bool configured[64] = {};
+  if (allow_dynamic_smem(kv4_decode_kernel<HD, NQ>, C::RING, configured)) return -5;
+  const int G = p.nh / p.nkv;
+  const dim3 grid(p.nkv * ((G + 8 * NQ - 1) / (8 * NQ)), p.rows, p.splits);
+  if (grid.y > 65535) return ERR_TOO_LARGE;
+  return launch_ex(kv4_decode_kernel<HD, NQ>, grid, dim3(C::THREADS), C::RING, s, p.splits, p);
+}
+
 template <typename T>
 int launch_simt(const Kv4Params& p, int hd, cudaStream_t s) {
   const long long blocks = ((long long)p.rows * p.nh + WARPS - 1) / WARPS;
@@ -137,8 +506,28 @@ RLLM_API int rllm_kv4_attention_simt(int dt, const void* q, int q_stride, const 
   if (nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0) return ERR_BAD_SIZE;
   if (((uintptr_t)k4 | (uintptr_t)ks | (uintptr_t)v4 | (uintptr_t)vs) & 15) return ERR_BAD_ALIGN;
   const Kv4Params p = {q, q_stride, (const uint8_t*)k4, (const bf16*)ks, (const uint8_t*)v4, (const bf16*)vs, num_pages, out, out_stride,
-                       token_seq, positions, nullptr, block_table, bt_stride, T, nh, nkv, page_size, window, scale};
+                       token_seq, positions, nullptr, block_table, bt_stride, T, nh, nkv, page_size, window, scale, -1, 1};
   if (dt == DT_F32) return launch_simt<float>(p, hd, (cudaStream_t)stream);
   if (dt == DT_BF16) return launch_simt<bf16>(p, hd, (cudaStream_t)stream);
   return ERR_BAD_DTYPE;
+}
+
+// One bf16 query row per sequence: q [S, ...] with row stride q_stride (a multiple of 8, 16-byte aligned), head h at h * hd; out likewise.
+// kv_lens int32 [S]: keys that a sequence's token sees, its own included. splits: ranges of keys (1..8, the CTAs of a cluster).
+RLLM_API int rllm_kv4_decode(const void* q, int q_stride, const void* k4, const void* ks, const void* v4, const void* vs,
+                             long long num_pages, void* out, int out_stride, const int* kv_lens, const int* block_table,
+                             int bt_stride, int num_seqs, int nh, int nkv, int hd, int page_size, float scale, int window, int splits,
+                             void* stream) {
+  if (num_seqs <= 0) return 0;
+  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || splits < 1 || splits > 8 || !(scale > 0.f))
+    return ERR_BAD_SIZE;
+  if (num_pages * nkv * page_size > 2147483647LL) return ERR_TOO_LARGE;
+  if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)k4 | (uintptr_t)ks | (uintptr_t)v4 | (uintptr_t)vs) & 15)) return ERR_BAD_ALIGN;
+  int shift = -1;
+  for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) shift = b;
+  const Kv4Params p = {q, q_stride, (const uint8_t*)k4, (const bf16*)ks, (const uint8_t*)v4, (const bf16*)vs, num_pages, out, out_stride,
+                       nullptr, nullptr, kv_lens, block_table, bt_stride, num_seqs, nh, nkv, page_size, window, scale, shift, splits};
+  cudaStream_t s = (cudaStream_t)stream;
+  if (hd == 64) return nh / nkv <= 8 ? launch_decode<64, 1>(p, s) : launch_decode<64, 2>(p, s);
+  return nh / nkv <= 8 ? launch_decode<128, 1>(p, s) : launch_decode<128, 2>(p, s);
 }

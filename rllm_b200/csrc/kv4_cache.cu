@@ -95,47 +95,51 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Page i of sequence s goes to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind the
-// sequence's last token are zeros, and so are pages it does not hold. With `cu_q` (attention of portions) pages that no query
-// of the step sees are left out; table_out says which are there, cu_out counts the portions' rows from zero.
+// Places i * out_page .. of sequence s go to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind
+// the sequence's last token are zeros, and so are those in pages it does not hold. A CTA takes one kv head's part of a page. With `cu_q` (attention
+// of portions) pages that no query of the step sees are left out; table_out says which are there, cu_out counts the portions' rows
+// from zero.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 kv4_read_kernel(Pages c, long long num_pages, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ kv_lens,
-                const int* __restrict__ cu_q, int window, int num_seqs, int width, T* __restrict__ k, T* __restrict__ v,
+                const int* __restrict__ cu_q, int window, int num_seqs, int width, int out_page, T* __restrict__ k, T* __restrict__ v,
                 int* __restrict__ table_out, int* __restrict__ cu_out) {
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x, s = blockIdx.y;
-  const int n = kv_lens[s];
+  const bool is_v = (int)blockIdx.z >= c.nkv;
+  const int kvh = (int)blockIdx.z - (is_v ? c.nkv : 0);
+  const int n = kv_lens[s], j0 = i * out_page;
   int first = 0;                                         // the first position that a query sees
   if (cu_q != nullptr && window > 0) first = max(0, n - (cu_q[s + 1] - cu_q[s]) - window + 1);
-  const int page = i * c.page_size < n ? block_table[(size_t)s * bt_stride + i] : -1;
-  const bool held = page >= 0 && page < num_pages;
-  const bool left_out = table_out != nullptr && (!held || (i + 1) * c.page_size <= first);
-  if (threadIdx.x == 0) {
-    if (table_out != nullptr && blockIdx.z == 0) table_out[(size_t)s * width + i] = left_out ? -1 : s * width + i;
-    if (cu_out != nullptr && i == 0 && blockIdx.z == 0) { cu_out[s] = cu_q[s] - cu_q[0]; if (s == num_seqs - 1) cu_out[s + 1] = cu_q[s + 1] - cu_q[0]; }
+  const bool left_out = table_out != nullptr && (j0 >= n || j0 + out_page <= first);
+  if (threadIdx.x == 0 && blockIdx.z == 0) {
+    if (table_out != nullptr) table_out[(size_t)s * width + i] = left_out ? -1 : s * width + i;
+    if (cu_out != nullptr && i == 0) {
+      cu_out[s] = cu_q[s] - cu_q[0];
+      if (s == num_seqs - 1) cu_out[s + 1] = cu_q[s + 1] - cu_q[0];
+    }
   }
   if (left_out) return;
   const int blocks = c.hd >> 6, w = threadIdx.x & 7;
-  const int rows = c.nkv * c.page_size;                  // a page's rows, in the order in which they lie
-  const bool is_v = blockIdx.z;
   const uint8_t* src = is_v ? c.v4 : c.k4;
   const bf16* sc = is_v ? c.vs : c.ks;
-  T* dst = is_v ? v : k;
-  for (int u = threadIdx.x >> 3; u < rows * blocks; u += THREADS / 8) {
-    const int r = u / blocks, b = u - r * blocks;
-    const bool there = held && i * c.page_size + r % c.page_size < n;
+  T* dst = (is_v ? v : k) + (((size_t)s * width + i) * c.nkv + kvh) * out_page * c.hd;
+  const int* bt = block_table + (size_t)s * bt_stride;
+  for (int u = threadIdx.x >> 3; u < out_page * blocks; u += THREADS / 8) {
+    const int r = u / blocks, b = u - r * blocks, j = j0 + r;
     float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
-    if (there) {
-      const size_t row = (size_t)page * rows + r;
+    const int pg = j / c.page_size;
+    const int page = j < n ? bt[pg] : -1;
+    if (page >= 0 && page < num_pages) {
+      const size_t row = ((size_t)page * c.nkv + kvh) * c.page_size + (j - pg * c.page_size);
       const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(src + row * (c.hd >> 1)) + 8 * b + w);
       const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(sc + row * (c.hd >> 5)) + b);
       const float d0 = bf16_lo(two), d1 = bf16_hi(two);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { x0[e] = (float)code4(word, e) * d0; x1[e] = (float)code4(word, 4 + e) * d1; }
     }
-    T* o = dst + (((size_t)s * width + i) * rows + r) * c.hd + 64 * b + 4 * w;
+    T* o = dst + (size_t)r * c.hd + 64 * b + 4 * w;
     store4(o, x0);
     store4(o + 32, x1);
   }
@@ -173,25 +177,26 @@ RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk,
   return ERR_BAD_DTYPE;
 }
 
-// The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, page_size, hd] float or bf16 (rounded once). kv_lens int32
-// [num_seqs], block_table int32 with bt_stride >= width. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
+// The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, out_page, hd] float or bf16 (rounded once). kv_lens int32
+// [num_seqs], none above width * out_page; block_table int32 with an entry for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
 // [num_seqs + 1] for attention of portions, or null.
 RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
-                           const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, void* k, void* v,
-                           int* table_out, int* cu_out, int nkv, int page_size, int hd, void* stream) {
+                           const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, int out_page, void* k,
+                           void* v, int* table_out, int* cu_out, int nkv, int page_size, int hd, void* stream) {
   if (num_seqs <= 0 || width <= 0) return 0;
+  if (out_page <= 0 || 2 * nkv > 65535) return ERR_BAD_SIZE;
   Pages c;
   const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
   if (rc) return rc;
-  if (num_seqs > 65535 || (cu_out != nullptr && cu_q == nullptr) || (long long)num_seqs * width > 2147483647LL) return ERR_TOO_LARGE;
+  if (num_seqs > 65535 || (cu_out != nullptr && cu_q == nullptr) || (long long)num_seqs * width > 2147483647LL || (long long)width * out_page > 2147483647LL) return ERR_TOO_LARGE;
   if (((uintptr_t)k | (uintptr_t)v) & 15) return ERR_BAD_ALIGN;
   cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid(width, num_seqs, 2);
+  const dim3 grid(width, num_seqs, 2 * nkv);
   if (dt == DT_F32)
     return launch_ex(kv4_read_kernel<float>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
-                     num_seqs, width, (float*)k, (float*)v, table_out, cu_out);
+                     num_seqs, width, out_page, (float*)k, (float*)v, table_out, cu_out);
   if (dt == DT_BF16)
     return launch_ex(kv4_read_kernel<bf16>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
-                     num_seqs, width, (bf16*)k, (bf16*)v, table_out, cu_out);
+                     num_seqs, width, out_page, (bf16*)k, (bf16*)v, table_out, cu_out);
   return ERR_BAD_DTYPE;
 }

@@ -286,7 +286,7 @@ class Backend:
 
     def attention(self, q, cache, ctx, nh, scale, window):
         if "k4" in cache.tensors:
-            return self._quant.attention_kv4_simt(q, cache.tensors, ctx.token_seq, ctx.positions, cache.block_table, nh, scale, window)
+            return self._quant.attention_kv4(q, cache.tensors, ctx, cache.block_table, nh, scale, window, self.fast, self._or_none)
         if self._sm100 is not None:
             out = self._sm100.attention(q, cache, ctx, nh, scale, window)
             if out is not None:

@@ -19,8 +19,10 @@ ops.register_signatures("quant", {
     "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, c_int, _P],
     "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
-    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
+    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int,
                       _P],
+    "rllm_kv4_decode": [_P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                        c_int, _P],
     "rllm_kv4_attention_simt": [c_int, _P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
                                 c_int, c_float, c_int, _P],
 })
@@ -191,7 +193,7 @@ def kv4_read(tensors: dict, block_table: torch.Tensor, kv_lens: torch.Tensor, ma
     k, v = (torch.empty((S, width, nkv, page_size, hd), dtype=dtype, device=k4.device) for _ in range(2))
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops._dt(k, "k"), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr(),
-        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, k.data_ptr(), v.data_ptr(), None, None, nkv, page_size, hd,
+        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), None, None, nkv, page_size, hd,
         ops._stream()), "kv4_read")
     return k, v
 
@@ -215,4 +217,124 @@ def attention_kv4_simt(q: torch.Tensor, tensors: dict, token_seq: torch.Tensor, 
         ops._dt(q, "q"), q.data_ptr(), q.stride(0), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr(),
         out.stride(0), token_seq.data_ptr(), positions.data_ptr(), block_table.data_ptr(), block_table.stride(0), T, nh, nkv, hd,
         page_size, float(scale), int(window or 0), ops._stream()), "attention_kv4_simt")
+    return out
+
+
+DECODE_MAX_SPLITS = 8
+# Places of a key range's page in the scratch that portions are read into, and bytes of scratch a run of portions may take at once
+READ_PAGE, READ_BYTES = 128, 2 << 30
+
+
+def decode_splits(num_seqs: int, ctas: int, max_kv_len: int, sm_count: int, hd: int) -> int:
+    """Ranges the keys of a sequence are cut into (= CTAs of a cluster)."""
+    base, best, cost = max(1, num_seqs * ctas), 1, None
+    for s in range(1, DECODE_MAX_SPLITS + 1):
+        if s > 1 and max_kv_len < 128 * s:
+            break
+        c = -(-base * s // (2 * sm_count)) * (1150 + max_kv_len * hd / 128 / s) + 50 * s + (200 if s > 1 else 0)
+        if cost is None or c < cost:
+            best, cost = s, c
+    return best
+
+
+def decode_supported(q: torch.Tensor, hd: int, scale: float) -> bool:
+    """Does the tensor-core kernel for single tokens take these queries?"""
+    return q.dtype == torch.bfloat16 and hd in (64, 128) and scale > 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+
+
+def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
+                         window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: the most keys of a sequence;
+    `splits`: that many ranges of keys (1 to 8), None: by `decode_splits`."""
+    k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
+    S = kv_lens.numel()
+    _queries(q, nh, nkv, hd, S)
+    if not decode_supported(q, hd, scale):
+        raise ops.KernelError("attention_kv4_decode: bfloat16, heads of 64 or 128, rows of q on 16 bytes, a scale above 0")
+    _i32(kv_lens, "kv_lens", S)
+    _table(block_table, S)
+    G = nh // nkv
+    if splits is None:
+        seen = min(max_kv_len, window) if window else max_kv_len
+        splits = decode_splits(S, nkv * (-(-G // 8) if G <= 8 else -(-G // 16)), seen, sm100.init(q.device).sm_count, hd)
+    if out is None:
+        out = torch.empty((S, nh * hd), dtype=q.dtype, device=q.device)
+    ops._check(ops._fn("quant", "rllm_kv4_decode")(
+        q.data_ptr(), q.stride(0), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr(), out.stride(0),
+        kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), S, nh, nkv, hd, page_size, float(scale), int(window or 0),
+        int(splits), ops._stream()), "attention_kv4_decode")
+    return out
+
+
+def _runs(ctx) -> list:
+    """The step's sequences as runs of neighbours that bring one token each, or more: [(first, last + 1, first row, last row + 1, single,
+    longest portion, most keys)]. Worked out once a forward pass."""
+    runs = ctx.per_forward.get("kv4_runs")
+    if runs is None:
+        runs, row = [], 0
+        keys = ctx.kv_lens_host or [ctx.max_kv_len] * ctx.num_seqs
+        for s, (n, kv) in enumerate(zip(ctx.q_lens_host, keys)):
+            if runs and runs[-1][4] == (n == 1):
+                a, _, r, _, one, longest, most = runs[-1]
+                runs[-1] = (a, s + 1, r, row + n, one, max(longest, n), max(most, kv))
+            else:
+                runs.append((s, s + 1, row, row + n, n == 1, n, kv))
+            row += n
+        ctx.per_forward["kv4_runs"] = runs
+    return runs
+
+
+def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch) -> bool:
+    """Attention of a run of portions (bfloat16, heads of 64 or 128): the keys and values that they see are read into scratch as bfloat16
+    pages of READ_PAGE places, and the kernels of the cache of whole numbers attend over those. A portion's rows share the keys,
+    so the numbers are made once instead of in every row tile; what rounding them to bfloat16 costs is what a bfloat16 cache
+    costs. False where the memory left does not hold the scratch."""
+    s0, s1, r0, r1, _, longest, most = run
+    k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
+    S, width, T = s1 - s0, -(-most // READ_PAGE), r1 - r0
+    size = S * width * nkv * READ_PAGE * hd * 2
+    if S > 1 and 2 * size > READ_BYTES:            # one by one, then
+        row = r0
+        for s in range(s0, s1):
+            n = ctx.q_lens_host[s]
+            if not _portions(q, tensors, ctx, block_table, nh, scale, window, (s, s + 1, row, row + n, False, n, ctx.kv_lens_host[s]), out, scratch):
+                return False
+            row += n
+        return True
+    room = scratch(2 * size, lambda: torch.empty((2, S * width, nkv, READ_PAGE, hd), dtype=torch.bfloat16, device=q.device))
+    if room is None:
+        return False
+    meta = torch.empty(S * width + S + 1, dtype=torch.int32, device=q.device)
+    table, cu = meta[: S * width].view(S, width), meta[S * width:]
+    kv_lens, bt = ctx.kv_lens[s0:s1], block_table[s0:s1]
+    ops._check(ops._fn("quant", "rllm_kv4_read")(
+        ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, bt.data_ptr(), bt.stride(0), kv_lens.data_ptr(),
+        ctx.cu_q[s0:].data_ptr(), int(window or 0), S, width, READ_PAGE, room[0].data_ptr(), room[1].data_ptr(), table.data_ptr(),
+        cu.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
+    a = (q[r0:r1], room[0], room[1], cu, kv_lens, table)
+    if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(a[0], room[0]):
+        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out[r0:r1])
+    else:
+        sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out[r0:r1])
+    return True
+
+
+def attention_kv4(q: torch.Tensor, tensors: dict, ctx, block_table: torch.Tensor, nh: int, scale: float, window: int | None,
+                  fast: bool, scratch) -> torch.Tensor:
+    """A step's attention over keys and values held in 4 bits: single tokens and portions each in their kernel on the tensor cores
+    (`fast`), all else on the CUDA cores. `scratch(bytes, make)`: make(), or None where the memory left does not hold it."""
+    hd = 2 * tensors["k4"].shape[3]
+    simt = lambda: attention_kv4_simt(q, tensors, ctx.token_seq, ctx.positions, block_table, nh, scale, window)
+    if not fast or not decode_supported(q, hd, scale):
+        return simt()
+    if ctx.max_q_len == 1:
+        return attention_kv4_decode(q, tensors, ctx.kv_lens, block_table, nh, scale, window, ctx.max_kv_len)
+    _queries(q, nh, tensors["k4"].shape[1], hd, ctx.num_tokens)
+    out = torch.empty((q.shape[0], nh * hd), dtype=q.dtype, device=q.device)
+    for run in _runs(ctx):
+        s0, s1, r0, r1, single, _, most = run
+        if single:
+            attention_kv4_decode(q[r0:r1], tensors, ctx.kv_lens[s0:s1], block_table[s0:s1], nh, scale, window, most, out=out[r0:r1])
+        elif not _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch):
+            return simt()
     return out
