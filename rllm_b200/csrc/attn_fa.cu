@@ -19,6 +19,7 @@
 // portion also sees what earlier steps left in the cache.
 // Cache layout: [page][kv head][offset in page][HD].
 #include "common.cuh"
+#include <cuda_fp16.h>
 using namespace rllm;
 
 namespace {
@@ -49,6 +50,18 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same with weights and values in half precision.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -65,9 +78,13 @@ struct FaParams {
   float* part_ml;     // [(token * nh + head) * splits + z][2]
   long long part_rows;   // rows the two buffers above have: a row index beyond it (a cu_q that names more
                          // tokens than the caller said) is skipped, never written
+  // V16: values are half numbers times 2^e, with one e per page and kv head; a page is a multiple of BN keys
+  const int* vexp;       // [page * nkv + kv head]
 };
 
-template <int HD, int NWARPS>
+// V16: a value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
+// that meet the half values are those of the sum itself and stay within half's range; the denominator's part is given it back.
+template <int HD, int NWARPS, bool V16>
 __global__ void __launch_bounds__(NWARPS * 32)
 fa_paged_kernel(const FaParams p) {
   pdl_launch();
@@ -192,6 +209,9 @@ fa_paged_kernel(const FaParams p) {
     const int j0 = kv_begin + t * BN;
 
     if (w_active && j0 <= wpos_max && j0 + BN - 1 >= wlo_min) {
+      const int page_v = V16 ? bt[pshift >= 0 ? (j0 >> pshift) : j0 / p.page_size] : -1;
+      const int ve = V16 && page_v >= 0 ? p.vexp[page_v * p.nkv + kvh] : 0;
+      const float vef = (float)ve, vback = V16 ? __int_as_float((127 - ve) << 23) : 1.f;
       // ---- scores S = Q K^T : 16 rows x 64 keys; the K fragments of a k-step are fetched together
       float s[BN / 8][4];
 #pragma unroll
@@ -231,7 +251,7 @@ fa_paged_kernel(const FaParams p) {
       mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 2));
       // the running maximum lives in the exp2 domain (the scale is positive: it commutes with max)
       const float sl = p.scale_log2e;
-      const float mnA = fmaxf(mA, mxA * sl), mnB = fmaxf(mB, mxB * sl);
+      const float mnA = fmaxf(mA, V16 ? fmaf(mxA, sl, vef) : mxA * sl), mnB = fmaxf(mB, V16 ? fmaf(mxB, sl, vef) : mxB * sl);
       const float useA = (mnA == -INFINITY) ? 0.f : mnA, useB = (mnB == -INFINITY) ? 0.f : mnB;
       if (__any_sync(0xffffffffu, mnA != mA || mnB != mB)) {      // a new maximum somewhere: rescale
         const float corrA = fast_exp2(mA - useA), corrB = fast_exp2(mB - useB);     // exp2(-inf) = 0
@@ -241,6 +261,7 @@ fa_paged_kernel(const FaParams p) {
         mA = mnA; mB = mnB;
       }
       // ---- probabilities (as bf16 A fragments) and the weighted sum O += P V
+      const float offA = V16 ? vef - useA : -useA, offB = V16 ? vef - useB : -useB;
 #pragma unroll
       for (int kb = 0; kb < BN / 16; ++kb) {
         uint32_t vb[DTILES / 2][4];
@@ -248,19 +269,31 @@ fa_paged_kernel(const FaParams p) {
         for (int dp = 0; dp < DTILES / 2; ++dp) ldsm_addr_x4_trans(vb[dp], vt + voff[dp] + (uint32_t)(kb * 16 * HD * 2));
         uint32_t a[4];
         {
-          const float p0 = fast_exp2(fmaf(s[2 * kb][0], sl, -useA)), p1 = fast_exp2(fmaf(s[2 * kb][1], sl, -useA));
-          const float p2 = fast_exp2(fmaf(s[2 * kb][2], sl, -useB)), p3 = fast_exp2(fmaf(s[2 * kb][3], sl, -useB));
-          const float p4 = fast_exp2(fmaf(s[2 * kb + 1][0], sl, -useA)), p5 = fast_exp2(fmaf(s[2 * kb + 1][1], sl, -useA));
-          const float p6 = fast_exp2(fmaf(s[2 * kb + 1][2], sl, -useB)), p7 = fast_exp2(fmaf(s[2 * kb + 1][3], sl, -useB));
-          lA += p0 + p1 + p4 + p5;
-          lB += p2 + p3 + p6 + p7;
-          a[0] = pack_bf16(p0, p1); a[1] = pack_bf16(p2, p3);
-          a[2] = pack_bf16(p4, p5); a[3] = pack_bf16(p6, p7);
+          const float p0 = fast_exp2(fmaf(s[2 * kb][0], sl, offA)), p1 = fast_exp2(fmaf(s[2 * kb][1], sl, offA));
+          const float p2 = fast_exp2(fmaf(s[2 * kb][2], sl, offB)), p3 = fast_exp2(fmaf(s[2 * kb][3], sl, offB));
+          const float p4 = fast_exp2(fmaf(s[2 * kb + 1][0], sl, offA)), p5 = fast_exp2(fmaf(s[2 * kb + 1][1], sl, offA));
+          const float p6 = fast_exp2(fmaf(s[2 * kb + 1][2], sl, offB)), p7 = fast_exp2(fmaf(s[2 * kb + 1][3], sl, offB));
+          if (V16) {
+            lA = fmaf(p0 + p1 + p4 + p5, vback, lA);
+            lB = fmaf(p2 + p3 + p6 + p7, vback, lB);
+            a[0] = pack_f16(p0, p1); a[1] = pack_f16(p2, p3);
+            a[2] = pack_f16(p4, p5); a[3] = pack_f16(p6, p7);
+          } else {
+            lA += p0 + p1 + p4 + p5;
+            lB += p2 + p3 + p6 + p7;
+            a[0] = pack_bf16(p0, p1); a[1] = pack_bf16(p2, p3);
+            a[2] = pack_bf16(p4, p5); a[3] = pack_bf16(p6, p7);
+          }
         }
 #pragma unroll
         for (int dp = 0; dp < DTILES / 2; ++dp) {
-          mma_bf16(o[2 * dp], a, vb[dp][0], vb[dp][1]);
-          mma_bf16(o[2 * dp + 1], a, vb[dp][2], vb[dp][3]);
+          if (V16) {
+            mma_f16(o[2 * dp], a, vb[dp][0], vb[dp][1]);
+            mma_f16(o[2 * dp + 1], a, vb[dp][2], vb[dp][3]);
+          } else {
+            mma_bf16(o[2 * dp], a, vb[dp][0], vb[dp][1]);
+            mma_bf16(o[2 * dp + 1], a, vb[dp][2], vb[dp][3]);
+          }
         }
       }
     }
@@ -323,27 +356,27 @@ __global__ void fa_combine_kernel(const float* __restrict__ part_o, const float*
   }
 }
 
-template <int HD, int NWARPS>
+template <int HD, int NWARPS, bool V16>
 int launch_fa(const FaParams& p, int num_seqs, int max_rows, cudaStream_t s) {
   constexpr int BM = 16 * NWARPS;
   constexpr int SMEM = 4 * BN * HD * 2;
   static bool configured[64] = {};             // the attribute belongs to a device's copy of the kernel
-  if (allow_dynamic_smem(fa_paged_kernel<HD, NWARPS>, SMEM, configured)) return -5;
+  if (allow_dynamic_smem(fa_paged_kernel<HD, NWARPS, V16>, SMEM, configured)) return -5;
   dim3 grid((max_rows + BM - 1) / BM, p.nkv * p.splits, num_seqs);
   if (grid.y > 65535 || grid.z > 65535) return ERR_TOO_LARGE;
-  return launch_ex(fa_paged_kernel<HD, NWARPS>, grid, dim3(NWARPS * 32), SMEM, s, 1, p);
+  return launch_ex(fa_paged_kernel<HD, NWARPS, V16>, grid, dim3(NWARPS * 32), SMEM, s, 1, p);
 }
 
-}  // namespace
+template <int HD, bool V16>
+int launch_rows(const FaParams& p, int num_seqs, int max_rows, cudaStream_t s) {
+  return max_rows <= 16 ? launch_fa<HD, 1, V16>(p, num_seqs, max_rows, s) : launch_fa<HD, 4, V16>(p, num_seqs, max_rows, s);
+}
 
-// q: [T, ...] bf16 rows with stride q_stride, head h at h*hd; out likewise. cu_q [S+1], kv_lens [S],
-// block_table [S, bt_stride]. max_q_len: the longest portion in the batch (sizes the grid).
-// splits > 1 needs part_o [T*nh*splits*hd] and part_ml [T*nh*splits*2] floats of scratch.
-RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, const void* vcache, void* out,
-                               int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
-                               int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
-                               int hd, int page_size, float scale, int window, int splits, float* part_o,
-                               float* part_ml, void* stream) {
+int run_fa(const void* q, int q_stride, const void* kcache, const void* vcache, void* out,
+           int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
+           int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
+           int hd, int page_size, float scale, int window, int splits, float* part_o,
+           float* part_ml, const int* vexp, void* stream) {
   if (num_seqs <= 0 || num_tokens <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh % nkv || page_size <= 0) return ERR_BAD_SIZE;
   if (q_stride % 2 || out_stride % 2 || ((uintptr_t)q & 3) || ((uintptr_t)out & 3) ||
@@ -357,14 +390,13 @@ RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, 
   p.window = window; p.splits = splits; p.scale_log2e = scale * 1.4426950408889634f;
   p.page_shift = -1;
   if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
-  p.part_o = part_o; p.part_ml = part_ml;
+  p.part_o = part_o; p.part_ml = part_ml; p.vexp = vexp;
   p.part_rows = (long long)num_tokens * nh * splits;
   cudaStream_t s = (cudaStream_t)stream;
   const int G = nh / nkv;
   const int max_rows = max_q_len * G;
-  int rc;
-  if (max_rows <= 16) rc = hd == 64 ? launch_fa<64, 1>(p, num_seqs, max_rows, s) : launch_fa<128, 1>(p, num_seqs, max_rows, s);
-  else rc = hd == 64 ? launch_fa<64, 4>(p, num_seqs, max_rows, s) : launch_fa<128, 4>(p, num_seqs, max_rows, s);
+  const int rc = vexp ? (hd == 64 ? launch_rows<64, true>(p, num_seqs, max_rows, s) : launch_rows<128, true>(p, num_seqs, max_rows, s))
+                      : (hd == 64 ? launch_rows<64, false>(p, num_seqs, max_rows, s) : launch_rows<128, false>(p, num_seqs, max_rows, s));
   if (rc || splits == 1) return rc;
   const int blocks = num_tokens * nh;
   if (hd == 64)
@@ -372,6 +404,31 @@ RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, 
                      (const float*)part_ml, (bf16*)out, out_stride, nh, splits);
   return launch_ex(fa_combine_kernel<128>, dim3(blocks), dim3(128), 0, s, 1, (const float*)part_o,
                    (const float*)part_ml, (bf16*)out, out_stride, nh, splits);
+}
+
+}  // namespace
+
+// q: [T, ...] bf16 rows with stride q_stride, head h at h*hd; out likewise. cu_q [S+1], kv_lens [S],
+// block_table [S, bt_stride]. max_q_len: the longest portion in the batch (sizes the grid).
+// splits > 1 needs part_o [T*nh*splits*hd] and part_ml [T*nh*splits*2] floats of scratch.
+RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, const void* vcache, void* out,
+                               int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
+                               int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
+                               int hd, int page_size, float scale, int window, int splits, float* part_o,
+                               float* part_ml, void* stream) {
+  return run_fa(q, q_stride, kcache, vcache, out, out_stride, cu_q, kv_lens, block_table, bt_stride, num_seqs, num_tokens, max_q_len,
+                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, nullptr, stream);
+}
+
+// The same with values in half precision times 2^vexp[page * nkv + kv head]; pages of a multiple of 64 keys.
+RLLM_API int rllm_attention_fa_v16(const void* q, int q_stride, const void* kcache, const void* vcache, const int* vexp, void* out,
+                                   int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
+                                   int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
+                                   int hd, int page_size, float scale, int window, int splits, float* part_o,
+                                   float* part_ml, void* stream) {
+  if (!vexp || page_size <= 0 || page_size % BN) return ERR_BAD_SIZE;
+  return run_fa(q, q_stride, kcache, vcache, out, out_stride, cu_q, kv_lens, block_table, bt_stride, num_seqs, num_tokens, max_q_len,
+                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, vexp, stream);
 }
 
 // ------------------------------------------------------------------------------------------

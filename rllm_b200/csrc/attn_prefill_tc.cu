@@ -52,6 +52,7 @@
 // in an orderly way (TMEM freed).
 #include "common.cuh"
 #include "sm100.cuh"
+#include <cuda_fp16.h>
 #include <mutex>
 #include <type_traits>
 #include <unordered_map>
@@ -129,6 +130,8 @@ struct PfParams {
   const bf16* q2; long long q2_stride; int q2_head;
   const bf16* gate_h; int gate_h_ld, gate_cols;   // logits [T, gate_h_ld] or null: a column per head, or (gate_cols) per output
   float scale_log2e;
+  // HALF_V: values are half numbers times 2^e, one e per page and kv head: [page * nkv + kv head]; a page is a multiple of a tile's keys
+  const int* vexp;
   int* err;
 };
 
@@ -141,6 +144,10 @@ __device__ __forceinline__ float fast_exp2(float x) {          // exp2(-inf) = 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -203,7 +210,10 @@ __device__ __forceinline__ void softcap_poly2(uint32_t& x0, uint32_t& x1, float 
 // CAP: scores are bounded (p.cap).
 // MODE PLAIN: pages. CROSS: pages, every head over every kv head's values, float outputs (PfParams). DENSE: keys and values in
 // rows, by tensor copies of whole tiles.
-enum : int { PLAIN = 0, CROSS = 1, DENSE_ROWS = 2 };
+// HALF_V: pages whose values are half numbers times a power of two a page (PfParams); the weights that meet them are half numbers
+// too. A value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
+// are those of the sum itself and stay within half's range; the denominator's part is given it back.
+enum : int { PLAIN = 0, CROSS = 1, DENSE_ROWS = 2, HALF_V = 3 };
 template <int KD, int VD, bool TMA, bool CAP, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
@@ -326,7 +336,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   if constexpr (!SOFTMAX) {
   // ---- the products. Step k is (row tile g, K tile t); its S lands in accumulator acc_of(k, g), used for the turn_of(k, t)-th time.
   constexpr uint32_t id_s = idesc(PM, PN, false);
-  constexpr uint32_t id_pv = idesc(PM, 64, true);       // 64 output values at a time
+  // 64 output values at a time; HALF_V: both operands' type field says half
+  constexpr uint32_t id_pv = idesc(PM, 64, true) & (MODE == HALF_V ? ~((7u << 7) | (7u << 10)) : ~0u);
   auto step = [&](int k, int& g, int& t) {
     if (k < 2 * n_both) { g = k & 1; t = k >> 1; } else { g = g_long; t = n_both + (k - 2 * n_both); }
   };
@@ -571,6 +582,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const int j0 = tile_first(t);
       const int k = t < n_both ? 2 * t + g : 2 * n_both + (t - n_both);
       const int sa = BESIDE ? g : k % SB;
+      int ve = 0;                                          // the tile's values' power of two
+      if (MODE == HALF_V) {
+        const int page = p.block_table[(size_t)seq * p.bt_stride + (j0 >> p.page_shift)];
+        if (page >= 0) ve = p.vexp[page * p.nkv + kvh];
+      }
       const uint32_t s_addr = lane_addr + C::S_COL + (uint32_t)sa * PN;          // this step's S accumulator
       const uint32_t p_addr = BESIDE ? lane_addr + C::P_COL + (uint32_t)g * (PN / 2) : s_addr;
       if (!wait_on(&s_full[sa], (uint32_t)(BESIDE ? t : k / SB) & 1u, 24, t)) { ok = false; break; }
@@ -645,7 +661,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       float mx = mq[0];
 #pragma unroll
       for (int c = 1; c < NC; ++c) mx = fmaxf(mx, mq[c]);
-      const float cand = fmaxf(m, mx * sl);               // the scale is positive: it commutes with max
+      const float cand = fmaxf(m, MODE == HALF_V ? fmaf(mx, sl, (float)ve) : mx * sl);               // the scale is positive: it commutes with max
       const bool move = !sig && cand > m + 8.f;           // also the first visible key (m = -inf)
       float corr = 1.f;
       if (move) { corr = fast_exp2(m - cand); m = cand; l *= corr; }      // exp2(-inf) = 0
@@ -673,7 +689,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       // ---- exponentials, their sum, P as bf16 into the scores' place, two keys a column
       const float use = (m == -INFINITY) ? 0.f : m;
       // two scores an instruction where the pipe takes two: what bounds a step is the instructions its warps issue
-      const uint64_t sl2 = f32x2(sl, sl), use2 = f32x2(-use, -use);
+      const float off = MODE == HALF_V ? (float)ve - use : -use;
+      const uint64_t sl2 = f32x2(sl, sl), use2 = f32x2(off, off);
       uint64_t lq[4];                                     // eight partial sums side by side, added up in a fixed order
 #pragma unroll
       for (int i = 0; i < 4; ++i) lq[i] = f32x2(0.f, 0.f);
@@ -695,7 +712,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             split2(fma2(f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, use2), e0, e1);
             e0 = fast_exp2(e0); e1 = fast_exp2(e1);         // hidden keys hold -inf: 0
             lq[i & 3] = add2(lq[i & 3], f32x2(e0, e1));
-            pk[i] = pack_bf16(e0, e1);
+            pk[i] = MODE == HALF_V ? pack_f16(e0, e1) : pack_bf16(e0, e1);
           }
         }
         tmem_st16(p_addr + 16 * c, pk);
@@ -708,7 +725,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       float ls[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(lq[i], ls[2 * i], ls[2 * i + 1]);
-      l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+      const float lt = ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+      if (MODE == HALF_V) l = fmaf(lt, __int_as_float((127 - ve) << 23), l); else l += lt;
     }
     if (ok && wait_on(&pv_full[g], (uint32_t)(n_mine - 1) & 1u, 25, n_mine)) {
       tc_fence_after();
@@ -843,6 +861,7 @@ template <int HD, bool TMA>
 int launch_pf(const CUtensorMap& mk, const CUtensorMap& mv, const PfParams& p, int ctas, cudaStream_t s) {
   if constexpr (TMA) {
     if (p.cross) return launch_pf_c<HD, HD, true, false, CROSS>(mk, mv, mk, p, ctas, s);
+    if (p.vexp) return launch_pf_c<HD, HD, true, false, HALF_V>(mk, mv, mk, p, ctas, s);
   }
   return p.cap.c > 0.f ? launch_pf_c<HD, HD, TMA, true, PLAIN>(mk, mv, mk, p, ctas, s)
                        : launch_pf_c<HD, HD, TMA, false, PLAIN>(mk, mv, mk, p, ctas, s);
@@ -881,14 +900,14 @@ int multiprocessors(int asked, int& sms) {
 // max_q_len: the longest portion in the batch (sizes the list of work items). Head sizes 64 and 128.
 // chunk > 0: a query sees only the keys of its own block of `chunk` positions (blocks counted from position 0);
 // sinks: float [nh] or null; gate: float logits [T, gate_ld] or null (see PfParams); keep_first, sigmoid: see PfParams.
-// softcap > 0: bounded scores. cross, long_from: see PfParams. sm_count: CTAs to launch at most (0: asked from the device).
+// softcap > 0: bounded scores. cross, long_from, vexp (values in half precision, pages of a power of two from 128 keys): see PfParams. sm_count: CTAs to launch at most (0: asked from the device).
 RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* kcache, const void* vcache,
                                        void* out, int out_stride, const int* cu_q, const int* kv_lens,
                                        const int* block_table, int bt_stride, int num_seqs, int max_q_len,
                                        int num_pages, int nh, int nkv, int hd, int page_size, float scale, int window,
                                        int chunk, const float* sinks, const float* gate, int gate_ld,
-                                       int keep_first, int sigmoid, float softcap, int long_from, float* cross, int* err,
-                                       int sm_count, void* stream) {
+                                       int keep_first, int sigmoid, float softcap, int long_from, float* cross, const int* vexp,
+                                       int* err, int sm_count, void* stream) {
   if (num_seqs <= 0 || max_q_len <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || keep_first < 0 || scale <= 0.f)
     return ERR_BAD_SIZE;
@@ -896,8 +915,9 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
       ((uintptr_t)kcache & 15) || ((uintptr_t)vcache & 15)) return ERR_BAD_ALIGN;
   if (long_from > 0 && !cross) return ERR_BAD_SIZE;
   if (cross && (softcap > 0.f || sigmoid || gate || ((uintptr_t)cross & 15))) return ERR_BAD_SIZE;
+  if (vexp && (cross || softcap > 0.f || sigmoid || sinks || page_size % 128)) return ERR_BAD_SIZE;
   PfParams p = {};
-  p.long_from = long_from; p.cross = cross;
+  p.long_from = long_from; p.cross = cross; p.vexp = vexp;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.kc = (const bf16*)kcache; p.vc = (const bf16*)vcache;
   p.out = (bf16*)out; p.out_stride = out_stride; p.cu_q = cu_q; p.kv_lens = kv_lens;
   p.block_table = block_table; p.bt_stride = bt_stride; p.nh = nh; p.nkv = nkv; p.page_size = page_size;
@@ -926,7 +946,7 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
     if ((rc = cache_map(&mv, vcache, (long long)num_pages * nkv, page_size, hd, p.box_rows))) return rc;
     return hd == 64 ? launch_pf<64, true>(mk, mv, p, ctas, s) : launch_pf<128, true>(mk, mv, p, ctas, s);
   }
-  if (cross) return ERR_BAD_SIZE;                        // only where tensor copies bring the pages
+  if (cross || vexp) return ERR_BAD_SIZE;                // only where tensor copies bring the pages
   p.box_rows = 0;
   memset(&mk, 0, sizeof(mk));
   mv = mk;

@@ -4,6 +4,7 @@
 // each of its two groups a lane: the groups' largest numbers meet in three shuffles, a lane's eight codes are one word,
 // and the block's 32 bytes and its two scales leave as whole pieces.
 #include "quant.cuh"
+#include <cuda_fp16.h>
 
 using namespace rllm;
 
@@ -95,15 +96,22 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+__device__ __forceinline__ void store4h(void* p, const float (&v)[4]) {
+  const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
 // Places i * out_page .. of sequence s go to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind
 // the sequence's last token are zeros, and so are those in pages it does not hold. A CTA takes one kv head's part of a page. With `cu_q` (attention
 // of portions) pages that no query of the step sees are left out; table_out says which are there, cu_out counts the portions' rows
 // from zero.
+// vexp: the values are half numbers times 2^vexp[page * nkv + kv head], with the largest of the page's scales between 1 and 2 of these
+// powers. (A value has 12 significant bits: half numbers hold 11 of them, bfloat16 8.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 kv4_read_kernel(Pages c, long long num_pages, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ kv_lens,
                 const int* __restrict__ cu_q, int window, int num_seqs, int width, int out_page, T* __restrict__ k, T* __restrict__ v,
-                int* __restrict__ table_out, int* __restrict__ cu_out) {
+                int* __restrict__ table_out, int* __restrict__ cu_out, int* __restrict__ vexp) {
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x, s = blockIdx.y;
@@ -126,22 +134,44 @@ kv4_read_kernel(Pages c, long long num_pages, const int* __restrict__ block_tabl
   const bf16* sc = is_v ? c.vs : c.ks;
   T* dst = (is_v ? v : k) + (((size_t)s * width + i) * c.nkv + kvh) * out_page * c.hd;
   const int* bt = block_table + (size_t)s * bt_stride;
-  for (int u = threadIdx.x >> 3; u < out_page * blocks; u += THREADS / 8) {
-    const int r = u / blocks, b = u - r * blocks, j = j0 + r;
-    float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
-    const int pg = j / c.page_size;
+  // the row at place r, or -1: behind the last token, or on a page that is not held
+  auto row_of = [&](int r) -> long long {
+    const int j = j0 + r, pg = j / c.page_size;
     const int page = j < n ? bt[pg] : -1;
-    if (page >= 0 && page < num_pages) {
-      const size_t row = ((size_t)page * c.nkv + kvh) * c.page_size + (j - pg * c.page_size);
+    return page >= 0 && page < num_pages ? ((long long)page * c.nkv + kvh) * c.page_size + (j - pg * c.page_size) : -1;
+  };
+  const bool half = is_v && vexp != nullptr;
+  float down = 1.f;
+  if (half) {
+    __shared__ float red[32];
+    float mx = 0.f;
+    for (int u = threadIdx.x; u < out_page * blocks; u += THREADS) {
+      const int r = u / blocks, b = u - r * blocks;
+      const long long row = row_of(r);
+      if (row >= 0) {
+        const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(sc + row * (c.hd >> 5)) + b);
+        mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(two)), fabsf(bf16_hi(two))));      // (fmaxf drops a NaN)
+      }
+    }
+    mx = block_max(mx, red);
+    const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -100), 120) : 0;
+    if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = e;
+    down = __int_as_float((127 - e) << 23);
+  }
+  for (int u = threadIdx.x >> 3; u < out_page * blocks; u += THREADS / 8) {
+    const int r = u / blocks, b = u - r * blocks;
+    float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
+    const long long row = row_of(r);
+    if (row >= 0) {
       const uint32_t word = __ldcg(reinterpret_cast<const uint32_t*>(src + row * (c.hd >> 1)) + 8 * b + w);
       const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(sc + row * (c.hd >> 5)) + b);
-      const float d0 = bf16_lo(two), d1 = bf16_hi(two);
+      const float d0 = bf16_lo(two) * down, d1 = bf16_hi(two) * down;
 #pragma unroll
       for (int e = 0; e < 4; ++e) { x0[e] = (float)code4(word, e) * d0; x1[e] = (float)code4(word, 4 + e) * d1; }
     }
     T* o = dst + (size_t)r * c.hd + 64 * b + 4 * w;
-    store4(o, x0);
-    store4(o + 32, x1);
+    if (half) { store4h(o, x0); store4h(o + 32, x1); }
+    else { store4(o, x0); store4(o + 32, x1); }
   }
 }
 
@@ -179,12 +209,12 @@ RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk,
 
 // The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, out_page, hd] float or bf16 (rounded once). kv_lens int32
 // [num_seqs], none above width * out_page; block_table int32 with an entry for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
-// [num_seqs + 1] for attention of portions, or null.
+// [num_seqs + 1], and vexp [num_seqs * width, nkv] (bf16 only: v is then half numbers) for attention of portions, or null.
 RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
                            const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, int out_page, void* k,
-                           void* v, int* table_out, int* cu_out, int nkv, int page_size, int hd, void* stream) {
+                           void* v, int* table_out, int* cu_out, int* vexp, int nkv, int page_size, int hd, void* stream) {
   if (num_seqs <= 0 || width <= 0) return 0;
-  if (out_page <= 0 || 2 * nkv > 65535) return ERR_BAD_SIZE;
+  if (out_page <= 0 || 2 * nkv > 65535 || (vexp != nullptr && dt != DT_BF16)) return ERR_BAD_SIZE;
   Pages c;
   const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
   if (rc) return rc;
@@ -194,9 +224,9 @@ RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long 
   const dim3 grid(width, num_seqs, 2 * nkv);
   if (dt == DT_F32)
     return launch_ex(kv4_read_kernel<float>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
-                     num_seqs, width, out_page, (float*)k, (float*)v, table_out, cu_out);
+                     num_seqs, width, out_page, (float*)k, (float*)v, table_out, cu_out, vexp);
   if (dt == DT_BF16)
     return launch_ex(kv4_read_kernel<bf16>, grid, dim3(THREADS), 0, s, 1, c, num_pages, block_table, bt_stride, kv_lens, cu_q, window,
-                     num_seqs, width, out_page, (bf16*)k, (bf16*)v, table_out, cu_out);
+                     num_seqs, width, out_page, (bf16*)k, (bf16*)v, table_out, cu_out, vexp);
   return ERR_BAD_DTYPE;
 }
