@@ -9,13 +9,15 @@
 //     much, the accumulator starts at minus that. Codes and queries are exact in bfloat16, so a group's sum is as exact as float; it is
 //     multiplied by the group's scale as a float number. No dequantised key exists.
 //   * O^T = V^T P^T, dimensions on the rows: a value fragment pairs two keys' codes of one dimension, which is two words' halves put side by
-//     side. (128 + nibble) - 136 is exact here, where starting at a correction would not do: values cancel. The scale of a (key, group)
-//     goes onto the weight in float, before its one rounding to bfloat16; movmatrix turns the rounded weights from rows of keys into the
-//     columns that the second product takes.
+//     side. (1024 + nibble) - 1032 is exact in half precision, where starting at a correction would not do: values cancel. The scale of a
+//     (key, group) goes onto the weight in float, before its one rounding, to half precision (bfloat16 cost 0.0016 of the output's
+//     norm); so that the product stays in half's range, the running maximum is that of score + log2 of the key's largest value
+//     scale, weights themselves being float of any size. movmatrix turns the rounded weights from rows of keys into the columns
+//     that the second product takes.
 //   * Which key a row of the fragment stands for is free, as long as both products agree, and is chosen so that neither product's reads of
 //     shared memory meet a bank twice.
-//   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which float and bfloat16
-//     hold as well as 1, and the lanes' maxima meet once in a while instead of in every tile.
+//   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which is as good as 1, and
+//     the lanes' maxima meet once in a while instead of in every tile.
 //
 // On the CUDA cores, for any mix of prompt portions and single tokens, both run types and head sizes of 64, 128, 192 and 256: one
 // warp per (query token, query head), keys 32 at a time in position order with a running maximum and sum, all arithmetic in
@@ -24,6 +26,7 @@
 // byte of a row's block a lane, which is two neighbouring dimensions.
 #include "quant.cuh"
 #include "sm100.cuh"
+#include <cuda_fp16.h>
 
 using namespace rllm;
 using namespace sm100;
@@ -156,8 +159,14 @@ __device__ __forceinline__ float fast_exp2(float x) {              // exp2(-inf)
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -172,11 +181,15 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 }
 // Nibble i of both halves of a word as two bfloat16 numbers 128 + nibble.
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t minus136(uint32_t v) {
-  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&v);
-  const uint32_t c = 0x43084308u;                                  // 136, 136
-  const __nv_bfloat162 r = __hsub2(a, *reinterpret_cast<const __nv_bfloat162*>(&c));
+// Nibble i of both halves as two half numbers, nibble - 8.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, int i) {
+  const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, c = 0x64086408u;             // 1024 + nibble, 1032
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// floor(log2 x) of a float >= 0, not below -100 (weights then stay below 2^108, and a sum of 2^17 of them below 2^126)
+__device__ __forceinline__ float exponent_of(float x) {
+  return fmaxf(__int_as_float((__float_as_int(x) >> 23) | 0x4b000000) - 8388735.f, -100.f);
 }
 
 // A warp's tile is 4.5 KB whatever the head size, three of them a warp: 108 KB a CTA, two CTAs an SM.
@@ -339,10 +352,22 @@ kv4_decode_kernel(const Kv4Params p) {
         }
       }
       // ---- weights
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + C::SCALES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
+      float big[2];                                      // log2 of the largest value scale of rows quad and quad + 8
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = 0.f;
+#pragma unroll
+        for (int b = 0; b < BL; ++b) x = fmaxf(x, fmaxf(fabsf(bf16_lo(sc[e][b])), fabsf(bf16_hi(sc[e][b]))));      // (drops a NaN)
+        big[e] = exponent_of(x);
+      }
       float pr[NQ][4];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        float mx0 = fmaxf(s[x][0], s[x][2]) * sl, mx1 = fmaxf(s[x][1], s[x][3]) * sl;
+        float mx0 = fmaxf(fmaf(s[x][0], sl, big[0]), fmaf(s[x][2], sl, big[1])), mx1 = fmaxf(fmaf(s[x][1], sl, big[0]), fmaf(s[x][3], sl, big[1]));
         if (__any_sync(0xffffffffu, mx0 > m[x][0] + 8.f || mx1 > m[x][1] + 8.f)) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
@@ -364,10 +389,6 @@ kv4_decode_kernel(const Kv4Params p) {
       }
       // ---- values: the keys of columns 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + C::SCALES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
-#pragma unroll
       for (int b = 0; b < BL; ++b) {
         uint32_t w[4];
 #pragma unroll
@@ -386,10 +407,9 @@ kv4_decode_kernel(const Kv4Params p) {
           // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the group
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t a[4] = {minus136(nibbles(ta, 2 * u)), minus136(nibbles(ta, 2 * u + 1)), minus136(nibbles(tb2, 2 * u)),
-                                   minus136(nibbles(tb2, 2 * u + 1))};
+            const uint32_t a[4] = {codes_f16(ta, 2 * u), codes_f16(ta, 2 * u + 1), codes_f16(tb2, 2 * u), codes_f16(tb2, 2 * u + 1)};
 #pragma unroll
-            for (int x = 0; x < NQ; ++x) mma16816(o[x][2 * g + u], a, b0[x], b1[x]);
+            for (int x = 0; x < NQ; ++x) mma16816_f16(o[x][2 * g + u], a, b0[x], b1[x]);
           }
         }
       }
