@@ -3,17 +3,23 @@
 // Single tokens, heads of 64 and 128 in bfloat16 (kv4_decode_kernel): one pass over the codes, which stay codes until they are fragments of
 // mma.sync. A CTA has one (sequence, kv head, range of keys), a warp tiles of keys of its own, which per-lane
 // asynchronous copies bring into a ring; the ranges of a sequence form a cluster and meet in distributed shared memory.
-//   * S^T = K Q^T, keys on the rows (16 of them an instruction), the query heads of the kv head on the 8 columns: with the queries on the
-//     rows, 4 heads a kv head would fill a quarter of the instruction.
-//   * A number of the key fragment is bf16 128 + nibble, two of them by one AND-OR of a word; 136 sum(q) is what the products have too
-//     much, the accumulator starts at minus that. Codes and queries are exact in bfloat16, so a group's sum is as exact as float; it is
-//     multiplied by the group's scale as a float number. No dequantised key exists.
-//   * O^T = V^T P^T, dimensions on the rows: a value fragment pairs two keys' codes of one dimension, which is two words' halves put side by
-//     side. (1024 + nibble) - 1032 is exact in half precision, where starting at a correction would not do: values cancel. The scale of a
-//     (key, group) goes onto the weight in float, before its one rounding, to half precision (bfloat16 cost 0.0016 of the output's
-//     norm); so that the product stays in half's range, the running maximum is that of score + log2 of the key's largest value
-//     scale, weights themselves being float of any size. movmatrix turns the rounded weights from rows of keys into the columns
-//     that the second product takes.
+//   * S^T = K Q^T, keys on the rows (16 of them an instruction), 4 query heads of the kv head twice on the 8 columns: columns 0-3 take the
+//     first of a block's two groups of 32 dimensions, columns 4-7 the second. A word holds four codes of either group, so a pair of
+//     numbers that a fragment's register wants is a word's nibble i of both halves, as it lies there: the queries' fragment holds a
+//     zero for the group that is not its column's. Nothing is permuted, every column does work with 4 query heads a kv head, and each
+//     lane multiplies by one group's scale; the two groups' sums meet by one shuffle.
+//   * Fragments hold codes, exact half numbers: nibbles 0 and 1 of a half word are the last four bits of 1024 + n and four higher ones of 64 + n
+//     by one AND-OR each for two numbers, nibbles 2 and 3 the same after a shift by 8; less 1032 and 72 they are the codes. (In bfloat16, with 7 bits
+//     behind the first, three of the four nibbles would want a shift; the pipe of shifts, ANDs and permutations is what bounds this
+//     kernel: with those and with pairs put together from two words, 64 sequences of 4,096 keys, 8 x 128, took 115 us.) Queries are half numbers
+//     times a power of two a row, which is exact down to 2^-14 of the row's largest. A group's sum is as exact as float; it is multiplied
+//     by the group's scale as a float number. No dequantised key exists.
+//   * O^T = V^T P^T, dimensions within a group on the rows; the contraction is over (key, group) pairs, so that a register is again a word's
+//     nibble of both halves, and a column's weights are zero for the group that is not its own: columns 0-3 become the
+//     output's first 32 dimensions of a block, columns 4-7 the second. The scale of a (key, group) goes onto the weight in float, before its
+//     one rounding, to half precision (bfloat16 cost 0.0016 of the output's norm); so that the product stays in half's range, the running
+//     maximum is that of score + log2 of the key's largest value scale, weights themselves being float of any size. movmatrix
+//     turns the rounded weights from rows of keys into the columns that the second product takes.
 //   * Which key a row of the fragment stands for is free, as long as both products agree, and is chosen so that neither product's reads of
 //     shared memory meet a bank twice.
 //   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which is as good as 1, and
@@ -136,12 +142,6 @@ kv4_attention_simt_kernel(const Kv4Params p) {
 }
 
 // ---------------------------------------------------------------------------- single tokens
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {          // an 8 x 8 matrix of 16-bit numbers, rows to columns
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -159,11 +159,17 @@ __device__ __forceinline__ float fast_exp2(float x) {              // exp2(-inf)
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {     // nothing to add to
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -179,13 +185,23 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-// Nibble i of both halves of a word as two bfloat16 numbers 128 + nibble.
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-// Nibble i of both halves as two half numbers, nibble - 8.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w, int i) {
-  const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, c = 0x64086408u;             // 1024 + nibble, 1032
+__device__ __forceinline__ uint32_t less(uint32_t v, uint32_t c) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// (a & mask) | bits, one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
+// The codes of the four nibbles of both halves of a word: two half numbers each.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&c)[4]) {
+  const uint32_t v = w >> 8;
+  c[0] = less(and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u);   // 1024 + n, 1032
+  c[1] = less(and_or(w, 0x00f000f0u, 0x54005400u), 0x54805480u);   // 64 + n, 72
+  c[2] = less(and_or(v, 0x000f000fu, 0x64006400u), 0x64086408u);
+  c[3] = less(and_or(v, 0x00f000f0u, 0x54005400u), 0x54805480u);
 }
 // floor(log2 x) of a float >= 0, not below -100 (weights then stay below 2^108, and a sum of 2^17 of them below 2^126)
 __device__ __forceinline__ float exponent_of(float x) {
@@ -209,9 +225,9 @@ template <int HD> __device__ __forceinline__ uint32_t code_off(int r, int ch) {
   return HD == 128 ? (uint32_t)(r * 64 + ((ch ^ ((((r >> 1) ^ (r >> 2)) & 1) << 1)) << 4)) : (uint32_t)((r ^ (((r >> 2) & 1) << 1)) * 32 + (ch << 4));
 }
 
-// NQ: groups of 8 query heads a CTA
+// NQ: groups of 4 query heads a CTA
 template <int HD, int NQ>
-__global__ void __launch_bounds__(256, NQ == 1 ? 2 : 1)
+__global__ void __launch_bounds__(256, NQ <= 2 ? 2 : 1)
 kv4_decode_kernel(const Kv4Params p) {
   typedef DecCfg<HD> C;
   constexpr int NW = C::NW, D = C::D, TILE = C::TILE, THREADS = C::THREADS;
@@ -219,10 +235,10 @@ kv4_decode_kernel(const Kv4Params p) {
   constexpr int CPR = HD / 32;                           // 16-byte pieces of a row's codes
   extern __shared__ __align__(128) uint8_t ring_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, qi = lane & 3;
-  const int G = p.nh / p.nkv, qgroups = (G + 8 * NQ - 1) / (8 * NQ);
+  const int G = p.nh / p.nkv, qgroups = (G + 4 * NQ - 1) / (4 * NQ);
   const int kvh = blockIdx.x / qgroups, seq = blockIdx.y;
-  const int h0 = kvh * G + blockIdx.x % qgroups * (8 * NQ);        // first query head
-  const int nq = min(8 * NQ, kvh * G + G - h0);
+  const int h0 = kvh * G + blockIdx.x % qgroups * (4 * NQ);        // first query head
+  const int nq = min(4 * NQ, kvh * G + G - h0);
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
   pdl_launch();
   pdl_wait();                                            // the kernel in front may have written any of the cache
@@ -236,113 +252,168 @@ kv4_decode_kernel(const Kv4Params p) {
   const int* bt = p.block_table + (size_t)seq * p.bt_stride;
   const uint32_t base = smem_u32(ring_raw), ring = base + (uint32_t)(warp * D) * C::STAGE;
 
+  // What a lane's copies share is worked out once: piece `lane % CPR` of every (32 / CPR)-th key row, and a key's scales.
+  const int ch = lane % CPR;
+  const uint8_t* k4 = p.k4 + 16 * ch;
+  const uint8_t* v4 = p.v4 + 16 * ch;
+  const uint32_t dst0 = ring + code_off<HD>(lane / CPR, ch), dst1 = ring + 2 * C::CODES + lane * (HD / 16);
+  // The pages of this lane's keys in tile i, -1 where there is no key; asked for a tile ahead of the copies.
+  int page[TILE / 32];
+  auto look_up = [&](int i) {
+    const int j0 = (tb + i) * TILE;
+#pragma unroll
+    for (int h = 0; h < TILE / 32; ++h) {
+      const int j = j0 + 32 * h + lane;
+      page[h] = i < n_tiles && j >= lo && j <= pos ? bt[p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size] : -1;
+    }
+  };
   // Starts the copies of this warp's tile i and closes a copy group, also when there is no such tile, so that the groups can be counted.
   auto issue = [&](int i, int slot) {
     if (i < n_tiles) {
-      const uint32_t st = ring + (uint32_t)slot * C::STAGE;
+      const uint32_t st = (uint32_t)slot * C::STAGE;
       const int j0 = (tb + i) * TILE;
-      int row[TILE / 32];                                // a lane finds the rows of its keys, the others ask it
+      int row[TILE / 32];                                // a lane has the rows of its keys, the others ask it
+      bool all = true;
 #pragma unroll
       for (int h = 0; h < TILE / 32; ++h) {
         const int j = j0 + 32 * h + lane;
-        row[h] = -1;
-        if (j >= lo && j <= pos) {
-          const int pg = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
-          const int page = __ldcg(bt + pg);
-          if (page >= 0 && page < p.num_pages) row[h] = (page * p.nkv + kvh) * p.page_size + (j - pg * p.page_size);
-        }
-        const size_t r = row[h] < 0 ? 0 : row[h];
-        copy_async<HD / 16>(st + 2 * C::CODES + (32 * h + lane) * (HD / 16), p.ks + r * GR, row[h] >= 0);
-        copy_async<HD / 16>(st + 2 * C::CODES + C::SCALES + (32 * h + lane) * (HD / 16), p.vs + r * GR, row[h] >= 0);
+        const int off = p.page_shift >= 0 ? j & (p.page_size - 1) : j % p.page_size;
+        row[h] = page[h] >= 0 && page[h] < p.num_pages ? (page[h] * p.nkv + kvh) * p.page_size + off : -1;
+        all = all && row[h] >= 0;
       }
+      all = __all_sync(0xffffffffu, all);
+      // (two loops: in the one that runs the lengths are constants)
+      auto copies = [&](bool known) {
 #pragma unroll
-      for (int c = 0; c < TILE * CPR / 32; ++c) {
-        const int key = (c * 32 + lane) / CPR, ch = lane % CPR;
-        const int r = __shfl_sync(0xffffffffu, row[c * 32 / CPR / 32], key & 31);
-        const size_t src = (size_t)(r < 0 ? 0 : r) * (HD / 2) + 16 * ch;
-        const uint32_t dst = st + code_off<HD>(key, ch);
-        copy_async<16>(dst, p.k4 + src, r >= 0);
-        copy_async<16>(dst + C::CODES, p.v4 + src, r >= 0);
-      }
+        for (int h = 0; h < TILE / 32; ++h) {
+          const bool there = known || row[h] >= 0;
+          const uint32_t r = there ? row[h] : 0;
+          copy_async<HD / 16>(dst1 + st + 32 * h * (HD / 16), p.ks + (size_t)r * GR, there);
+          copy_async<HD / 16>(dst1 + st + C::SCALES + 32 * h * (HD / 16), p.vs + (size_t)r * GR, there);
+        }
+#pragma unroll
+        for (int c = 0; c < TILE * CPR / 32; ++c) {
+          const int r = __shfl_sync(0xffffffffu, row[c * 32 / CPR / 32], (c * 32 / CPR + lane / CPR) & 31);
+          const bool there = known || r >= 0;
+          const size_t src = (size_t)(uint32_t)(there ? r : 0) * (HD / 2);
+          copy_async<16>(dst0 + st + c * 512, k4 + src, there);
+          copy_async<16>(dst0 + st + C::CODES + c * 512, v4 + src, there);
+        }
+      };
+      if (all) copies(true); else copies(false);
     }
     copy_commit();
+    look_up(i + NW);
   };
+  look_up(warp);
 #pragma unroll
   for (int d = 0; d < D; ++d) issue(warp + d * NW, d);
 
-  // the queries as fragments: lane (quad, qi) has numbers 8 qi .. 8 qi + 7 of each group of query `quad`; in a step of 16 numbers go
-  // number 2s of both its words (pairs i, i + 4), then 2s + 1
-  uint32_t qf[NQ][GR][2][2];
-  float qsum[NQ][GR][2];                                 // -136 sum(q) of queries 2 qi and 2 qi + 1
+  // The queries as fragments: lane (quad, qi) has numbers 8 qi .. 8 qi + 7 of group quad / 4 of each block of query quad % 4; in step t
+  // of a block go numbers t and t + 4, in the half of the register that the group's codes have, the other half zero.
+  const int hi_cols = quad >> 2;
+  uint32_t qf[NQ][BL][4][2];
+  float sl[NQ][2];                                       // scale, log2 e and the power of two of the queries of columns 2 qi and 2 qi + 1
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
-    const bool live = 8 * x + quad < nq;
-    const bf16* qp = (const bf16*)p.q + (size_t)seq * p.q_stride + (size_t)(h0 + (live ? 8 * x + quad : 0)) * HD + 8 * qi;
+    const bool live = 4 * x + (quad & 3) < nq;
+    const bf16* qp = (const bf16*)p.q + (size_t)seq * p.q_stride + (size_t)(h0 + (live ? 4 * x + (quad & 3) : 0)) * HD + 32 * hi_cols + 8 * qi;
+    uint4 v[BL];
+    float big = 0.f;
 #pragma unroll
-    for (int g = 0; g < GR; ++g) {
-      uint4 v = live ? __ldcg(reinterpret_cast<const uint4*>(qp + 32 * g)) : make_uint4(0u, 0u, 0u, 0u);
-      qf[x][g][0][0] = __byte_perm(v.x, v.z, 0x5410); qf[x][g][0][1] = __byte_perm(v.x, v.z, 0x7632);
-      qf[x][g][1][0] = __byte_perm(v.y, v.w, 0x5410); qf[x][g][1][1] = __byte_perm(v.y, v.w, 0x7632);
-      const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      mma16816(c, ones, qf[x][g][0][0], qf[x][g][0][1]);
-      mma16816(c, ones, qf[x][g][1][0], qf[x][g][1][1]);
-      qsum[x][g][0] = -136.f * c[0]; qsum[x][g][1] = -136.f * c[1];
+    for (int b = 0; b < BL; ++b) {
+      v[b] = live ? __ldcg(reinterpret_cast<const uint4*>(qp + 64 * b)) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t w[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+    const int e = (int)fminf(exponent_of(big), 100.f);
+    const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23) * p.scale * 1.4426950408889634f;
+    sl[x][0] = __shfl_sync(0xffffffffu, up, 8 * (qi & 1));
+    sl[x][1] = __shfl_sync(0xffffffffu, up, 8 * (qi & 1) + 4);
+#pragma unroll
+    for (int b = 0; b < BL; ++b) {
+      const uint32_t w[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float f = (t & 1 ? bf16_hi(w[2 * u + (t >> 1)]) : bf16_lo(w[2 * u + (t >> 1)])) * down;
+          qf[x][b][t][u] = hi_cols ? pack2(0.f, f) : pack2(f, 0.f);
+        }
     }
   }
 
-  float o[NQ][2 * GR][4];                                // rows: dimensions (see below), columns: queries 2 qi, 2 qi + 1
+  float o[NQ][2 * BL][4];                                // [block, half of a group]: rows dimensions, columns queries (see below)
   float m[NQ][2], l[NQ][2];
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
 #pragma unroll
-    for (int i = 0; i < 2 * GR; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+    for (int i = 0; i < 2 * BL; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
     m[x][0] = m[x][1] = -INFINITY;
     l[x][0] = l[x][1] = 0.f;
   }
-  const float sl = p.scale * 1.4426950408889634f;
+  // a scale of this lane's columns' group out of the two, as float; where the weights of the keys 2 qi and 2 qi + 1 go
+  const uint32_t pick = qi & 2 ? 0x3244u : 0x1044u, put0 = hi_cols ? 0x1044u : 0x4410u, put1 = hi_cols ? 0x3244u : 0x4432u;
+  auto scale_of = [&](uint32_t two) { return __uint_as_float(__byte_perm(two, 0u, pick)); };
   // row r of a fragment is key (r & 7) / 2 + 4 (r & 1) + (r & 8)
   const int krow = (quad >> 1) + 4 * (quad & 1);
+  // this lane's places in a stage: both rows' codes (words 2 qi, 2 qi + 1 of a block), the value words of its four keys, the scales. A fragment's
+  // keys are 16 rows on from the one before, which changes nothing in where pieces lie within a row.
+  uint32_t ka[BL], va[BL], vb[BL];
+#pragma unroll
+  for (int b = 0; b < BL; ++b) {
+    ka[b] = ring + code_off<HD>(krow, 2 * b + (qi >> 1)) + 8 * (qi & 1);
+    va[b] = ring + C::CODES + code_off<HD>(qi, 2 * b + (quad >> 2)) + 4 * (quad & 3);
+    vb[b] = ring + C::CODES + code_off<HD>(qi + 4, 2 * b + (quad >> 2)) + 4 * (quad & 3);
+  }
+  constexpr int ROW = HD / 2;
+  const uint32_t sa = ring + 2 * C::CODES + krow * (HD / 16);
   int slot = 0;
   for (int i = warp; i < n_tiles; i += NW) {
     copy_wait<D - 1>();                                  // this warp's oldest group, tile i, has landed
     __syncwarp();
-    const uint32_t st = ring + (uint32_t)slot * C::STAGE;
+    const uint32_t st = (uint32_t)slot * C::STAGE;
     const int j0 = (tb + i) * TILE;
     const bool edge = j0 < lo || j0 + TILE - 1 > pos;
-#pragma unroll 1
+#pragma unroll
     for (int sub = 0; sub < TILE / 16; ++sub) {
       const int k0 = 16 * sub;
       float s[NQ][4];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-      // ---- scores, group by group
+      // ---- scores, block by block
       uint32_t sc[2][BL];                                // the scales of rows quad and quad + 8
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
+        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(sa + st + (k0 + 8 * e) * (HD / 16) + 4 * b);
 #pragma unroll
       for (int b = 0; b < BL; ++b) {
-        const uint2 wa = lds64(st + code_off<HD>(k0 + krow, 2 * b + (qi >> 1)) + 8 * (qi & 1));
-        const uint2 wb = lds64(st + code_off<HD>(k0 + krow + 8, 2 * b + (qi >> 1)) + 8 * (qi & 1));
+        const uint2 wa = lds64(ka[b] + st + k0 * ROW), wb = lds64(ka[b] + st + (k0 + 8) * ROW);
+        uint32_t c0[4], c1[4], c2[4], c3[4];
+        codes_f16(wa.x, c0); codes_f16(wb.x, c1); codes_f16(wa.y, c2); codes_f16(wb.y, c3);
+        const float d0 = scale_of(sc[0][b]), d1 = scale_of(sc[1][b]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t ta = __byte_perm(wa.x, wa.y, h ? 0x7632 : 0x5410), tb2 = __byte_perm(wb.x, wb.y, h ? 0x7632 : 0x5410);
-          const uint32_t a0[4] = {nibbles(ta, 0), nibbles(tb2, 0), nibbles(ta, 1), nibbles(tb2, 1)};
-          const uint32_t a1[4] = {nibbles(ta, 2), nibbles(tb2, 2), nibbles(ta, 3), nibbles(tb2, 3)};
-          const float d0 = h ? bf16_hi(sc[0][b]) : bf16_lo(sc[0][b]), d1 = h ? bf16_hi(sc[1][b]) : bf16_lo(sc[1][b]);
+        for (int x = 0; x < NQ; ++x) {
+          float c[4];
 #pragma unroll
-          for (int x = 0; x < NQ; ++x) {
-            const int g = 2 * b + h;
-            float c[4] = {qsum[x][g][0], qsum[x][g][1], qsum[x][g][0], qsum[x][g][1]};
-            mma16816(c, a0, qf[x][g][0][0], qf[x][g][0][1]);
-            mma16816(c, a1, qf[x][g][1][0], qf[x][g][1][1]);
-            s[x][0] = fmaf(d0, c[0], s[x][0]); s[x][1] = fmaf(d0, c[1], s[x][1]);
-            s[x][2] = fmaf(d1, c[2], s[x][2]); s[x][3] = fmaf(d1, c[3], s[x][3]);
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t a[4] = {c0[t], c1[t], c2[t], c3[t]};
+            if (t == 0) mma16816_first(c, a, qf[x][b][t][0], qf[x][b][t][1]);
+            else mma16816(c, a, qf[x][b][t][0], qf[x][b][t][1]);
           }
+          s[x][0] = fmaf(d0, c[0], s[x][0]); s[x][1] = fmaf(d0, c[1], s[x][1]);
+          s[x][2] = fmaf(d1, c[2], s[x][2]); s[x][3] = fmaf(d1, c[3], s[x][3]);
         }
       }
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][e] += __shfl_xor_sync(0xffffffffu, s[x][e], 2);      // the other group's columns
       if (edge) {
         const int ja = j0 + k0 + krow, jb = ja + 8;
 #pragma unroll
@@ -355,7 +426,7 @@ kv4_decode_kernel(const Kv4Params p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(st + 2 * C::CODES + C::SCALES + (k0 + krow + 8 * e) * (HD / 16) + 4 * b);
+        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(sa + st + C::SCALES + (k0 + 8 * e) * (HD / 16) + 4 * b);
       float big[2];                                      // log2 of the largest value scale of rows quad and quad + 8
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -367,7 +438,9 @@ kv4_decode_kernel(const Kv4Params p) {
       float pr[NQ][4];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        float mx0 = fmaxf(fmaf(s[x][0], sl, big[0]), fmaf(s[x][2], sl, big[1])), mx1 = fmaxf(fmaf(s[x][1], sl, big[0]), fmaf(s[x][3], sl, big[1]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][e] *= sl[x][e & 1];
+        float mx0 = fmaxf(s[x][0] + big[0], s[x][2] + big[1]), mx1 = fmaxf(s[x][1] + big[0], s[x][3] + big[1]);
         if (__any_sync(0xffffffffu, mx0 > m[x][0] + 8.f || mx1 > m[x][1] + 8.f)) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
@@ -379,37 +452,34 @@ kv4_decode_kernel(const Kv4Params p) {
           m[x][0] = mx0; m[x][1] = mx1;
           l[x][0] *= c0; l[x][1] *= c1;
 #pragma unroll
-          for (int t = 0; t < 2 * GR; ++t) { o[x][t][0] *= c0; o[x][t][1] *= c1; o[x][t][2] *= c0; o[x][t][3] *= c1; }
+          for (int t = 0; t < 2 * BL; ++t) { o[x][t][0] *= c0; o[x][t][1] *= c1; o[x][t][2] *= c0; o[x][t][3] *= c1; }
         }
         const float u0 = m[x][0] == -INFINITY ? 0.f : m[x][0], u1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
-        pr[x][0] = fast_exp2(fmaf(s[x][0], sl, -u0)); pr[x][1] = fast_exp2(fmaf(s[x][1], sl, -u1));
-        pr[x][2] = fast_exp2(fmaf(s[x][2], sl, -u0)); pr[x][3] = fast_exp2(fmaf(s[x][3], sl, -u1));
+        pr[x][0] = fast_exp2(s[x][0] - u0); pr[x][1] = fast_exp2(s[x][1] - u1);
+        pr[x][2] = fast_exp2(s[x][2] - u0); pr[x][3] = fast_exp2(s[x][3] - u1);
         l[x][0] += pr[x][0] + pr[x][2];
         l[x][1] += pr[x][1] + pr[x][3];
       }
-      // ---- values: the keys of columns 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
+      // ---- values: the keys of weights 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
 #pragma unroll
       for (int b = 0; b < BL; ++b) {
-        uint32_t w[4];
+        const float d0 = scale_of(sc[0][b]), d1 = scale_of(sc[1][b]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = lds32(st + C::CODES + code_off<HD>(k0 + qi + 4 * e, 2 * b + (quad >> 2)) + 4 * (quad & 3));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t ta = __byte_perm(w[0], w[1], h ? 0x7632 : 0x5410), tb2 = __byte_perm(w[2], w[3], h ? 0x7632 : 0x5410);
-          const int g = 2 * b + h;
-          const float d0 = h ? bf16_hi(sc[0][b]) : bf16_lo(sc[0][b]), d1 = h ? bf16_hi(sc[1][b]) : bf16_lo(sc[1][b]);
-          uint32_t b0[NQ], b1[NQ];
+        for (int e = 0; e < 2; ++e) {                    // rows 0-7, then 8-15
+          uint32_t ca[4], cb[4];
+          codes_f16(lds32(va[b] + st + (k0 + 8 * e) * ROW), ca);
+          codes_f16(lds32(vb[b] + st + (k0 + 8 * e) * ROW), cb);
 #pragma unroll
           for (int x = 0; x < NQ; ++x) {
-            b0[x] = turn8x8(pack2(pr[x][0] * d0, pr[x][1] * d0));
-            b1[x] = turn8x8(pack2(pr[x][2] * d1, pr[x][3] * d1));
-          }
-          // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the group
+            const float d = e ? d1 : d0;
+            const uint32_t w = turn8x8(pack2(pr[x][2 * e] * d, pr[x][2 * e + 1] * d));
+            const uint32_t b0 = __byte_perm(w, 0u, put0), b1 = __byte_perm(w, 0u, put1);
+            // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the columns' group
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t a[4] = {codes_f16(ta, 2 * u), codes_f16(ta, 2 * u + 1), codes_f16(tb2, 2 * u), codes_f16(tb2, 2 * u + 1)};
-#pragma unroll
-            for (int x = 0; x < NQ; ++x) mma16816_f16(o[x][2 * g + u], a, b0[x], b1[x]);
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a[4] = {ca[2 * u], ca[2 * u + 1], cb[2 * u], cb[2 * u + 1]};
+              mma16816(o[x][2 * b + u], a, b0, b1);
+            }
           }
         }
       }
@@ -420,9 +490,9 @@ kv4_decode_kernel(const Kv4Params p) {
   }
   copy_wait<0>();
   __syncthreads();                                       // the ring is done with: the parts go over it
-  float* w_o = reinterpret_cast<float*>(ring_raw);       // [NW][nq][HD]
-  float* c_o = w_o + NW * 8 * NQ * HD;                   // [nq][HD]
-  float* w_m = c_o + 8 * NQ * HD;                        // [NW][16]
+  float* w_o = reinterpret_cast<float*>(ring_raw);       // [NW][4 NQ][HD]
+  float* c_o = w_o + NW * 4 * NQ * HD;                   // [4 NQ][HD]
+  float* w_m = c_o + 4 * NQ * HD;                        // [NW][16]
   float* w_l = w_m + NW * 16;
   float* c_m = w_l + NW * 16;                            // [16]
   float* c_l = c_m + 16;
@@ -433,17 +503,14 @@ kv4_decode_kernel(const Kv4Params p) {
       l[x][0] += __shfl_xor_sync(0xffffffffu, l[x][0], d);
       l[x][1] += __shfl_xor_sync(0xffffffffu, l[x][1], d);
     }
-    if (quad == 0) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) { w_m[warp * 16 + 8 * x + 2 * qi + e] = m[x][e]; w_l[warp * 16 + 8 * x + 2 * qi + e] = l[x][e]; }
-    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int query = 8 * x + 2 * qi + e;
+      const int query = 4 * x + ((2 * qi + e) & 3);
+      if (lane < 2) { w_m[warp * 16 + query] = m[x][e]; w_l[warp * 16 + query] = l[x][e]; }
       if (query < nq) {
 #pragma unroll
-        for (int t = 0; t < 2 * GR; ++t)
-          *reinterpret_cast<float2*>(w_o + ((size_t)warp * 8 * NQ + query) * HD + 32 * (t >> 1) + 4 * quad + 2 * (t & 1)) =
+        for (int t = 0; t < 2 * BL; ++t)
+          *reinterpret_cast<float2*>(w_o + ((size_t)warp * 4 * NQ + query) * HD + 64 * (t >> 1) + 32 * (qi >> 1) + 4 * quad + 2 * (t & 1)) =
               make_float2(o[x][t][e], o[x][t][2 + e]);
       }
     }
@@ -461,7 +528,7 @@ kv4_decode_kernel(const Kv4Params p) {
       // a part whose scores were all NaN has a maximum of -inf and a sum of NaN
       const float mw = w_m[w * 16 + r], f = mw == -INFINITY ? 1.f : exp2f(mw - M);
       L += w_l[w * 16 + r] * f;
-      O += w_o[((size_t)w * 8 * NQ + r) * HD + d] * f;
+      O += w_o[((size_t)w * 4 * NQ + r) * HD + d] * f;
     }
     if (p.splits == 1) out[idx] = __float2bfloat16_rn(finish(O, L));
     else {
@@ -496,7 +563,7 @@ int launch_decode(const Kv4Params& p, cudaStream_t s) {
   static bool configured[64] = {};
   if (allow_dynamic_smem(kv4_decode_kernel<HD, NQ>, C::RING, configured)) return -5;
   const int G = p.nh / p.nkv;
-  const dim3 grid(p.nkv * ((G + 8 * NQ - 1) / (8 * NQ)), p.rows, p.splits);
+  const dim3 grid(p.nkv * ((G + 4 * NQ - 1) / (4 * NQ)), p.rows, p.splits);
   if (grid.y > 65535) return ERR_TOO_LARGE;
   return launch_ex(kv4_decode_kernel<HD, NQ>, grid, dim3(C::THREADS), C::RING, s, p.splits, p);
 }
@@ -548,6 +615,7 @@ RLLM_API int rllm_kv4_decode(const void* q, int q_stride, const void* k4, const 
   const Kv4Params p = {q, q_stride, (const uint8_t*)k4, (const bf16*)ks, (const uint8_t*)v4, (const bf16*)vs, num_pages, out, out_stride,
                        nullptr, nullptr, kv_lens, block_table, bt_stride, num_seqs, nh, nkv, page_size, window, scale, shift, splits};
   cudaStream_t s = (cudaStream_t)stream;
-  if (hd == 64) return nh / nkv <= 8 ? launch_decode<64, 1>(p, s) : launch_decode<64, 2>(p, s);
-  return nh / nkv <= 8 ? launch_decode<128, 1>(p, s) : launch_decode<128, 2>(p, s);
+  const int G = nh / nkv;
+  if (hd == 64) return G <= 4 ? launch_decode<64, 1>(p, s) : G <= 8 ? launch_decode<64, 2>(p, s) : launch_decode<64, 4>(p, s);
+  return G <= 4 ? launch_decode<128, 1>(p, s) : G <= 8 ? launch_decode<128, 2>(p, s) : launch_decode<128, 4>(p, s);
 }
