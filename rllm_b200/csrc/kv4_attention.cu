@@ -144,7 +144,7 @@ kv4_attention_simt_kernel(const Kv4Params p) {
 // ---------------------------------------------------------------------------- single tokens
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {          // an 8 x 8 matrix of 16-bit numbers, rows to columns
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
@@ -160,13 +160,13 @@ __device__ __forceinline__ float fast_exp2(float x) {              // exp2(-inf)
   return y;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {     // nothing to add to
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
@@ -380,67 +380,69 @@ kv4_decode_kernel(const Kv4Params p) {
     const int j0 = (tb + i) * TILE;
     const bool edge = j0 < lo || j0 + TILE - 1 > pos;
 #pragma unroll
-    for (int sub = 0; sub < TILE / 16; ++sub) {
-      const int k0 = 16 * sub;
-      float s[NQ][4];
+    for (int half = 0; half < TILE / 32; ++half) {
+      // two fragments of 16 keys go together: their chains of products hide each other, and they share a look at the maximum
+      float s[2][NQ][4];
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-      // ---- scores, block by block
-      uint32_t sc[2][BL];                                // the scales of rows quad and quad + 8
+      for (int f = 0; f < 2; ++f) {
+        const int k0 = 32 * half + 16 * f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+        for (int x = 0; x < NQ; ++x) s[f][x][0] = s[f][x][1] = s[f][x][2] = s[f][x][3] = 0.f;
+        // ---- scores, block by block
 #pragma unroll
-        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(sa + st + (k0 + 8 * e) * (HD / 16) + 4 * b);
+        for (int b = 0; b < BL; ++b) {
+          const uint2 wa = lds64(ka[b] + st + k0 * ROW), wb = lds64(ka[b] + st + (k0 + 8) * ROW);
+          const float d0 = scale_of(lds32(sa + st + k0 * (HD / 16) + 4 * b)), d1 = scale_of(lds32(sa + st + (k0 + 8) * (HD / 16) + 4 * b));
+          uint32_t c0[4], c1[4], c2[4], c3[4];
+          codes_f16(wa.x, c0); codes_f16(wb.x, c1); codes_f16(wa.y, c2); codes_f16(wb.y, c3);
 #pragma unroll
-      for (int b = 0; b < BL; ++b) {
-        const uint2 wa = lds64(ka[b] + st + k0 * ROW), wb = lds64(ka[b] + st + (k0 + 8) * ROW);
-        uint32_t c0[4], c1[4], c2[4], c3[4];
-        codes_f16(wa.x, c0); codes_f16(wb.x, c1); codes_f16(wa.y, c2); codes_f16(wb.y, c3);
-        const float d0 = scale_of(sc[0][b]), d1 = scale_of(sc[1][b]);
+          for (int x = 0; x < NQ; ++x) {
+            float c[4];
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          float c[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint32_t a[4] = {c0[t], c1[t], c2[t], c3[t]};
-            if (t == 0) mma16816_first(c, a, qf[x][b][t][0], qf[x][b][t][1]);
-            else mma16816(c, a, qf[x][b][t][0], qf[x][b][t][1]);
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t a[4] = {c0[t], c1[t], c2[t], c3[t]};
+              if (t == 0) mma16816_first(c, a, qf[x][b][t][0], qf[x][b][t][1]);
+              else mma16816(c, a, qf[x][b][t][0], qf[x][b][t][1]);
+            }
+            s[f][x][0] = fmaf(d0, c[0], s[f][x][0]); s[f][x][1] = fmaf(d0, c[1], s[f][x][1]);
+            s[f][x][2] = fmaf(d1, c[2], s[f][x][2]); s[f][x][3] = fmaf(d1, c[3], s[f][x][3]);
           }
-          s[x][0] = fmaf(d0, c[0], s[x][0]); s[x][1] = fmaf(d0, c[1], s[x][1]);
-          s[x][2] = fmaf(d1, c[2], s[x][2]); s[x][3] = fmaf(d1, c[3], s[x][3]);
         }
-      }
 #pragma unroll
-      for (int x = 0; x < NQ; ++x)
+        for (int x = 0; x < NQ; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][e] += __shfl_xor_sync(0xffffffffu, s[x][e], 2);      // the other group's columns
-      if (edge) {
-        const int ja = j0 + k0 + krow, jb = ja + 8;
+          for (int e = 0; e < 4; ++e) {                  // plus the other group's columns
+            s[f][x][e] += __shfl_xor_sync(0xffffffffu, s[f][x][e], 2);
+            s[f][x][e] *= sl[x][e & 1];
+          }
+        if (edge) {
+          const int ja = j0 + k0 + krow, jb = ja + 8;
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          if (ja < lo || ja > pos) s[x][0] = s[x][1] = -INFINITY;
-          if (jb < lo || jb > pos) s[x][2] = s[x][3] = -INFINITY;
+          for (int x = 0; x < NQ; ++x) {
+            if (ja < lo || ja > pos) s[f][x][0] = s[f][x][1] = -INFINITY;
+            if (jb < lo || jb > pos) s[f][x][2] = s[f][x][3] = -INFINITY;
+          }
         }
       }
       // ---- weights
+      uint32_t sc[2][2][BL];                             // the value scales of rows quad and quad + 8
+      float big[2][2];                                   // log2 of the largest of a row
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int b = 0; b < BL; ++b) sc[e][b] = lds32(sa + st + C::SCALES + (k0 + 8 * e) * (HD / 16) + 4 * b);
-      float big[2];                                      // log2 of the largest value scale of rows quad and quad + 8
+        for (int e = 0; e < 2; ++e) {
+          float x = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = 0.f;
-#pragma unroll
-        for (int b = 0; b < BL; ++b) x = fmaxf(x, fmaxf(fabsf(bf16_lo(sc[e][b])), fabsf(bf16_hi(sc[e][b]))));      // (drops a NaN)
-        big[e] = exponent_of(x);
-      }
-      float pr[NQ][4];
+          for (int b = 0; b < BL; ++b) {
+            sc[f][e][b] = lds32(sa + st + C::SCALES + (32 * half + 16 * f + 8 * e) * (HD / 16) + 4 * b);
+            x = fmaxf(x, fmaxf(fabsf(bf16_lo(sc[f][e][b])), fabsf(bf16_hi(sc[f][e][b]))));      // (drops a NaN)
+          }
+          big[f][e] = exponent_of(x);
+        }
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][e] *= sl[x][e & 1];
-        float mx0 = fmaxf(s[x][0] + big[0], s[x][2] + big[1]), mx1 = fmaxf(s[x][1] + big[0], s[x][3] + big[1]);
+        float mx0 = fmaxf(fmaxf(s[0][x][0] + big[0][0], s[0][x][2] + big[0][1]), fmaxf(s[1][x][0] + big[1][0], s[1][x][2] + big[1][1]));
+        float mx1 = fmaxf(fmaxf(s[0][x][1] + big[0][0], s[0][x][3] + big[0][1]), fmaxf(s[1][x][1] + big[1][0], s[1][x][3] + big[1][1]));
         if (__any_sync(0xffffffffu, mx0 > m[x][0] + 8.f || mx1 > m[x][1] + 8.f)) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
@@ -455,34 +457,38 @@ kv4_decode_kernel(const Kv4Params p) {
           for (int t = 0; t < 2 * BL; ++t) { o[x][t][0] *= c0; o[x][t][1] *= c1; o[x][t][2] *= c0; o[x][t][3] *= c1; }
         }
         const float u0 = m[x][0] == -INFINITY ? 0.f : m[x][0], u1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
-        pr[x][0] = fast_exp2(s[x][0] - u0); pr[x][1] = fast_exp2(s[x][1] - u1);
-        pr[x][2] = fast_exp2(s[x][2] - u0); pr[x][3] = fast_exp2(s[x][3] - u1);
-        l[x][0] += pr[x][0] + pr[x][2];
-        l[x][1] += pr[x][1] + pr[x][3];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          s[f][x][0] = fast_exp2(s[f][x][0] - u0); s[f][x][1] = fast_exp2(s[f][x][1] - u1);
+          s[f][x][2] = fast_exp2(s[f][x][2] - u0); s[f][x][3] = fast_exp2(s[f][x][3] - u1);
+          l[x][0] += s[f][x][0] + s[f][x][2];
+          l[x][1] += s[f][x][1] + s[f][x][3];
+        }
       }
       // ---- values: the keys of weights 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
 #pragma unroll
-      for (int b = 0; b < BL; ++b) {
-        const float d0 = scale_of(sc[0][b]), d1 = scale_of(sc[1][b]);
+      for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                    // rows 0-7, then 8-15
-          uint32_t ca[4], cb[4];
-          codes_f16(lds32(va[b] + st + (k0 + 8 * e) * ROW), ca);
-          codes_f16(lds32(vb[b] + st + (k0 + 8 * e) * ROW), cb);
+        for (int b = 0; b < BL; ++b)
 #pragma unroll
-          for (int x = 0; x < NQ; ++x) {
-            const float d = e ? d1 : d0;
-            const uint32_t w = turn8x8(pack2(pr[x][2 * e] * d, pr[x][2 * e + 1] * d));
-            const uint32_t b0 = __byte_perm(w, 0u, put0), b1 = __byte_perm(w, 0u, put1);
-            // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the columns' group
+          for (int e = 0; e < 2; ++e) {                  // rows 0-7, then 8-15
+            const int k0 = 32 * half + 16 * f + 8 * e;
+            const float d = scale_of(sc[f][e][b]);
+            uint32_t ca[4], cb[4];
+            codes_f16(lds32(va[b] + st + k0 * ROW), ca);
+            codes_f16(lds32(vb[b] + st + k0 * ROW), cb);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t a[4] = {ca[2 * u], ca[2 * u + 1], cb[2 * u], cb[2 * u + 1]};
-              mma16816(o[x][2 * b + u], a, b0, b1);
+            for (int x = 0; x < NQ; ++x) {
+              const uint32_t w = turn8x8(pack2(s[f][x][2 * e] * d, s[f][x][2 * e + 1] * d));
+              const uint32_t b0 = __byte_perm(w, 0u, put0), b1 = __byte_perm(w, 0u, put1);
+              // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the columns' group
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t a[4] = {ca[2 * u], ca[2 * u + 1], cb[2 * u], cb[2 * u + 1]};
+                mma16816(o[x][2 * b + u], a, b0, b1);
+              }
             }
           }
-        }
-      }
     }
     __syncwarp();                                        // every lane has read the stage
     issue(i + D * NW, slot);
@@ -560,8 +566,19 @@ kv4_decode_kernel(const Kv4Params p) {
 template <int HD, int NQ>
 int launch_decode(const Kv4Params& p, cudaStream_t s) {
   typedef DecCfg<HD> C;
-  static bool configured[64] = {};
+  static bool configured[64] = {}, wide[64] = {};
   if (allow_dynamic_smem(kv4_decode_kernel<HD, NQ>, C::RING, configured)) return -5;
+  if (p.splits > 8) {                                    // a cluster beyond the portable size needs the kernel's own permission, per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return -5; }
+    if (!wide[dev]) {
+      if (cudaFuncSetAttribute(kv4_decode_kernel<HD, NQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        return ERR_BAD_SIZE;
+      }
+      wide[dev] = true;
+    }
+  }
   const int G = p.nh / p.nkv;
   const dim3 grid(p.nkv * ((G + 4 * NQ - 1) / (4 * NQ)), p.rows, p.splits);
   if (grid.y > 65535) return ERR_TOO_LARGE;
@@ -600,13 +617,13 @@ RLLM_API int rllm_kv4_attention_simt(int dt, const void* q, int q_stride, const 
 }
 
 // One bf16 query row per sequence: q [S, ...] with row stride q_stride (a multiple of 8, 16-byte aligned), head h at h * hd; out likewise.
-// kv_lens int32 [S]: keys that a sequence's token sees, its own included. splits: ranges of keys (1..8, the CTAs of a cluster).
+// kv_lens int32 [S]: keys that a sequence's token sees, its own included. splits: ranges of keys (1..16, the CTAs of a cluster).
 RLLM_API int rllm_kv4_decode(const void* q, int q_stride, const void* k4, const void* ks, const void* v4, const void* vs,
                              long long num_pages, void* out, int out_stride, const int* kv_lens, const int* block_table,
                              int bt_stride, int num_seqs, int nh, int nkv, int hd, int page_size, float scale, int window, int splits,
                              void* stream) {
   if (num_seqs <= 0) return 0;
-  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || splits < 1 || splits > 8 || !(scale > 0.f))
+  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || splits < 1 || splits > 16 || !(scale > 0.f))
     return ERR_BAD_SIZE;
   if (num_pages * nkv * page_size > 2147483647LL) return ERR_TOO_LARGE;
   if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)k4 | (uintptr_t)ks | (uintptr_t)v4 | (uintptr_t)vs) & 15)) return ERR_BAD_ALIGN;
