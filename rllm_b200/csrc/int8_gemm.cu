@@ -2,8 +2,8 @@
 // code products is exact in 32 bits up to K = 131,072 (127^2 K < 2^31), so it does not matter how it is cut; the two scales and
 // the rounding to the output's type follow in float.
 //
-// Two kernels. Few tokens (`streams`): the weights' stream, with the tokens quantised on the way. More: tcgen05.mma.kind::i8, the codes of both sides brought
-// in by TMA, accumulators in TMEM.
+// For more than a few tokens (those: int8_stream.cu), behind the kernel that quantises them: tcgen05.mma.kind::i8, the codes of both sides
+// brought in by TMA, accumulators in TMEM.
 #include "quant.cuh"
 #include "sm100.cuh"
 
@@ -22,10 +22,6 @@ struct Int8Params {
   int box;                           // token rows a copy brings
   int* err;
 };
-
-__device__ __forceinline__ float silu_gate(float g, float u, bool precise) {
-  return precise ? g / (1.f + expf(-g)) * u : __fdividef(g, 1.f + __expf(-g)) * u;
-}
 
 // D (+)= A B with 8-bit signed operands and 32-bit sums.
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -328,4 +324,25 @@ RLLM_API int rllm_int8_gemm(int epi, int out_dt, const void* x, const float* sx,
   if (epi == EPI_ACCUM_F32) return launch_epi<EPI_ACCUM_F32, float>(x, w, p, sm_count, s);
   if (epi == EPI_STORE) return out_dt == DT_F32 ? launch_epi<EPI_STORE, float>(x, w, p, sm_count, s) : launch_epi<EPI_STORE, bf16>(x, w, p, sm_count, s);
   return out_dt == DT_F32 ? launch_epi<EPI_SWIGLU, float>(x, w, p, sm_count, s) : launch_epi<EPI_SWIGLU, bf16>(x, w, p, sm_count, s);
+}
+
+// The two launchers that a product from numbers goes through (quant_rows.cu, int8_stream.cu).
+RLLM_API int rllm_quantize_rows(int dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps, void* codes,
+                                long long ldc, float* scales, int T, int K, int early, void* stream);
+RLLM_API int rllm_int8_streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g);
+RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
+                              const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int sm_count,
+                              void* stream);
+
+// y = x w^T from numbers x [*, xk] (as rllm_quantize_rows takes them): in one kernel for few tokens, else quantised into codes [T, K] and scales [T]
+// first. Without scratch (codes null) a product that wants it is not run: 1000000.
+RLLM_API int rllm_int8_linear(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
+                              void* codes, float* scales, const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk,
+                              int K, int* err, int sm_count, void* stream) {
+  if (T <= 0 || N <= 0) return 0;
+  if (rllm_int8_streams(T, xk, x_dt, x, ldx, g))
+    return rllm_int8_stream(epi, out_dt, x_dt, x, ldx, rows, g, g_dt, eps, w, sw, y, ldy, T, N, xk, K, sm_count, stream);
+  if (codes == nullptr) return 1000000;
+  const int rc = rllm_quantize_rows(x_dt, x, ldx, rows, g, g_dt, eps, codes, K, scales, T, xk, 1, stream);
+  return rc ? rc : rllm_int8_gemm(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, err, sm_count, stream);
 }

@@ -215,6 +215,7 @@ template <int HD> struct DecCfg {
   static constexpr int CODES = TILE * HD / 2, SCALES = TILE * HD / 16;
   static constexpr int STAGE = 2 * (CODES + SCALES);               // K codes, V codes, K scales, V scales
   static constexpr int RING = NW * D * STAGE;
+  static constexpr int ALONE = 120 * 1024;                         // more than half of an SM's shared memory
   // the warps' parts lie over the ring once it is done with: [NW][queries][HD], then the CTA's [queries][HD], maxima and sums
   static constexpr int parts(int nq) { return (NW + 1) * nq * HD * 4 + (NW + 1) * 16 * 8; }
 };
@@ -564,10 +565,10 @@ kv4_decode_kernel(const Kv4Params p) {
 }
 
 template <int HD, int NQ>
-int launch_decode(const Kv4Params& p, cudaStream_t s) {
+int launch_decode(const Kv4Params& p, int sm_count, cudaStream_t s) {
   typedef DecCfg<HD> C;
   static bool configured[64] = {}, wide[64] = {};
-  if (allow_dynamic_smem(kv4_decode_kernel<HD, NQ>, C::RING, configured)) return -5;
+  if (allow_dynamic_smem(kv4_decode_kernel<HD, NQ>, C::ALONE, configured)) return -5;
   if (p.splits > 8) {                                    // a cluster beyond the portable size needs the kernel's own permission, per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return -5; }
@@ -582,7 +583,11 @@ int launch_decode(const Kv4Params& p, cudaStream_t s) {
   const int G = p.nh / p.nkv;
   const dim3 grid(p.nkv * ((G + 4 * NQ - 1) / (4 * NQ)), p.rows, p.splits);
   if (grid.y > 65535) return ERR_TOO_LARGE;
-  return launch_ex(kv4_decode_kernel<HD, NQ>, grid, dim3(C::THREADS), C::RING, s, p.splits, p);
+  // While every CTA can have an SM of its own it takes one: the CTAs of a cluster are otherwise put on SMs in pairs (8 sequences of 4,096
+  // keys, 8 kv heads of 64, 2 ranges: 16.1 us, alone 12.4). Not so clusters of 16, for which too few GPCs have 16 SMs (41 us for one
+  // sequence of 60,000 keys of 128, 57 alone).
+  const long long ctas = (long long)grid.x * grid.y * grid.z;
+  return launch_ex(kv4_decode_kernel<HD, NQ>, grid, dim3(C::THREADS), ctas <= sm_count && p.splits <= 8 ? C::ALONE : C::RING, s, p.splits, p);
 }
 
 template <typename T>
@@ -621,7 +626,7 @@ RLLM_API int rllm_kv4_attention_simt(int dt, const void* q, int q_stride, const 
 RLLM_API int rllm_kv4_decode(const void* q, int q_stride, const void* k4, const void* ks, const void* v4, const void* vs,
                              long long num_pages, void* out, int out_stride, const int* kv_lens, const int* block_table,
                              int bt_stride, int num_seqs, int nh, int nkv, int hd, int page_size, float scale, int window, int splits,
-                             void* stream) {
+                             int sm_count, void* stream) {
   if (num_seqs <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || splits < 1 || splits > 16 || !(scale > 0.f))
     return ERR_BAD_SIZE;
@@ -633,6 +638,7 @@ RLLM_API int rllm_kv4_decode(const void* q, int q_stride, const void* k4, const 
                        nullptr, nullptr, kv_lens, block_table, bt_stride, num_seqs, nh, nkv, page_size, window, scale, shift, splits};
   cudaStream_t s = (cudaStream_t)stream;
   const int G = nh / nkv;
-  if (hd == 64) return G <= 4 ? launch_decode<64, 1>(p, s) : G <= 8 ? launch_decode<64, 2>(p, s) : launch_decode<64, 4>(p, s);
-  return G <= 4 ? launch_decode<128, 1>(p, s) : G <= 8 ? launch_decode<128, 2>(p, s) : launch_decode<128, 4>(p, s);
+  if (hd == 64)
+    return G <= 4 ? launch_decode<64, 1>(p, sm_count, s) : G <= 8 ? launch_decode<64, 2>(p, sm_count, s) : launch_decode<64, 4>(p, sm_count, s);
+  return G <= 4 ? launch_decode<128, 1>(p, sm_count, s) : G <= 8 ? launch_decode<128, 2>(p, sm_count, s) : launch_decode<128, 4>(p, sm_count, s);
 }

@@ -43,15 +43,11 @@ __device__ __forceinline__ bf16 quantize_group(const float (&v)[4], int shift, u
   bf16 d = __float2bfloat16_rn((hi >= -lo ? hi : lo) * -0.125f);
   if (bad != 0.f) d = __ushort_as_bfloat16((unsigned short)0x7fc0);
   const float df = __bfloat162float(d);
-  const float inv = 1.f / df;
+  const bool codes = df != 0.f && bad == 0.f;
+  const Rounding rd(codes ? df : 1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int c = 0;
-    if (df != 0.f && bad == 0.f) {
-      // (1 / d leaves the float range where |d| is below 2^-126: the division itself then)
-      const float r = fabsf(df) >= 1.17549435e-38f ? round_quotient(v[i], df, inv) : rintf(__fdiv_rn(v[i], df));
-      c = (int)fminf(fmaxf(r, -8.f), 7.f);
-    }
+    const int c = codes ? rd.code(v[i], -8, 7) : 0;
     word |= (uint32_t)(c + 8) << (shift + 4 * i);
   }
   return d;

@@ -10,22 +10,62 @@
 
 namespace rllm {
 
-// x / s to the nearest integer by the exact quotient, ties to even, for quotients below 2^9. `inv` is 1 / s, rounded: x * inv is
-// off by less than 2^-13, so only a product within 2^-12 of a half-integer leaves the question open. Then the quotient is
-// rounded once by the division; where that gives a half-integer, the remainder x - q s (exact, as the quotient is to the
-// nearest) says on which side of it the exact quotient lies.
-__device__ __forceinline__ float round_quotient(float x, float s, float inv) {
-  const float q0 = x * inv;
-  float r = rintf(q0);
-  if (fabsf(q0 - r) > 0.5f - 0.000244140625f) {
-    const float q = __fdiv_rn(x, s);
-    r = rintf(q);
-    if (fabsf(q - r) == 0.5f) {
-      const float rem = fmaf(-q, s, x);
-      if (rem != 0.f) r = ((rem > 0.f) == (s > 0.f)) ? q + 0.5f : q - 0.5f;
-    }
+// x / s to the nearest integer by the exact quotient, ties to even, |x / s| below 2^9, s normal; inv is 1 / s, rounded. x * inv is off by
+// less than 2^-13, so its nearest integer r is at most one off, next to a half-integer. What x has more than r s is a multiple of the
+// last place of s and not above s, or a difference of numbers within a factor of two: the fused product gives it exactly, and half of s
+// decides.
+__device__ __forceinline__ int round_quotient(float x, float s, float inv) {
+  const float y = fmaf(x, inv, 12582912.f);              // 1.5 2^23: the last bits are the integer
+  const int r = __float_as_int(y) - 0x4b400000;
+  const float e = fmaf(12582912.f - y, s, x), over = fabsf(e) - 0.5f * fabsf(s);
+  const bool step = over > 0.f || (over == 0.f && (r & 1));
+  return step ? r + ((e > 0.f) == (s > 0.f) ? 1 : -1) : r;
+}
+
+// A row's (group's) scale as the rounding wants it: where it is small enough for its inverse to leave the float range, numbers and scale
+// are taken times 2^64.
+struct Rounding {
+  float up, s, inv;
+  __device__ __forceinline__ explicit Rounding(float scale) {
+    up = fabsf(scale) < 1e-30f ? 18446744073709551616.f : 1.f;
+    s = scale * up;
+    inv = 1.f / s;
   }
-  return r;
+  __device__ __forceinline__ int code(float x, int lo, int hi) const { return min(max(round_quotient(x * up, s, inv), lo), hi); }
+};
+
+// Four 8-bit codes in a word, next to borders and for tiny scales (out of line: this is most of the code and runs once in a while).
+static __device__ __noinline__ uint32_t codes8_exact(float a, float b, float c, float d, float scale) {
+  const Rounding rd(scale);
+  return ((uint32_t)rd.code(a, -127, 127) & 0xffu) | ((uint32_t)rd.code(b, -127, 127) & 0xffu) << 8 |
+         ((uint32_t)rd.code(c, -127, 127) & 0xffu) << 16 | ((uint32_t)rd.code(d, -127, 127) & 0xffu) << 24;
+}
+// The 8-bit codes of N numbers of a row with scale s > 0, four a word. The exact quotient lies between x times numbers just below and just
+// above 1 / s; where both have the same nearest integer, it is that. (All but one number in 10,000; with a division for every number the
+// rows of a prompt took as long again as their memory.)
+template <int N>
+__device__ __forceinline__ void codes8(const float (&v)[N], float s, float inv, uint32_t (&w)[N / 4]) {
+  const float lo = inv * (1.f - 2.384185791e-7f), hi = inv * (1.f + 2.384185791e-7f);      // 2^-22, more than the two roundings of inv
+  uint32_t differ = s < 1e-30f;                          // (the inverse of a tiny scale leaves the float range)
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = __float_as_uint(fmaf(v[i + e], lo, 12582912.f));            // 1.5 2^23: the last byte is the code
+      differ |= y[e] ^ __float_as_uint(fmaf(v[i + e], hi, 12582912.f));
+    }
+    w[i / 4] = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+  }
+  if (differ) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) w[i / 4] = codes8_exact(v[i], v[i + 1], v[i + 2], v[i + 3], s);
+  }
+}
+
+// silu(g) u; in full float precision, or for a result that is rounded to bfloat16
+__device__ __forceinline__ float silu_gate(float g, float u, bool precise) {
+  return precise ? g / (1.f + expf(-g)) * u : __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
 // One layer's keys (or values) in 4 bits: codes [page][kv head][offset in page][hd / 2 bytes], scales bf16 [..][hd / 32]. 64

@@ -4,7 +4,7 @@
 //
 // The row has to be read before its scale is known, so a CTA holds it: 256 threads with up to VPT groups of 8 numbers in registers
 // each (8,192 numbers with four groups), longer rows are read twice, the second time out of the caches. The bound is the
-// read of x and the write of the codes; a quotient is a multiplication by 1 / s except next to a border (`round_quotient`), since
+// read of x and the write of the codes; a quotient is a multiplication by 1 / s except next to a border (`codes8`), since
 // a division for every number took as long as the memory.
 // Codes lie in rows of a multiple of 16 bytes (`ldc`), the numbers behind K are zeros: the products' copies are whole pieces.
 #include "quant.cuh"
@@ -99,18 +99,16 @@ quantize_rows_kernel(const RowArgs a) {
   const bool whole = b == 0.f && amax <= 3.402823466e38f;
   const float s = __fdiv_rn(amax, 127.f);
   if (threadIdx.x == 0) a.scales[t] = whole ? s : __int_as_float(0x7fc00000);
-  const float inv = whole && s > 0.f ? 1.f / s : 0.f;
+  const bool codes = whole && s > 0.f;
+  const float inv = codes ? 1.f / s : 0.f;
   int8_t* row = a.codes + (size_t)t * a.ldc;
   auto put = [&](int k, const float (&v)[8]) {
     uint32_t w[2] = {0u, 0u};
-    if (inv > 0.f) {                                     // (no scale: codes of zero)
+    if (codes) {                                         // (no scale: codes of zero)
+      float n[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float n = a.g ? v[e] * rstd : v[e];
-        // (1 / s leaves the float range where s is below 2^-126: the division itself then)
-        const float r = fminf(fmaxf(s >= 1.17549435e-38f ? round_quotient(n, s, inv) : rintf(__fdiv_rn(n, s)), -127.f), 127.f);
-        w[e >> 2] |= ((uint32_t)(int)r & 0xffu) << (8 * (e & 3));
-      }
+      for (int e = 0; e < 8; ++e) n[e] = a.g ? v[e] * rstd : v[e];
+      codes8<8>(n, s, inv, w);
     }
     *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
   };

@@ -161,9 +161,9 @@ class Backend:
 
     def _int8(self, x, w, epilogue, out=None):
         """The product with a weight in 8 bits: the rows are quantised first, a norm in front in the same kernel."""
-        q = self._quant
-        rows = q.quantize_rows(x.h, (x.weight, x.eps), x.rows) if isinstance(x, Normed) else q.quantize_rows(x)
-        return q.linear_int8(rows, w, epilogue, out, self.dtype)
+        if isinstance(x, Normed):
+            return self._quant.linear(x.h, w, epilogue, out, self.dtype, (x.weight, x.eps), x.rows)
+        return self._quant.linear(x, w, epilogue, out, self.dtype)
 
     def linear(self, x, w, bias=None, tag=None):
         # `tag` names the product for per-operation timing (kernels/profile.py); it changes nothing here

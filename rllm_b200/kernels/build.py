@@ -42,7 +42,7 @@ LIBRARIES: dict[str, list[str]] = {
     "sink": ["sink_attention.cu", "stream_ops.cu"],
     "recurrent": ["recurrent.cu"],
     "rows": ["row_mix.cu"],
-    "quant": ["quant_rows.cu", "int8_gemm.cu", "kv4_cache.cu", "kv4_attention.cu"],
+    "quant": ["quant_rows.cu", "int8_gemm.cu", "int8_stream.cu", "kv4_cache.cu", "kv4_attention.cu"],
     "hybrid": ["talk_attention.cu", "gated_ops.cu"],
     "host": ["host_runtime.cpp"],          # no CUDA: the cache manager's bookkeeping and metadata writer
 }

@@ -9,6 +9,7 @@ even, clamped to -8..7; the number stands for code * d. (The layout is in csrc/q
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from functools import lru_cache
 
 import torch
 
@@ -18,11 +19,13 @@ _P = c_void_p
 ops.register_signatures("quant", {
     "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, c_int, _P],
     "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, _P, c_int, _P],
+    "rllm_int8_linear": [c_int, c_int, c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int,
+                         c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
     "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int,
                       c_int, _P],
     "rllm_kv4_decode": [_P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                        c_int, _P],
+                        c_int, c_int, _P],
     "rllm_kv4_attention_simt": [c_int, _P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
                                 c_int, c_float, c_int, _P],
 })
@@ -33,8 +36,8 @@ HEAD_SIZES = (64, 128, 192, 256)
 
 def _here(t: torch.Tensor, name: str) -> None:
     """The launch goes to the current device's current stream: a tensor of another device would be read from there."""
-    ops._cuda(t, name)
-    if t.device.index != ops._raw_device():
+    if not t.is_cuda or t.get_device() != ops._raw_device():
+        ops._cuda(t, name)
         raise ops.KernelError(f"{name} is on {t.device}, the current device is cuda:{ops._raw_device()}")
 
 
@@ -66,31 +69,38 @@ class Int8Matrix(Int8Rows):
     """A weight [N, K] in 8 bits, a scale per output channel: the backend's products take it where they take a tensor."""
 
 
-def quantize_rows(x: torch.Tensor, norm: tuple | None = None, rows: torch.Tensor | None = None, cls=Int8Rows) -> Int8Rows:
-    """Rows of x [T, K] (float32 or bfloat16, unit inner stride) in 8 bits. `norm` (weight, eps): of their RMSNorm, which is not
-    rounded in between. `rows` int32 [R]: of those rows only."""
+def _rows(x: torch.Tensor, norm: tuple | None, rows: torch.Tensor | None):
+    """(dtype, rows, columns, norm weight or None, its dtype, eps) of rows to be quantised, checked."""
     _here(x, "x")
     dt = ops._dt(x, "x")
     if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ops.KernelError("quantize_rows takes [T, K] rows with unit inner stride")
+        raise ops.KernelError("rows in 8 bits: x must be [T, K] with unit inner stride")
     T, K = x.shape
     if K < 1:
-        raise ops.KernelError("quantize_rows: rows without numbers")
+        raise ops.KernelError("rows in 8 bits: rows without numbers")
     if rows is not None:
         _here(rows, "rows")
         if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
-            raise ops.KernelError("quantize_rows: rows must be a contiguous int32 vector")
+            raise ops.KernelError("rows in 8 bits: rows must be a contiguous int32 vector")
         T = rows.numel()
-    w, eps = norm if norm is not None else (None, 0.0)
-    if w is not None:
-        _here(w, "norm weight")
-        if w.shape != (K,) or not w.is_contiguous():
-            raise ops.KernelError(f"norm weight must be a contiguous [{K}], got {tuple(w.shape)}")
+    if norm is None:
+        return dt, T, K, None, 0, 0.0
+    w, eps = norm
+    _here(w, "norm weight")
+    if w.shape != (K,) or not w.is_contiguous():
+        raise ops.KernelError(f"norm weight must be a contiguous [{K}], got {tuple(w.shape)}")
+    return dt, T, K, w.data_ptr(), ops._dt(w, "norm weight"), eps
+
+
+def quantize_rows(x: torch.Tensor, norm: tuple | None = None, rows: torch.Tensor | None = None, cls=Int8Rows) -> Int8Rows:
+    """Rows of x [T, K] (float32 or bfloat16, unit inner stride) in 8 bits. `norm` (weight, eps): of their RMSNorm, which is not
+    rounded in between. `rows` int32 [R]: of those rows only."""
+    dt, T, K, g, g_dt, eps = _rows(x, norm, rows)
     codes = torch.empty((T, (K + 15) // 16 * 16), dtype=torch.int8, device=x.device)
     scales = torch.empty(T, dtype=torch.float32, device=x.device)
     ops._check(ops._fn("quant", "rllm_quantize_rows")(
-        dt, x.data_ptr(), x.stride(0), ops._ptr(rows), ops._ptr(w), 0 if w is None else ops._dt(w, "norm weight"), float(eps),
-        codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, K, int(cls is Int8Rows), ops._stream()), "quantize_rows")
+        dt, x.data_ptr(), x.stride(0), ops._ptr(rows), g, g_dt, float(eps), codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, K,
+        int(cls is Int8Rows), ops._stream()), "quantize_rows")
     return cls(codes, scales, K)
 
 
@@ -99,37 +109,73 @@ def quantize_matrix(w: torch.Tensor) -> Int8Matrix:
     return quantize_rows(w, cls=Int8Matrix)
 
 
+def _output(T: int, K: int, w: Int8Matrix, epilogue: int, out: torch.Tensor | None, out_dtype: torch.dtype, device):
+    """(outputs, output tensor) of a product with w, checked."""
+    if not isinstance(w, Int8Matrix):
+        raise ops.KernelError("a product in 8 bits takes an Int8Matrix")
+    _here(w.codes, "w")
+    N = w.codes.shape[0]
+    if w.width != K:
+        raise ops.KernelError(f"product in 8 bits: x has {K} columns, w has {w.width}")
+    if K > INT8_MAX_K:
+        raise ops.KernelError(f"product in 8 bits: {K} columns; the sums are exact in 32 bits up to {INT8_MAX_K}")
+    if epilogue == ops.EPI_SWIGLU:
+        if N % 2:
+            raise ops.KernelError("product in 8 bits: a gate/up pair has an even number of rows")
+        N //= 2
+    elif epilogue in (ops.EPI_STORE_F32, ops.EPI_ACCUM_F32):
+        out_dtype = torch.float32
+    elif epilogue != ops.EPI_STORE:
+        raise ops.KernelError(f"product in 8 bits: no epilogue {epilogue}")
+    if out is None:
+        if epilogue == ops.EPI_ACCUM_F32:
+            raise ops.KernelError("product in 8 bits: nothing to add into (`out`)")
+        return N, torch.empty((T, N), dtype=out_dtype, device=device)
+    _here(out, "out")
+    if out.shape != (T, N) or out.dtype != out_dtype or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N):
+        raise ops.KernelError(f"product in 8 bits: out must be {out_dtype} [{T}, {N}] with unit inner stride and rows side by side")
+    return N, out
+
+
 def linear_int8(x: Int8Rows, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x w^T from the codes: the integer sums are exact, times both scales in float. `epilogue`: `ops.EPI_STORE` (rounded once to
     out_dtype), `EPI_STORE_F32`, `EPI_ACCUM_F32` (added into the float `out`) or `EPI_SWIGLU` (w = [gate; up])."""
-    if not isinstance(x, Int8Rows) or not isinstance(w, Int8Matrix):
-        raise ops.KernelError("linear_int8 takes Int8Rows and an Int8Matrix")
-    _here(x.codes, "x"); _here(w.codes, "w")
+    if not isinstance(x, Int8Rows) or isinstance(x, Int8Matrix):
+        raise ops.KernelError("linear_int8 takes Int8Rows (numbers: linear)")
+    _here(x.codes, "x")
     T, K = x.shape
-    N = w.shape[0]
-    if w.shape[1] != K:
-        raise ops.KernelError(f"linear_int8: x has {K} columns, w has {w.shape[1]}")
-    if K > INT8_MAX_K:
-        raise ops.KernelError(f"linear_int8: {K} columns; the sums are exact in 32 bits up to {INT8_MAX_K}")
-    if epilogue not in (ops.EPI_STORE, ops.EPI_STORE_F32, ops.EPI_ACCUM_F32, ops.EPI_SWIGLU):
-        raise ops.KernelError(f"linear_int8 has no epilogue {epilogue}")
-    if epilogue == ops.EPI_SWIGLU:
-        if N % 2:
-            raise ops.KernelError("linear_int8: a gate/up pair has an even number of rows")
-        N //= 2
-    want = torch.float32 if epilogue in (ops.EPI_STORE_F32, ops.EPI_ACCUM_F32) else out_dtype
-    if out is None:
-        if epilogue == ops.EPI_ACCUM_F32:
-            raise ops.KernelError("linear_int8: nothing to add into (`out`)")
-        out = torch.empty((T, N), dtype=want, device=x.device)
-    _here(out, "out")
-    if tuple(out.shape) != (T, N) or out.dtype != want or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N):
-        raise ops.KernelError(f"linear_int8: out must be {want} [{T}, {N}] with unit inner stride and rows side by side")
-    st = sm100.init(x.device)
+    N, out = _output(T, K, w, epilogue, out, out_dtype, x.codes.device)
+    st = sm100.init(x.codes.device)
     ops._check(ops._fn("quant", "rllm_int8_gemm")(
         epilogue, ops._dt(out, "out"), x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
         max(out.stride(0), N), T, N, x.codes.shape[1], st.err.data_ptr(), st.sm_count, ops._stream()), "linear_int8")
+    return out
+
+
+_NEEDS_SCRATCH = 1000000
+# Tokens up to which a product may quantise them itself (int8_stream.cu has the whole rule)
+STREAM_TOKENS = 16
+
+
+def linear(x: torch.Tensor, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: torch.Tensor | None = None,
+           out_dtype: torch.dtype = torch.bfloat16, norm: tuple | None = None, rows: torch.Tensor | None = None) -> torch.Tensor:
+    """x w^T in 8 bits from numbers: `linear_int8(quantize_rows(x, norm, rows), w, ...)`, in one kernel for few tokens."""
+    dt, T, K, g, g_dt, eps = _rows(x, norm, rows)
+    device = x.device
+    N, out = _output(T, K, w, epilogue, out, out_dtype, device)
+    st = sm100.init(device)
+    KP = w.codes.shape[1]
+    fn = ops._fn("quant", "rllm_int8_linear")
+    call = lambda codes, scales: fn(
+        epilogue, ops._dt(out, "out"), dt, x.data_ptr(), x.stride(0), ops._ptr(rows), g, g_dt, eps, codes, scales, w.codes.data_ptr(),
+        w.scales.data_ptr(), out.data_ptr(), max(out.stride(0), N), T, N, K, KP, st.err.data_ptr(), st.sm_count, ops._stream())
+    rc = call(None, None) if T <= STREAM_TOKENS else _NEEDS_SCRATCH
+    launches = 1
+    if rc == _NEEDS_SCRATCH:
+        room = torch.empty(T * KP + 4 * T, dtype=torch.uint8, device=device)       # codes (rows of 16 bytes), then scales
+        rc, launches = call(room.data_ptr(), room.data_ptr() + T * KP), 2
+    ops._check(rc, "linear in 8 bits", launches)
     return out
 
 
@@ -138,16 +184,17 @@ def linear_int8(x: Int8Rows, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: 
 
 def _kv4(tensors: dict) -> tuple:
     """(k4, ks, v4, vs, pages, kv heads, page size, head size) of a layer's tensors, checked."""
-    k4, ks, v4, vs = (tensors[n] for n in ("k4", "ks", "v4", "vs"))
-    pages, nkv, page_size, half = k4.shape
+    k4, ks, v4, vs = tensors["k4"], tensors["ks"], tensors["v4"], tensors["vs"]
+    shape = k4.shape
+    pages, nkv, page_size, half = shape
     hd = 2 * half
     if hd not in HEAD_SIZES:
         raise ops.KernelError(f"a cache held in 4 bits has heads of {HEAD_SIZES}, not {hd}")
-    for t, name, dt, n in ((k4, "k4", torch.uint8, half), (v4, "v4", torch.uint8, half), (ks, "ks", torch.bfloat16, hd // 32),
-                           (vs, "vs", torch.bfloat16, hd // 32)):
-        _here(t, name)
-        if t.dtype != dt or tuple(t.shape) != (pages, nkv, page_size, n) or not t.is_contiguous():
-            raise ops.KernelError(f"{name} must be contiguous {dt} [{pages}, {nkv}, {page_size}, {n}]")
+    here, scales = ops._raw_device(), (pages, nkv, page_size, hd // 32)
+    for t, want, dt in ((k4, shape, torch.uint8), (v4, shape, torch.uint8), (ks, scales, torch.bfloat16), (vs, scales, torch.bfloat16)):
+        if t.dtype != dt or t.shape != want or not t.is_contiguous() or not t.is_cuda or t.get_device() != here:
+            raise ops.KernelError(f"a cache held in 4 bits: codes must be contiguous uint8 {tuple(shape)} and scales bfloat16 {scales}, on the "
+                                  f"current CUDA device (cuda:{here})")
     return k4, ks, v4, vs, pages, nkv, page_size, hd
 
 
@@ -167,11 +214,11 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, tensors: dict, slots: torch.Tens
     """Keys and values [T, kv heads * head size] (float32 or bfloat16, rows may lie apart) into the pages at slots int32 [T]
     (page * page size + offset; -1: not stored). A slot may stand in a call once."""
     k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
-    for t, name in ((k, "k"), (v, "v")):
-        _here(t, name)
-        if t.dim() != 2 or t.shape[1] != nkv * hd or t.stride(1) != 1 or t.shape[0] != k.shape[0] or t.dtype != k.dtype:
-            raise ops.KernelError(f"kv4_store: {name} must be [T, {nkv * hd}] with unit inner stride, k and v alike")
-    T = k.shape[0]
+    _here(k, "k"); _here(v, "v")
+    shape = k.shape
+    if len(shape) != 2 or shape[1] != nkv * hd or v.shape != shape or v.dtype != k.dtype or k.stride(1) != 1 or v.stride(1) != 1:
+        raise ops.KernelError(f"kv4_store: k and v must be alike, [T, {nkv * hd}] with unit inner stride")
+    T = shape[0]
     _i32(slots, "slots", T)
     ops._check(ops._fn("quant", "rllm_kv4_store")(
         ops._dt(k, "k"), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), slots.data_ptr(), k4.data_ptr(), ks.data_ptr(),
@@ -190,7 +237,7 @@ def kv4_read(tensors: dict, block_table: torch.Tensor, kv_lens: torch.Tensor, ma
     width = -(-int(max_kv_len) // page_size)
     if width > block_table.shape[1]:
         raise ops.KernelError(f"kv4_read: {max_kv_len} positions are {width} pages, the table has {block_table.shape[1]}")
-    k, v = (torch.empty((S, width, nkv, page_size, hd), dtype=dtype, device=k4.device) for _ in range(2))
+    k, v = torch.empty((2, S, width, nkv, page_size, hd), dtype=dtype, device=k4.device).unbind(0)
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops._dt(k, "k"), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr(),
         block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), None, None, None, nkv, page_size, hd,
@@ -220,18 +267,25 @@ def attention_kv4_simt(q: torch.Tensor, tensors: dict, token_seq: torch.Tensor, 
     return out
 
 
-DECODE_MAX_SPLITS = 8
 # Places of a key range's page in the scratch that portions are read into, and bytes of scratch a run of portions may take at once
 READ_PAGE, READ_BYTES = 128, 2 << 30
 
 
-def decode_splits(num_seqs: int, ctas: int, max_kv_len: int, sm_count: int, hd: int) -> int:
-    """Ranges the keys of a sequence are cut into (= CTAs of a cluster)."""
-    base, best, cost = max(1, num_seqs * ctas), 1, None
-    for s in range(1, DECODE_MAX_SPLITS + 1):
-        if s > 1 and max_kv_len < 128 * s:
+@lru_cache(maxsize=4096)
+def decode_splits(base: int, keys: int, sm_count: int, hd: int) -> int:
+    """Ranges the keys of a sequence are cut into (= CTAs of a cluster), `base` CTAs without: by the time in us of the rounds of CTAs over
+    the places, two an SM: 2.6 before the first key (4 in later rounds), 0.0047 a key at heads of 64 and 0.007 at 128, a tenth (three tenths)
+    more where two share an SM (the CTAs of a cluster of 16 do), and 1.6 + 0.1 a range for a cluster's merge."""
+    best, cost = 1, None
+    step, shared = (0.0047, 1.1) if hd == 64 else (0.007, 1.3)
+    for s in (1, 2, 3, 4, 5, 6, 7, 8, 16):
+        n = base * s
+        if s > 1 and keys < 64 * s or s > 8 and n > sm_count:
             break
-        c = -(-base * s // (2 * sm_count)) * (1150 + max_kv_len * hd / 128 / s) + 50 * s + (200 if s > 1 else 0)
+        rounds = -(-n // (2 * sm_count))
+        if s in (3, 5, 6, 7, 8) and n > sm_count and n * 16 > rounds * 2 * sm_count * 13:    # such clusters do not fill a GPC evenly
+            continue
+        c = 2.6 + 4 * (rounds - 1) + rounds * step * (shared if n > sm_count or s > 8 else 1) * keys / s + (1.6 + 0.1 * s if s > 1 else 0)
         if cost is None or c < cost:
             best, cost = s, c
     return best
@@ -245,7 +299,7 @@ def decode_supported(q: torch.Tensor, hd: int, scale: float) -> bool:
 def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
                          window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: the most keys of a sequence;
-    `splits`: that many ranges of keys (1 to 8), None: by `decode_splits`."""
+    `splits`: that many ranges of keys (1 to 8, 16), None: by `decode_splits`."""
     k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
     S = kv_lens.numel()
     _queries(q, nh, nkv, hd, S)
@@ -254,15 +308,16 @@ def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, 
     _i32(kv_lens, "kv_lens", S)
     _table(block_table, S)
     G = nh // nkv
+    sms = sm100.init(q.device).sm_count
     if splits is None:
         seen = min(max_kv_len, window) if window else max_kv_len
-        splits = decode_splits(S, nkv * (-(-G // 8) if G <= 8 else -(-G // 16)), seen, sm100.init(q.device).sm_count, hd)
+        splits = decode_splits(S * nkv * -(-G // 16), seen, sms, hd)
     if out is None:
-        out = torch.empty((S, nh * hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((S, nh * hd))
     ops._check(ops._fn("quant", "rllm_kv4_decode")(
         q.data_ptr(), q.stride(0), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr(), out.stride(0),
         kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), S, nh, nkv, hd, page_size, float(scale), int(window or 0),
-        int(splits), ops._stream()), "attention_kv4_decode")
+        int(splits), sms, ops._stream()), "attention_kv4_decode")
     return out
 
 
@@ -306,19 +361,22 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
     room = scratch(2 * size, lambda: torch.empty((2, S * width, nkv, READ_PAGE, hd), dtype=torch.bfloat16, device=q.device))
     if room is None:
         return False
-    k, v = room[0], room[1].view(torch.float16)
-    meta = torch.empty(S * width * (1 + nkv) + S + 1, dtype=torch.int32, device=q.device)
-    table, vexp, cu = meta[: S * width].view(S, width), meta[S * width: S * width * (1 + nkv)], meta[S * width * (1 + nkv):]
-    kv_lens, bt = ctx.kv_lens[s0:s1], block_table[s0:s1]
+    k, v = room.unbind(0)
+    v = v.view(torch.float16)
+    table, vexp, cu = q.new_empty(S * width * (1 + nkv) + S + 1, dtype=torch.int32).split((S * width, S * width * nkv, S + 1))
+    whole = S == ctx.num_seqs                      # (a view costs the host as much as half a launch)
+    kv_lens, bt = (ctx.kv_lens, block_table) if whole else (ctx.kv_lens[s0:s1], block_table[s0:s1])
+    if not whole:
+        q, out = q[r0:r1], out[r0:r1]
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, bt.data_ptr(), bt.stride(0), kv_lens.data_ptr(),
-        ctx.cu_q[s0:].data_ptr(), int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+        ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), table.data_ptr(),
         cu.data_ptr(), vexp.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
-    a = (q[r0:r1], k, v, cu, kv_lens, table)
-    if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(a[0], k):
-        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out[r0:r1], vexp=vexp)
+    a = (q, k, v, cu, kv_lens, table.view(S, width))
+    if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(q, k):
+        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out, vexp=vexp)
     else:
-        sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out[r0:r1], vexp=vexp)
+        sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out, vexp=vexp)
     return True
 
 
@@ -333,7 +391,7 @@ def attention_kv4(q: torch.Tensor, tensors: dict, ctx, block_table: torch.Tensor
     if ctx.max_q_len == 1:
         return attention_kv4_decode(q, tensors, ctx.kv_lens, block_table, nh, scale, window, ctx.max_kv_len)
     _queries(q, nh, tensors["k4"].shape[1], hd, ctx.num_tokens)
-    out = torch.empty((q.shape[0], nh * hd), dtype=q.dtype, device=q.device)
+    out = q.new_empty((q.shape[0], nh * hd))
     for run in _runs(ctx):
         s0, s1, r0, r1, single, _, most = run
         if single:

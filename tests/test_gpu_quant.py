@@ -157,6 +157,40 @@ def test_product_swiglu(T, N, K, dtype):
     assert ((y - want).abs() <= (e + HALF[dt]) * want.abs() + 1e-30).all()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,N,K", [(1, 1, 8), (1, 48, 2048), (2, 40, 40), (3, 17, 4104), (5, 130, 1000), (8, 515, 8192), (8, 36, 16384), (7, 33, 16392),
+                                   (9, 256, 512), (16, 96, 8192), (13, 100, 4096), (16, 72, 2048), (16, 20, 8200), (17, 64, 64), (4, 30, 33),
+                                   (1, 4000, 512), (8, 2400, 256)])
+def test_product_from_numbers(T, N, K, dtype):
+    """The product that quantises its tokens itself (few of them) equals the two calls, every epilogue, with and without a norm."""
+    q, o = quant(), ops()
+    w = q.quantize_matrix(rnd(2 * N, K, seed=2, dtype=torch.bfloat16).to(DEV))
+    x = rnd(T + 3, K, seed=1, dtype=DT[dtype], scale=2.0).to(DEV)
+    if T > 3:
+        x[1] = 0
+        x[2] *= 1e-36
+        x[3, 5] = math.inf
+    half = q.Int8Matrix(w.codes[:N], w.scales[:N], K)
+    g = (1 + rnd(K, seed=5, scale=0.2)).to(DEV)
+    rows = torch.arange(T - 1, -1, -1, dtype=torch.int32, device=DEV)
+    for kw in ({}, {"rows": rows}):
+        a = q.quantize_rows(x if kw else x[:T], **kw)
+        for epi, m in ((o.EPI_STORE, half), (o.EPI_STORE_F32, half), (o.EPI_SWIGLU, w)):
+            want = q.linear_int8(a, m, epi, out_dtype=DT[dtype])
+            got = q.linear(x if kw else x[:T], m, epi, out_dtype=DT[dtype], **kw)
+            assert equal(got, want), (epi, kw)
+        res = rnd(T, N, seed=9).to(DEV)
+        assert equal(q.linear(x if kw else x[:T], half, o.EPI_ACCUM_F32, res.clone(), **kw), q.linear_int8(a, half, o.EPI_ACCUM_F32, res.clone()))
+    # a norm in front sums its squares in another order: the row's scale moves by a few units in the last place, a code by a step
+    # where it was next to a border
+    for gw in (g, g.bfloat16()):
+        want = q.linear_int8(q.quantize_rows(x[:T], (gw, 1e-5)), half, o.EPI_STORE_F32).double()
+        got = q.linear(x[:T], half, o.EPI_STORE_F32, norm=(gw, 1e-5)).double()
+        size = want.abs().nan_to_num().amax(dim=1, keepdim=True)
+        assert equal(torch.isnan(got), torch.isnan(want)) and ((got - want).nan_to_num().abs() <= 0.02 * size + 1e-30).all()
+        assert float(((got - want).nan_to_num().abs() <= 1e-5 * size).float().mean()) > 0.5
+
+
 def test_product_into_a_wider_tensor_and_wide_sums():
     x, w, px, pw = product_inputs(20, 48, 96, torch.bfloat16)
     big = torch.full((20, 100), 7.0, dtype=torch.bfloat16, device=DEV)
@@ -166,6 +200,8 @@ def test_product_into_a_wider_tensor_and_wide_sums():
     # every product at its largest: 127^2 K is still a whole number below 2^31
     K = 131072
     ones = torch.ones(3, K, dtype=torch.bfloat16, device=DEV)
+    far = quant().linear(torch.full((8, 16384), 3.0, device=DEV), quant().quantize_matrix(torch.full((5, 16384), -2.0, device=DEV)), ops().EPI_STORE_F32)
+    assert float((far.double() / -(6 * 16384) - 1).abs().max()) <= 6 * 2.0 ** -24
     for T in (3, 40):
         q = quant()
         y = q.linear_int8(q.quantize_rows(ones.expand(3, K).repeat(14, 1)[:T].contiguous()), q.quantize_matrix(-ones), ops().EPI_STORE_F32)
