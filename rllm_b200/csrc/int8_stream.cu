@@ -188,7 +188,7 @@ int8_stream_kernel(const StreamParams p) {
       const bool whole = mx <= 3.402823466e38f && amax <= 3.402823466e38f;      // every number finite
       const float s = __fdiv_rn(amax, 127.f);
       const bool codes = whole && s > 0.f;
-      const float inv = codes ? 1.f / s : 0.f;
+      const Rounding rd(codes ? s : 1.f);
       if (warp == 0 && t == 0) s_scale[SNT * q + g] = whole ? s : __int_as_float(0x7fc00000);
 #pragma unroll
       for (int ci = 0; ci < NCH; ++ci)
@@ -197,12 +197,8 @@ int8_stream_kernel(const StreamParams p) {
           float fresh[16], unused = 0.f;
           if (!KEEP) load16<F32>(p, xr[q], (warp * NCH + ci) * SCK + 64 * kb + 16 * t, fresh, unused);
           float (&v)[16] = KEEP ? keep[KEEP ? kb : 0] : fresh;
-          if (p.g) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= rstd;
-          }
           uint32_t w[4] = {0u, 0u, 0u, 0u};
-          if (codes) codes8<16>(v, s, inv, w);
+          if (codes) codes8<16>(v, rstd, rd, w);
 #pragma unroll
           for (int i = 0; i < 4; ++i) b[ci][q][kb][i] = w[i] ^ 0x80808080u;
         }

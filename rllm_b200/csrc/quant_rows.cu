@@ -100,15 +100,12 @@ quantize_rows_kernel(const RowArgs a) {
   const float s = __fdiv_rn(amax, 127.f);
   if (threadIdx.x == 0) a.scales[t] = whole ? s : __int_as_float(0x7fc00000);
   const bool codes = whole && s > 0.f;
-  const float inv = codes ? 1.f / s : 0.f;
+  const Rounding rd(codes ? s : 1.f);
   int8_t* row = a.codes + (size_t)t * a.ldc;
   auto put = [&](int k, const float (&v)[8]) {
     uint32_t w[2] = {0u, 0u};
     if (codes) {                                         // (no scale: codes of zero)
-      float n[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) n[e] = a.g ? v[e] * rstd : v[e];
-      codes8<8>(n, s, inv, w);
+      codes8<8>(v, a.g ? rstd : 1.f, rd, w);
     }
     *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
   };
