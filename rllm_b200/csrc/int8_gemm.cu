@@ -20,6 +20,7 @@ struct Int8Params {
   int vec;                           // rows of y start on 16 bytes
   int T, N, K;                       // N: outputs (of one half with SwiGLU); K: bytes a row, a multiple of 16
   int box;                           // token rows a copy brings
+  int splits;                        // ranges of K
   int* err;
 };
 
@@ -246,6 +247,159 @@ int8_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, C::TMEM_COLS); }
 }
 
+// ---------------------------------------------------------------------------- few tiles: ranges of K
+// Four MMAs on a block of K take 0.26 us whatever the tile's width (32 weight rows or 256), so a CTA's time goes with its blocks. Where the tiles
+// leave most SMs idle and K is long, a tile is shared by the CTAs of a cluster, each with a range of K. The parts are whole numbers, so
+// their sum does not depend on the cut. Rank r finishes the r-th part of the tile's features: every rank pushes its accumulator's
+// columns to their owners through distributed shared memory, into the stage ring, which is idle once all ranks' products are
+// complete (one cluster barrier), and the owners add them up behind a second one. A landing area holds [rank][four columns][128 rows] x 16 bytes,
+// a warp's rows side by side (with a column's rows side by side, 4 bytes a push, the exchange alone took 15 us).
+template <int BN, int EPI, typename OUT>
+__global__ void __launch_bounds__(THREADS_TC, 1)
+int8_split_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Int8Params p) {
+  constexpr bool DUAL = EPI == EPI_SWIGLU;
+  constexpr int F = DUAL ? BN / 2 : BN;
+  typedef TcCfg<BN> C;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t acc_full;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+  __shared__ int never_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int splits = p.splits, rank = (int)cluster_rank(), tile = blockIdx.x;
+  const int t_tiles = (p.T + BM - 1) / BM;
+  const int t0 = tile % t_tiles * BM, n0 = tile / t_tiles * F;
+  const int n_kb = (p.K + BK - 1) / BK, kb0 = rank * n_kb / splits, mine = (rank + 1) * n_kb / splits - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    mbar_init(&acc_full, 1);
+    abort_flag = 0;
+    never_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) { prefetch_tensormap(&tmap_w); prefetch_tensormap(&tmap_x); }
+  if (warp == 1) { tmem_alloc(&tmem_base_slot, C::TMEM_COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch();
+  const uint32_t tmem_base = tmem_base_slot;
+  bool got = false;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t bytes = (uint32_t)(C::B_BYTES + p.box * BK), st0 = smem_u32(smem);
+      const int pre = min(mine, C::STAGES);
+      auto weights = [&](int s, int kb) {
+        const uint32_t dst = st0 + s * C::STAGE_BYTES + C::A_BYTES, full = smem_u32(&full_bar[s]);
+        tma_load_2d(dst, &tmap_w, full, kb * BK, n0);
+        if (DUAL) tma_load_2d(dst + F * BK, &tmap_w, full, kb * BK, p.N + n0);
+      };
+      for (int i = 0; i < pre; ++i) { mbar_expect_tx(&full_bar[i], bytes); weights(i, kb0 + i); }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) tma_load_2d(st0 + i * C::STAGE_BYTES, &tmap_x, smem_u32(&full_bar[i]), (kb0 + i) * BK, t0);
+      int it = pre;
+      for (; it < mine; ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&empty_bar[s], (uint32_t)(it / C::STAGES - 1) & 1u, &abort_flag)) {
+          abort_flag = 1; record_failure(p.err, 5); break;
+        }
+        mbar_expect_tx(&full_bar[s], bytes);
+        weights(s, kb0 + it);
+        tma_load_2d(st0 + s * C::STAGE_BYTES, &tmap_x, smem_u32(&full_bar[s]), (kb0 + it) * BK, t0);
+      }
+      if (abort_flag)
+        for (int i = max(0, it - C::STAGES); i < it; ++i)
+          mbar_wait(&full_bar[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, &never_flag, 200000000LL);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_i8(BM, BN);
+      const uint64_t d0 = umma_desc_sw128(smem_u32(smem));
+      bool ok = true;
+      for (int it = 0; it < mine; ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&full_bar[s], (uint32_t)(it / C::STAGES) & 1u, &abort_flag)) { abort_flag = 1; record_failure(p.err, 2); ok = false; break; }
+        tc_fence_after();
+        const uint64_t da = d0 + (uint64_t)(s * (C::STAGE_BYTES >> 4)), db = da + (uint64_t)(C::A_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          umma_i8(tmem_base, da + (uint64_t)(k * UMMA_K / 16), db + (uint64_t)(k * UMMA_K / 16), idesc, it > 0 || k > 0);
+        umma_commit(&empty_bar[s]);
+      }
+      if (ok) umma_commit(&acc_full);
+    }
+  } else {
+    pdl_wait();
+    got = mbar_wait(&acc_full, 0u, &abort_flag);
+    if (!got) { abort_flag = 1; record_failure(p.err, 3); }
+    got = __all_sync(0xffffffffu, got);
+    tc_fence_after();
+  }
+  __syncwarp();
+  cluster_sync_all();                                    // every rank's products have read its ring
+  const int part = F / splits;                           // features that a rank finishes
+  const int row = (warp & 3) * 32 + lane, grp = (warp - 2) >> 2;
+  const bool rows_live = warp >= 2 && t0 + (warp & 3) * 32 < p.T;
+  const uint32_t land = smem_u32(smem);
+  if (rows_live && got) {
+    const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
+    for (int c = 16 * grp; c < BN; c += 32) {            // 16 columns at a time, dealt out to the two warps of a quarter
+      uint32_t a[16];
+      tmem_ld16(taddr + c, a);
+      tmem_ld_wait();
+      const int f = c % F, owner = f / part;
+      const int col = rank * (BN / splits) + c / F * part + f % part;
+      const uint32_t dst = map_to_rank(land + (uint32_t)((col >> 2) * 128 + row) * 16, (uint32_t)owner);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 * i), "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]) : "memory");
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();                                    // every part has landed
+  if (rows_live && got) {
+    const int t = t0 + row;
+    const float sx = t < p.T ? p.sx[t] : 0.f;
+    const int4* src = reinterpret_cast<const int4*>(smem) + row;
+    auto add_up = [&](int col, int (&a)[16]) {           // 16 columns from `col` of a rank's area on, over the ranks
+#pragma unroll
+      for (int i = 0; i < 16; ++i) a[i] = 0;
+      for (int z = 0; z < splits; ++z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int4 q = src[((z * (BN / splits) + col) / 4 + i) * 128];
+          a[4 * i] += q.x; a[4 * i + 1] += q.y; a[4 * i + 2] += q.z; a[4 * i + 3] += q.w;
+        }
+      }
+    };
+#pragma unroll 1
+    for (int c = 16 * grp; c < part; c += 32) {
+      const int n = n0 + rank * part + c;
+      if (n >= p.N) break;
+      int a[16], b[DUAL ? 16 : 1];
+      add_up(c, a);
+      if constexpr (DUAL) add_up(part + c, b);
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int ni = min(n + i, p.N - 1);
+        v[i] = (float)a[i] * sx * __ldg(p.sw + ni);
+        if constexpr (DUAL) v[i] = silu_gate(v[i], (float)b[i] * sx * __ldg(p.sw + p.N + ni), sizeof(OUT) == 4);
+      }
+      if (t < p.T) emit_row<EPI, OUT, 16>(p, t, n, v);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, C::TMEM_COLS); }
+}
+
 // ------------------------------------------------------------------------------------ host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -278,8 +432,7 @@ template <int BN, int EPI, typename OUT>
 int launch_tc(const void* x, const void* w, Int8Params p, int sm_count, cudaStream_t s) {
   typedef TcCfg<BN> C;
   constexpr int F = EPI == EPI_SWIGLU ? BN / 2 : BN;
-  static bool configured[64] = {};
-  if (allow_dynamic_smem(int8_tc_kernel<BN, EPI, OUT>, C::SMEM_BYTES, configured)) return -5;
+  static bool configured[64] = {}, configured_split[64] = {};
   p.box = p.T >= BM ? BM : (p.T + 7) / 8 * 8;
   CUtensorMap mx, mw;
   int rc = make_map(&mx, x, p.T, p.K, p.box);
@@ -287,20 +440,35 @@ int launch_tc(const void* x, const void* w, Int8Params p, int sm_count, cudaStre
   if (rc) return rc;
   const long long tiles = (long long)((p.T + BM - 1) / BM) * ((p.N + F - 1) / F);
   if (tiles > 2147483647LL) return ERR_TOO_LARGE;
+  if (p.splits > 1) {
+    if (allow_dynamic_smem(int8_split_kernel<BN, EPI, OUT>, C::SMEM_BYTES, configured_split)) return -5;
+    return launch_ex(int8_split_kernel<BN, EPI, OUT>, dim3((unsigned)tiles, 1, p.splits), dim3(THREADS_TC), C::SMEM_BYTES, s, p.splits, mx, mw, p);
+  }
+  if (allow_dynamic_smem(int8_tc_kernel<BN, EPI, OUT>, C::SMEM_BYTES, configured)) return -5;
   return launch_ex(int8_tc_kernel<BN, EPI, OUT>, dim3((unsigned)(tiles < sm_count ? tiles : sm_count)), dim3(THREADS_TC), C::SMEM_BYTES, s, 1, mx, mw, p);
 }
 
-// Weight rows a tile: the widest that still gives most SMs one, since a CTA reads its token tile again for every weight tile.
-int tile_rows(int T, int rows, int sm_count) {
-  const long long t_tiles = (T + BM - 1) / BM;
-  for (int bn = 256; bn > 64; bn >>= 1)
-    if (t_tiles * ((rows + bn - 1) / bn) * 4 >= 3ll * sm_count) return bn;
-  return 64;
+// Weight rows a tile and ranges of K, by the time in us of the CTA with the most to do: 0.26 a block of K, tile after tile, or of its range and 2.5 and
+// a us for 40 KB of the exchange; a wide tile's epilogue 0.002 a row.
+void plan(int epi, int T, int N, int K, int sm_count, int& bn, int& splits) {
+  const int half = epi == EPI_SWIGLU ? 2 : 1, rows = half * N, box = T >= BM ? BM : (T + 7) / 8 * 8;
+  const long long t_tiles = (T + BM - 1) / BM, n_kb = (K + BK - 1) / BK;
+  double best = 1e30;
+  for (int b = 256; b >= 64; b >>= 1)
+    for (int z = 1; z <= 4; z <<= 1) {
+      const long long tiles = t_tiles * ((rows + b - 1) / b);
+      if (z > 1 && (b / half / z < 16 || n_kb < 4 * z || tiles * z > sm_count)) break;
+      const long long rounds = (tiles * z + sm_count - 1) / sm_count;
+      const double cost = 0.26 * (double)(rounds * ((n_kb + z - 1) / z)) + (z > 1 ? 2.5 + 1e-4 * b * box : 0.0) + 0.002 * (double)(rounds * b);
+      if (cost < best) { best = cost; bn = b; splits = z; }
+    }
 }
 
 template <int EPI, typename OUT>
-int launch_epi(const void* x, const void* w, const Int8Params& p, int sm_count, cudaStream_t s) {
-  switch (tile_rows(p.T, EPI == EPI_SWIGLU ? 2 * p.N : p.N, sm_count)) {
+int launch_epi(const void* x, const void* w, Int8Params p, int sm_count, cudaStream_t s) {
+  int bn = 64;
+  plan(EPI, p.T, p.N, p.K, sm_count, bn, p.splits);
+  switch (bn) {
     case 256: return launch_tc<256, EPI, OUT>(x, w, p, sm_count, s);
     case 128: return launch_tc<128, EPI, OUT>(x, w, p, sm_count, s);
     default: return launch_tc<64, EPI, OUT>(x, w, p, sm_count, s);
@@ -308,6 +476,14 @@ int launch_epi(const void* x, const void* w, const Int8Params& p, int sm_count, 
 }
 
 }  // namespace
+
+// The tile and the ranges that rllm_int8_gemm takes (for measurement).
+RLLM_API int rllm_int8_plan(int epi, int T, int N, int K, int sm_count, int* bn, int* splits) {
+  if (epi < 0 || epi > 3 || T <= 0 || N <= 0 || K <= 0 || sm_count <= 0) return ERR_BAD_SIZE;
+  *bn = 64; *splits = 1;
+  plan(epi, T, N, K, sm_count, *bn, *splits);
+  return 0;
+}
 
 // x int8 [T, K] with scales sx [T]; w int8 [N, K] (SwiGLU: [2 N, K], gate rows first) with scales sw; K a multiple of 16, both
 // 16-byte aligned. y [T, N] in out_dt (epilogues 0 and 3) or float (1, 2: added), row stride ldy.
@@ -318,7 +494,7 @@ RLLM_API int rllm_int8_gemm(int epi, int out_dt, const void* x, const float* sx,
   if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
   if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
   const int size = epi == EPI_STORE_F32 || epi == EPI_ACCUM_F32 || out_dt == DT_F32 ? 4 : 2;
-  const Int8Params p = {sx, sw, y, ldy, !((uintptr_t)y & 15) && ldy * size % 16 == 0, T, N, K, 0, err};
+  const Int8Params p = {sx, sw, y, ldy, !((uintptr_t)y & 15) && ldy * size % 16 == 0, T, N, K, 0, 1, err};
   cudaStream_t s = (cudaStream_t)stream;
   if (epi == EPI_STORE_F32) return launch_epi<EPI_STORE_F32, float>(x, w, p, sm_count, s);
   if (epi == EPI_ACCUM_F32) return launch_epi<EPI_ACCUM_F32, float>(x, w, p, sm_count, s);

@@ -1,6 +1,6 @@
 // Products in 8-bit integers for few tokens: Y[t, n] = (sum_k X[t, k] W[n, k]) * sx[t] * sw[n], X quantised on the way.
 //
-// Up to 16 tokens the product is a read of W. A job is a slab of 16 weight rows (SwiGLU: a gate and an up slab); the warps of a CTA share
+// Up to 8 tokens the product is a read of W. A job is a slab of 16 weight rows (SwiGLU: a gate and an up slab); the warps of a CTA share
 // K, every warp copies its own pieces (16 rows x 256 codes, 4 KB) with cp.async into a ring of its own and multiplies with mma.sync
 // m16n8k16 in half precision: weights are the A operand, tokens the B operand, the contraction index permuted alike on both sides so
 // that the 16 bytes that a lane reads are fragments. (The instruction's 8-bit form takes some 200 cycles here: 1 token of 14,336 numbers
@@ -35,7 +35,6 @@ struct StreamParams {
 
 constexpr int SNT = 8, SCK = 256, SCHUNK = 16 * SCK;
 constexpr int SUMS = 4;              // slabs' sums, of 8 tokens each, that lie in shared memory together
-// (The largest form takes 226.1 KB with what is declared in the kernel; a CTA may have 227.)
 template <int WARPS> struct StreamCfg {
   static constexpr int THREADS = WARPS * 32, RING = 48 / WARPS;          // 192 KB on the way
   static constexpr int RING_BYTES = WARPS * RING * SCHUNK;
@@ -47,14 +46,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Bytes 0, 1 (hi: 2, 3) of a word of codes + 128 as two half numbers. HERE: made where it stands (the tokens' fragments of a long row,
-// all made before the loop over the weights, do not fit the registers).
-template <bool HERE = false>
+// Bytes 0, 1 (hi: 2, 3) of a word of codes + 128 as two half numbers.
 __device__ __forceinline__ uint32_t halves(uint32_t w, bool hi) {
-  uint32_t v;                                             // 1024 + byte
-  const uint32_t c = 0x64806480u;                         // 1152
-  if (HERE) asm volatile("prmt.b32 %0, %1, %2, %3;" : "=r"(v) : "r"(w), "r"(0x64646464u), "r"(hi ? 0x4342 : 0x4140));
-  else v = __byte_perm(w, 0x64646464u, hi ? 0x4342 : 0x4140);
+  const uint32_t v = __byte_perm(w, 0x64646464u, hi ? 0x4342 : 0x4140), c = 0x64806480u;        // 1024 + byte, 1152
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -105,15 +99,15 @@ __device__ __forceinline__ void load16(const StreamParams& p, const void* xrow, 
   }
 }
 
-// TILES: 2 with SwiGLU; NCH: pieces of K a warp has; G: groups of 8 tokens
-template <bool F32, int TILES, int WARPS, int NCH, int G>
+// TILES: 2 with SwiGLU; NCH: pieces of K a warp has
+template <bool F32, int TILES, int WARPS, int NCH>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 int8_stream_kernel(const StreamParams p) {
   typedef StreamCfg<WARPS> C;
-  constexpr int RING = C::RING, THREADS = C::THREADS, BATCH = SUMS / (TILES * G);
+  constexpr int RING = C::RING, THREADS = C::THREADS, BATCH = SUMS / TILES;
   extern __shared__ __align__(128) uint8_t stream_smem[];
-  __shared__ float s_max[WARPS][SNT * G], s_sq[WARPS][SNT * G], s_scale[SNT * G];
-  int* red = reinterpret_cast<int*>(stream_smem + C::RING_BYTES);        // [job of batch][tile][group][warp][row][token]
+  __shared__ float s_max[WARPS][SNT], s_sq[WARPS][SNT], s_scale[SNT];
+  int* red = reinterpret_cast<int*>(stream_smem + C::RING_BYTES);        // [job of batch][tile][warp][row][token]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(stream_smem) + warp * (RING * SCHUNK);
   const int my_jobs = p.njobs > (int)blockIdx.x ? (p.njobs - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
@@ -142,67 +136,59 @@ int8_stream_kernel(const StreamParams p) {
   for (int i = 0; i < RING; ++i) produce();
   pdl_wait();
 
-  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[piece][group][step] words of codes + 128
-  constexpr bool KEEP = NCH * G == 1;                     // the numbers stay in registers between the two looks
-  uint32_t b[NCH][G][4][4];
+  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[piece][step] words of codes + 128
+  constexpr bool KEEP = NCH == 1;                         // the numbers stay in registers between the two looks
+  uint32_t b[NCH][4][4];
   {
-    const uint8_t* xr[G];
-    float keep[KEEP ? 4 : 1][16];
+    const int tok = min(g, p.T - 1);                      // tokens beyond the last one: its codes again, never stored
+    const uint8_t* xr = (const uint8_t*)p.x + (size_t)(p.rows ? p.rows[tok] : tok) * p.ldx * (F32 ? 4 : 2);
+    float keep[KEEP ? 4 : 1][16], mx = 0.f, ss = 0.f, bad = 0.f;
+    auto look = [&](int c, float (&v)[4][16]) {
 #pragma unroll
-    for (int q = 0; q < G; ++q) {
-      const int tok = min(SNT * q + g, p.T - 1);          // tokens beyond the last one: its codes again, never stored
-      xr[q] = (const uint8_t*)p.x + (size_t)(p.rows ? p.rows[tok] : tok) * p.ldx * (F32 ? 4 : 2);
-      float mx = 0.f, ss = 0.f, bad = 0.f;
-      auto look = [&](int c, float (&v)[4][16]) {
+      for (int kb = 0; kb < 4; ++kb) load16<F32>(p, xr, (warp * NCH + c) * SCK + 64 * kb + 16 * t, v[kb], ss);
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) load16<F32>(p, xr[q], (warp * NCH + c) * SCK + 64 * kb + 16 * t, v[kb], ss);
+      for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) { mx = fmaxf(mx, fabsf(v[kb][i])); bad = fmaf(v[kb][i], 0.f, bad); }
-      };
-      if constexpr (KEEP) look(0, keep);
-      else {
+        for (int i = 0; i < 16; ++i) { mx = fmaxf(mx, fabsf(v[kb][i])); bad = fmaf(v[kb][i], 0.f, bad); }
+    };
+    if constexpr (KEEP) look(0, keep);
+    else {
 #pragma unroll 1
-        for (int c = 0; c < NCH; ++c) { float v[4][16]; look(c, v); }
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        bad += __shfl_xor_sync(0xffffffffu, bad, o);
-      }
-      if (t == 0) { s_max[warp][SNT * q + g] = bad == 0.f ? mx : INFINITY; s_sq[warp][SNT * q + g] = ss; }
+      for (int c = 0; c < NCH; ++c) { float v[4][16]; look(c, v); }
     }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      bad += __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    if (t == 0) { s_max[warp][g] = bad == 0.f ? mx : INFINITY; s_sq[warp][g] = ss; }
     __syncthreads();
+    mx = ss = 0.f;
 #pragma unroll
-    for (int q = 0; q < G; ++q) {
-      float mx = 0.f, ss = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        mx = fmaxf(mx, s_max[w][SNT * q + g]);
-        ss += s_sq[w][SNT * q + g];
-      }
-      const float rstd = p.g ? rsqrtf(ss / (float)p.xk + p.eps) : 1.f;
-      const float amax = mx * rstd;
-      const bool whole = mx <= 3.402823466e38f && amax <= 3.402823466e38f;      // every number finite
-      const float s = __fdiv_rn(amax, 127.f);
-      const bool codes = whole && s > 0.f;
-      const Rounding rd(codes ? s : 1.f);
-      if (warp == 0 && t == 0) s_scale[SNT * q + g] = whole ? s : __int_as_float(0x7fc00000);
-#pragma unroll
-      for (int ci = 0; ci < NCH; ++ci)
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          float fresh[16], unused = 0.f;
-          if (!KEEP) load16<F32>(p, xr[q], (warp * NCH + ci) * SCK + 64 * kb + 16 * t, fresh, unused);
-          float (&v)[16] = KEEP ? keep[KEEP ? kb : 0] : fresh;
-          uint32_t w[4] = {0u, 0u, 0u, 0u};
-          if (codes) codes8<16>(v, rstd, rd, w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b[ci][q][kb][i] = w[i] ^ 0x80808080u;
-        }
+    for (int w = 0; w < WARPS; ++w) {
+      mx = fmaxf(mx, s_max[w][g]);
+      ss += s_sq[w][g];
     }
+    const float rstd = p.g ? rsqrtf(ss / (float)p.xk + p.eps) : 1.f;
+    const float amax = mx * rstd;
+    const bool whole = mx <= 3.402823466e38f && amax <= 3.402823466e38f;      // every number finite
+    const float s = __fdiv_rn(amax, 127.f);
+    const bool codes = whole && s > 0.f;
+    const Rounding rd(codes ? s : 1.f);
+    if (warp == 0 && t == 0) s_scale[g] = whole ? s : __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int ci = 0; ci < NCH; ++ci)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        float fresh[16], unused = 0.f;
+        if (!KEEP) load16<F32>(p, xr, (warp * NCH + ci) * SCK + 64 * kb + 16 * t, fresh, unused);
+        float (&v)[16] = KEEP ? keep[KEEP ? kb : 0] : fresh;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (codes) codes8<16>(v, rstd, rd, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[ci][kb][i] = w[i] ^ 0x80808080u;
+      }
   }
 
   int cslot = 0;
@@ -212,13 +198,13 @@ int8_stream_kernel(const StreamParams p) {
     for (int jb = 0; jb < nb; ++jb) {
 #pragma unroll
       for (int tile = 0; tile < TILES; ++tile) {
-        int acc[G][4] = {};
+        int acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int ci = 0; ci < NCH; ++ci) {
           asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
           __syncwarp();
           const uint32_t src = ring + cslot * SCHUNK + frag_off;
-          float sum[G][4] = {};
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb) {
             const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
@@ -229,38 +215,31 @@ int8_stream_kernel(const StreamParams p) {
             for (int i = 0; i < 4; ++i) {
               const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u;
               const uint32_t a0 = halves(u, false), a1 = halves(v, false), a2 = halves(u, true), a3 = halves(v, true);
-#pragma unroll
-              for (int q = 0; q < G; ++q)
-                mma_f16(sum[q], a0, a1, a2, a3, halves<(NCH * G > 2)>(b[ci][q][kb][i], false), halves<(NCH * G > 2)>(b[ci][q][kb][i], true));
+              mma_f16(sum, a0, a1, a2, a3, halves(b[ci][kb][i], false), halves(b[ci][kb][i], true));
             }
           }
 #pragma unroll
-          for (int q = 0; q < G; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[q][i] += __float2int_rn(sum[q][i]);
+          for (int i = 0; i < 4; ++i) acc[i] += __float2int_rn(sum[i]);
           cslot = cslot + 1 == RING ? 0 : cslot + 1;
           __syncwarp();                                   // every lane has read the slot that is refilled now
           produce();
         }
-#pragma unroll
-        for (int q = 0; q < G; ++q) {
-          int* r = red + ((size_t)(((jb * TILES + tile) * G + q) * WARPS + warp)) * (16 * SNT);
-          *reinterpret_cast<int2*>(r + g * SNT + sum_col(g, 2 * t)) = make_int2(acc[q][0], acc[q][1]);
-          *reinterpret_cast<int2*>(r + (g + 8) * SNT + sum_col(g + 8, 2 * t)) = make_int2(acc[q][2], acc[q][3]);
-        }
+        int* r = red + (size_t)((jb * TILES + tile) * WARPS + warp) * (16 * SNT);
+        *reinterpret_cast<int2*>(r + g * SNT + sum_col(g, 2 * t)) = make_int2(acc[0], acc[1]);
+        *reinterpret_cast<int2*>(r + (g + 8) * SNT + sum_col(g + 8, 2 * t)) = make_int2(acc[2], acc[3]);
       }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nb * (16 * SNT * G); e += THREADS) {
-      const int jb = e / (16 * SNT * G), tok = (e >> 4) & (SNT * G - 1), r = e & 15;
+    for (int e = threadIdx.x; e < nb * (16 * SNT); e += THREADS) {
+      const int jb = e / (16 * SNT), tok = (e >> 4) & (SNT - 1), r = e & 15;
       const int n = (blockIdx.x + (batch0 + jb) * gridDim.x) * 16 + r;
       if (tok >= p.T || n >= p.N) continue;
       int s0 = 0, s1 = 0;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const int* part = red + (size_t)((jb * TILES * G + tok / SNT) * WARPS + w) * (16 * SNT) + r * SNT + sum_col(r, tok % SNT);
+        const int* part = red + (size_t)(jb * TILES * WARPS + w) * (16 * SNT) + r * SNT + sum_col(r, tok);
         s0 += part[0];
-        if (TILES == 2) s1 += part[G * WARPS * 16 * SNT];
+        if (TILES == 2) s1 += part[WARPS * 16 * SNT];
       }
       const float sx = s_scale[tok], v = (float)s0 * sx * __ldg(p.sw + n);
       const size_t o = (size_t)tok * p.ldy + n;
@@ -273,33 +252,28 @@ int8_stream_kernel(const StreamParams p) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool F32, int TILES, int WARPS, int NCH, int G>
+template <bool F32, int TILES, int WARPS, int NCH>
 int launch_stream(const StreamParams& p, int sm_count, cudaStream_t s) {
   typedef StreamCfg<WARPS> C;
   static bool configured[64] = {};
-  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, WARPS, NCH, G>, C::SMEM_BYTES, configured)) return -5;
-  return launch_ex(int8_stream_kernel<F32, TILES, WARPS, NCH, G>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(C::THREADS), C::SMEM_BYTES, s, 1, p);
+  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, WARPS, NCH>, C::SMEM_BYTES, configured)) return -5;
+  return launch_ex(int8_stream_kernel<F32, TILES, WARPS, NCH>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(C::THREADS), C::SMEM_BYTES, s, 1, p);
 }
 
-// What the kernel takes: fragments of all of K in registers, four pieces a warp (two with two groups of tokens); rows that 16-byte loads
-// read, a norm in front of float ones only.
+// What the kernel takes: fragments of all of K in registers, two pieces a warp; rows that 16-byte loads read, a norm in front of float ones
+// only. (Beyond 8,192 numbers a CTA has too much to quantise: 8 tokens, 14,336 to 4,096 29 us, on tcgen05 with ranges of K 22. With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
+// tcgen05 behind a kernel that quantises 11.)
 bool streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g) {
-  if (T > 2 * SNT || xk % 8 || xk > 16 * (T <= SNT ? 4 : 2) * SCK || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
+  if (T > SNT || xk % 8 || xk > 16 * 2 * SCK || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
   return x_dt == DT_F32 ? ldx % 4 == 0 : ldx % 8 == 0 && !g;
 }
 
 template <bool F32, int TILES>
 int launch_stream_k(const StreamParams& p, int sm_count, cudaStream_t s) {
   const int pieces = (p.K + SCK - 1) / SCK;
-  if (p.T > SNT) {
-    if (pieces <= 8) return launch_stream<F32, TILES, 8, 1, 2>(p, sm_count, s);
-    if (pieces <= 16) return launch_stream<F32, TILES, 16, 1, 2>(p, sm_count, s);
-    return launch_stream<F32, TILES, 16, 2, 2>(p, sm_count, s);
-  }
-  if (pieces <= 8) return launch_stream<F32, TILES, 8, 1, 1>(p, sm_count, s);
-  if (pieces <= 16) return launch_stream<F32, TILES, 16, 1, 1>(p, sm_count, s);
-  if (pieces <= 32) return launch_stream<F32, TILES, 16, 2, 1>(p, sm_count, s);
-  return launch_stream<F32, TILES, 16, 4, 1>(p, sm_count, s);
+  if (pieces <= 8) return launch_stream<F32, TILES, 8, 1>(p, sm_count, s);
+  if (pieces <= 16) return launch_stream<F32, TILES, 16, 1>(p, sm_count, s);
+  return launch_stream<F32, TILES, 16, 2>(p, sm_count, s);
 }
 
 }  // namespace

@@ -3,7 +3,7 @@
 // step and, once at load, the rows of a weight.
 //
 // The row has to be read before its scale is known, so a CTA holds it: 256 threads with up to VPT groups of 8 numbers in registers
-// each (8,192 numbers with four groups), longer rows are read twice, the second time out of the caches. The bound is the
+// each (16,384 numbers with eight groups), longer rows are read twice, the second time out of the caches. The bound is the
 // read of x and the write of the codes; a quotient is a multiplication by 1 / s except next to a border (`codes8`), since
 // a division for every number took as long as the memory.
 // Codes lie in rows of a multiple of 16 bytes (`ldc`), the numbers behind K are zeros: the products' copies are whole pieces.
@@ -90,13 +90,12 @@ quantize_rows_kernel(const RowArgs a) {
   } else {
     for (int k = threadIdx.x * 8; k < K; k += THREADS * 8) look(k, keep[0]);
   }
-  mx = block_max(mx, red);
-  const float b = block_sum(bad, red);
+  mx = block_max(bad == 0.f ? mx : INFINITY, red);
   float rstd = 1.f;
   if (a.g) rstd = rsqrtf(block_sum(ss, red) / (float)K + a.eps);
   // the row's numbers are v * rstd; the largest is the largest v's, as rounding keeps order
   const float amax = mx * rstd;
-  const bool whole = b == 0.f && amax <= 3.402823466e38f;
+  const bool whole = mx <= 3.402823466e38f && amax <= 3.402823466e38f;      // every number finite
   const float s = __fdiv_rn(amax, 127.f);
   if (threadIdx.x == 0) a.scales[t] = whole ? s : __int_as_float(0x7fc00000);
   const bool codes = whole && s > 0.f;
@@ -134,6 +133,7 @@ int launch_rows(const RowArgs& a, int T_, cudaStream_t s) {
   if (groups <= 1) return launch_ex(quantize_rows_kernel<T, 1, VEC>, dim3(T_), dim3(THREADS), 0, s, 1, a);
   if (groups <= 2) return launch_ex(quantize_rows_kernel<T, 2, VEC>, dim3(T_), dim3(THREADS), 0, s, 1, a);
   if (groups <= 4) return launch_ex(quantize_rows_kernel<T, 4, VEC>, dim3(T_), dim3(THREADS), 0, s, 1, a);
+  if (groups <= 8) return launch_ex(quantize_rows_kernel<T, 8, VEC>, dim3(T_), dim3(THREADS), 0, s, 1, a);
   return launch_ex(quantize_rows_kernel<T, 0, VEC>, dim3(T_), dim3(THREADS), 0, s, 1, a);
 }
 

@@ -19,6 +19,7 @@ _P = c_void_p
 ops.register_signatures("quant", {
     "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, c_int, _P],
     "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, _P, c_int, _P],
+    "rllm_int8_plan": [c_int, c_int, c_int, c_int, c_int, _P, _P],
     "rllm_int8_linear": [c_int, c_int, c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int,
                          c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
@@ -155,7 +156,7 @@ def linear_int8(x: Int8Rows, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: 
 
 _NEEDS_SCRATCH = 1000000
 # Tokens up to which a product may quantise them itself (int8_stream.cu has the whole rule)
-STREAM_TOKENS = 16
+STREAM_TOKENS = 8
 
 
 def linear(x: torch.Tensor, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: torch.Tensor | None = None,

@@ -109,7 +109,7 @@ def test_rows_lie_apart():
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 2048), (2, 40, 33), (7, 130, 1000), (8, 515, 4096), (9, 256, 512), (16, 96, 8192), (17, 1000, 300),
          (33, 2048, 256), (64, 128, 14336), (65, 72, 96), (128, 513, 640), (129, 384, 1111), (200, 1001, 257), (300, 2050, 512),
-         (513, 300, 128), (1000, 260, 2048)]
+         (513, 300, 128), (1000, 260, 2048), (130, 96, 4096), (40, 4096, 4096), (100, 17, 8200), (20, 600, 1024)]
 
 
 def product_inputs(T, N, K, dtype, seed=0):
