@@ -299,8 +299,8 @@ def decode_supported(q: torch.Tensor, hd: int, scale: float) -> bool:
 
 def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
                          window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: the most keys of a sequence;
-    `splits`: that many ranges of keys (1 to 8, 16), None: by `decode_splits`."""
+    """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: about how many keys a sequence has
+    (for the number of ranges only); `splits`: that many ranges of keys (1 to 8, 16), None: by `decode_splits`."""
     k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
     S = kv_lens.numel()
     _queries(q, nh, nkv, hd, S)
@@ -390,7 +390,9 @@ def attention_kv4(q: torch.Tensor, tensors: dict, ctx, block_table: torch.Tensor
     if not fast or not decode_supported(q, hd, scale):
         return simt()
     if ctx.max_q_len == 1:
-        return attention_kv4_decode(q, tensors, ctx.kv_lens, block_table, nh, scale, window, ctx.max_kv_len)
+        # a captured step's bound serves contexts from half of it up
+        keys = ctx.max_kv_len * 3 // 4 if ctx.graph_safe else ctx.max_kv_len
+        return attention_kv4_decode(q, tensors, ctx.kv_lens, block_table, nh, scale, window, max(keys, 1))
     _queries(q, nh, tensors["k4"].shape[1], hd, ctx.num_tokens)
     out = q.new_empty((q.shape[0], nh * hd))
     for run in _runs(ctx):
