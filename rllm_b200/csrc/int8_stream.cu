@@ -1,7 +1,7 @@
 // Products in 8-bit integers for few tokens: Y[t, n] = (sum_k X[t, k] W[n, k]) * sx[t] * sw[n], X quantised on the way.
 //
 // Up to 8 tokens the product is a read of W. A job is a slab of 16 weight rows (SwiGLU: a gate and an up slab); the warps of a CTA share
-// K, every warp copies its own pieces (16 rows x 256 codes, 4 KB) with cp.async into a ring of its own and multiplies with mma.sync
+// K, every warp copies its own pieces (16 rows x 128 or 256 codes, 2 or 4 KB) with cp.async into a ring of its own and multiplies with mma.sync
 // m16n8k16 in half precision: weights are the A operand, tokens the B operand, the contraction index permuted alike on both sides so
 // that the 16 bytes that a lane reads are fragments. (The instruction's 8-bit form takes some 200 cycles here: 1 token of 14,336 numbers
 // with 4,096 outputs 34 us.) A code is an exact half number, 1024 + (code + 128) by one byte permutation for two of them, less 1152; a piece's
@@ -33,11 +33,14 @@ struct StreamParams {
   int epi, out_f32;
 };
 
-constexpr int SNT = 8, SCK = 256, SCHUNK = 16 * SCK;
-constexpr int SUMS = 4;              // slabs' sums, of 8 tokens each, that lie in shared memory together
-template <int WARPS> struct StreamCfg {
-  static constexpr int THREADS = WARPS * 32, RING = 48 / WARPS;          // 192 KB on the way
-  static constexpr int RING_BYTES = WARPS * RING * SCHUNK;
+constexpr int SNT = 8;
+constexpr int SUMS = 4;              // slabs' sums that lie in shared memory together
+constexpr int WARPS = 16, THREADS = WARPS * 32;
+// KB: steps of 64 numbers that a warp's piece of K has, 2 or 4. Rows of up to 2,048 numbers are shared by all 16 warps in pieces of 128.
+template <int KB> struct StreamCfg {
+  static constexpr int SCK = 64 * KB, CHUNK = 16 * SCK;                  // 128 or 256 codes of each of 16 rows
+  static constexpr int RING = 192 * 1024 / (WARPS * CHUNK);              // 192 KB on the way
+  static constexpr int RING_BYTES = WARPS * RING * CHUNK;
   static constexpr int SMEM_BYTES = RING_BYTES + SUMS * WARPS * 16 * SNT * 4;
 };
 
@@ -100,31 +103,32 @@ __device__ __forceinline__ void load16(const StreamParams& p, const void* xrow, 
 }
 
 // TILES: 2 with SwiGLU; NCH: pieces of K a warp has
-template <bool F32, int TILES, int WARPS, int NCH>
-__global__ void __launch_bounds__(WARPS * 32, 1)
+template <bool F32, int TILES, int KB, int NCH>
+__global__ void __launch_bounds__(THREADS, 1)
 int8_stream_kernel(const StreamParams p) {
-  typedef StreamCfg<WARPS> C;
-  constexpr int RING = C::RING, THREADS = C::THREADS, BATCH = SUMS / TILES;
+  typedef StreamCfg<KB> C;
+  constexpr int RING = C::RING, SCK = C::SCK, BATCH = SUMS / TILES;
+  constexpr int UNITS = SCK / 16, STEP = 32 / UNITS;      // 16-byte units of a row, rows a copy instruction brings
   extern __shared__ __align__(128) uint8_t stream_smem[];
   __shared__ float s_max[WARPS][SNT], s_sq[WARPS][SNT], s_scale[SNT];
   int* red = reinterpret_cast<int*>(stream_smem + C::RING_BYTES);        // [job of batch][tile][warp][row][token]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(stream_smem) + warp * (RING * SCHUNK);
+  const uint32_t ring = smem_u32(stream_smem) + warp * (RING * C::CHUNK);
   const int my_jobs = p.njobs > (int)blockIdx.x ? (p.njobs - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
   pdl_launch();
 
   int pj = 0, ptile = 0, pci = 0, pslot = 0;
-  const int crow = lane >> 4, cunit = lane & 15;          // a copy instruction brings 256 bytes of two rows
+  const int crow = lane / UNITS, cunit = lane % UNITS;
   auto produce = [&]() {
     if (pj < my_jobs) {
       const int n0 = (blockIdx.x + pj * gridDim.x) * 16;
       const int k = (warp * NCH + pci) * SCK + 16 * cunit;
       const int8_t* src = p.w + (size_t)(n0 + (ptile ? p.N : 0) + crow) * p.K + k;
-      const uint32_t dst = ring + pslot * SCHUNK + crow * 256 + ((cunit ^ (crow << 2)) << 4);
+      const uint32_t dst = ring + pslot * C::CHUNK + crow * SCK + ((cunit ^ ((crow & 1) << 2)) << 4);      // odd rows: units' bit 2 flipped
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool there = k < p.K && n0 + crow + 2 * i < p.N;
-        copy16(dst + i * 512, there ? src + (size_t)(2 * i) * p.K : p.w, there);
+      for (int i = 0; i < 16 / STEP; ++i) {
+        const bool there = k < p.K && n0 + crow + STEP * i < p.N;
+        copy16(dst + i * 512, there ? src + (size_t)(STEP * i) * p.K : p.w, there);
       }
       if (++pci == NCH) { pci = 0; if (++ptile == TILES) { ptile = 0; ++pj; } }
     }
@@ -138,23 +142,23 @@ int8_stream_kernel(const StreamParams p) {
 
   // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[piece][step] words of codes + 128
   constexpr bool KEEP = NCH == 1;                         // the numbers stay in registers between the two looks
-  uint32_t b[NCH][4][4];
+  uint32_t b[NCH][KB][4];
   {
     const int tok = min(g, p.T - 1);                      // tokens beyond the last one: its codes again, never stored
     const uint8_t* xr = (const uint8_t*)p.x + (size_t)(p.rows ? p.rows[tok] : tok) * p.ldx * (F32 ? 4 : 2);
-    float keep[KEEP ? 4 : 1][16], mx = 0.f, ss = 0.f, bad = 0.f;
-    auto look = [&](int c, float (&v)[4][16]) {
+    float keep[KEEP ? KB : 1][16], mx = 0.f, ss = 0.f, bad = 0.f;
+    auto look = [&](int c, float (&v)[KB][16]) {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) load16<F32>(p, xr, (warp * NCH + c) * SCK + 64 * kb + 16 * t, v[kb], ss);
+      for (int kb = 0; kb < KB; ++kb) load16<F32>(p, xr, (warp * NCH + c) * SCK + 64 * kb + 16 * t, v[kb], ss);
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) { mx = fmaxf(mx, fabsf(v[kb][i])); bad = fmaf(v[kb][i], 0.f, bad); }
     };
     if constexpr (KEEP) look(0, keep);
     else {
 #pragma unroll 1
-      for (int c = 0; c < NCH; ++c) { float v[4][16]; look(c, v); }
+      for (int c = 0; c < NCH; ++c) { float v[KB][16]; look(c, v); }
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -180,19 +184,23 @@ int8_stream_kernel(const StreamParams p) {
 #pragma unroll
     for (int ci = 0; ci < NCH; ++ci)
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
+      for (int kb = 0; kb < KB; ++kb) {
         float fresh[16], unused = 0.f;
         if (!KEEP) load16<F32>(p, xr, (warp * NCH + ci) * SCK + 64 * kb + 16 * t, fresh, unused);
         float (&v)[16] = KEEP ? keep[KEEP ? kb : 0] : fresh;
         uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (codes) codes8<16>(v, rstd, rd, w);
+        if (p.g) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] *= rstd;
+        }
+        if (codes) codes8<16>(v, rd, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) b[ci][kb][i] = w[i] ^ 0x80808080u;
       }
   }
 
   int cslot = 0;
-  const uint32_t frag_off = (uint32_t)(g * 256), frag_key = (uint32_t)((g & 1) << 2);
+  const uint32_t frag_off = (uint32_t)(g * SCK), frag_key = (uint32_t)((g & 1) << 2);
   for (int batch0 = 0; batch0 < my_jobs; batch0 += BATCH) {
     const int nb = min(BATCH, my_jobs - batch0);
     for (int jb = 0; jb < nb; ++jb) {
@@ -203,14 +211,14 @@ int8_stream_kernel(const StreamParams p) {
         for (int ci = 0; ci < NCH; ++ci) {
           asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
           __syncwarp();
-          const uint32_t src = ring + cslot * SCHUNK + frag_off;
+          const uint32_t src = ring + cslot * C::CHUNK + frag_off;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kb = 0; kb < 4; ++kb) {
+          for (int kb = 0; kb < KB; ++kb) {
             const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
             uint32_t lo[4], hi[4];
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(at));
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * 256));
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * SCK));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u;
@@ -252,28 +260,27 @@ int8_stream_kernel(const StreamParams p) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool F32, int TILES, int WARPS, int NCH>
+template <bool F32, int TILES, int KB, int NCH>
 int launch_stream(const StreamParams& p, int sm_count, cudaStream_t s) {
-  typedef StreamCfg<WARPS> C;
+  typedef StreamCfg<KB> C;
   static bool configured[64] = {};
-  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, WARPS, NCH>, C::SMEM_BYTES, configured)) return -5;
-  return launch_ex(int8_stream_kernel<F32, TILES, WARPS, NCH>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(C::THREADS), C::SMEM_BYTES, s, 1, p);
+  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, KB, NCH>, C::SMEM_BYTES, configured)) return -5;
+  return launch_ex(int8_stream_kernel<F32, TILES, KB, NCH>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(THREADS), C::SMEM_BYTES, s, 1, p);
 }
 
 // What the kernel takes: fragments of all of K in registers, two pieces a warp; rows that 16-byte loads read, a norm in front of float ones
 // only. (Beyond 8,192 numbers a CTA has too much to quantise: 8 tokens, 14,336 to 4,096 29 us, on tcgen05 with ranges of K 22. With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
 // tcgen05 behind a kernel that quantises 11.)
 bool streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g) {
-  if (T > SNT || xk % 8 || xk > 16 * 2 * SCK || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
+  if (T > SNT || xk % 8 || xk > WARPS * 2 * 256 || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
   return x_dt == DT_F32 ? ldx % 4 == 0 : ldx % 8 == 0 && !g;
 }
 
 template <bool F32, int TILES>
 int launch_stream_k(const StreamParams& p, int sm_count, cudaStream_t s) {
-  const int pieces = (p.K + SCK - 1) / SCK;
-  if (pieces <= 8) return launch_stream<F32, TILES, 8, 1>(p, sm_count, s);
-  if (pieces <= 16) return launch_stream<F32, TILES, 16, 1>(p, sm_count, s);
-  return launch_stream<F32, TILES, 16, 2>(p, sm_count, s);
+  if (p.K <= WARPS * 128) return launch_stream<F32, TILES, 2, 1>(p, sm_count, s);
+  if (p.K <= WARPS * 256) return launch_stream<F32, TILES, 4, 1>(p, sm_count, s);
+  return launch_stream<F32, TILES, 4, 2>(p, sm_count, s);
 }
 
 }  // namespace

@@ -41,25 +41,21 @@ static __device__ __noinline__ uint32_t codes8_exact(float a, float b, float c, 
   return ((uint32_t)min(max(round_quotient(a, s, inv), lo), hi) & 0xffu) | ((uint32_t)min(max(round_quotient(b, s, inv), lo), hi) & 0xffu) << 8 |
          ((uint32_t)min(max(round_quotient(c, s, inv), lo), hi) & 0xffu) << 16 | (uint32_t)min(max(round_quotient(d, s, inv), lo), hi) << 24;
 }
-// The 8-bit codes of N numbers v * k of a row with scale s > 0, four a word, `rd` the row's Rounding, k a factor on all of them. The exact
-// quotient lies between x times numbers just below and just above 1 / s; where both have the same nearest integer, it is that. (A division
+// The 8-bit codes of N numbers of a row with scale s > 0, four a word, `rd` the row's Rounding. The exact quotient lies between x times numbers just below and just above 1 / s; where both have the same nearest integer, it is that. (A division
 // for every number took as long again as a prompt's memory.)
 template <int N>
-__device__ __forceinline__ void codes8(const float (&v)[N], float k, const Rounding& rd, uint32_t (&w)[N / 4]) {
+__device__ __forceinline__ void codes8(const float (&v)[N], const Rounding& rd, uint32_t (&w)[N / 4]) {
   const float lo = rd.inv * (1.f - 2.384185791e-7f), hi = rd.inv * (1.f + 2.384185791e-7f);      // 2^-22, more than the two roundings of inv
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
-    uint32_t y[4], differ = 0u;
-    float x[4];
+    uint32_t y[4], differ = rd.up != 1.f;                // (a tiny scale may have been rounded far enough down for codes beyond 127)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[e] = v[i + e] * k * rd.up;
-      y[e] = __float_as_uint(fmaf(x[e], lo, 12582912.f));                // 1.5 2^23: the last byte is the code
-      differ |= y[e] ^ __float_as_uint(fmaf(x[e], hi, 12582912.f));
+      y[e] = __float_as_uint(fmaf(v[i + e], lo, 12582912.f));            // 1.5 2^23: the last byte is the code
+      differ |= y[e] ^ __float_as_uint(fmaf(v[i + e], hi, 12582912.f));
     }
     w[i / 4] = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
-    // (a tiny scale may have been rounded far enough down for codes beyond 127)
-    if (differ || rd.up != 1.f) w[i / 4] = codes8_exact(x[0], x[1], x[2], x[3], rd.s, rd.inv);
+    if (differ) w[i / 4] = codes8_exact(v[i] * rd.up, v[i + 1] * rd.up, v[i + 2] * rd.up, v[i + 3] * rd.up, rd.s, rd.inv);
   }
 }
 
