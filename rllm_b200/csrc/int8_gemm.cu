@@ -17,7 +17,7 @@ enum : int { EPI_STORE = 0, EPI_STORE_F32 = 1, EPI_ACCUM_F32 = 2, EPI_SWIGLU = 3
 struct Int8Params {
   const float* sx; const float* sw;
   void* y; long long ldy;
-  int vec;                           // rows of y start on 16 bytes
+  int vec;                           // rows of y start on 16 bytes, and so do scales of every fourth weight row (N % 4 == 0)
   int T, N, K;                       // N: outputs (of one half with SwiGLU); K: bytes a row, a multiple of 16
   int box;                           // token rows a copy brings
   int splits;                        // ranges of K
@@ -50,41 +50,78 @@ template <int BN> struct TcCfg {                      // BN: weight rows a tile 
   static constexpr int TMEM_COLS = 2 * BN <= 64 ? 64 : 2 * BN;
 };
 
-// CH neighbouring outputs of one token.
+// CH neighbouring outputs of one token, in rows that start on 16 bytes.
 template <int EPI, typename OUT, int CH>
 __device__ __forceinline__ void emit_row(const Int8Params& p, int t, int n, const float (&v)[CH]) {
-  if (EPI == EPI_ACCUM_F32) {
-    float* y = (float*)p.y + (size_t)t * p.ldy + n;
-    if (p.vec && n + CH <= p.N) {
-#pragma unroll
-      for (int i = 0; i < CH; i += 4)
-        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) if (n + i < p.N) atomicAdd(y + i, v[i]);
-    }
-    return;
-  }
   OUT* y = (OUT*)p.y + (size_t)t * p.ldy + n;
-  if (p.vec && n + CH <= p.N) {
-    if (sizeof(OUT) == 4) {
+  if (n + CH > p.N) {                                    // the last ones
 #pragma unroll
-      for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(y + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; i += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * e], v[i + 2 * e + 1]);
-          w[e] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(y + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < CH; ++i)
+      if (n + i < p.N) {
+        if constexpr (EPI == EPI_ACCUM_F32) atomicAdd(y + i, v[i]);
+        else y[i] = from_f32<OUT>(v[i]);
       }
+  } else if constexpr (EPI == EPI_ACCUM_F32) {
+#pragma unroll
+    for (int i = 0; i < CH; i += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
+  } else if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+    for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(y + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; i += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * e], v[i + 2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(y + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// The same in rows that start anywhere: a warp's block of 32 tokens (one a lane) x 16 outputs is turned first, in four steps of exchanges
+// between lanes, so that neighbouring lanes store neighbouring outputs. Number by number from each lane's row, 32 rows an
+// instruction, 333 tokens of 1,111 with 1,001 outputs took 14.5 us (the quantising in front included), turned 7.6.
+template <int EPI, typename OUT>
+__device__ __forceinline__ void emit_turned(const Int8Params& p, int t_warp, int n, float (&v)[16], int lane) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!(i & o)) {
+        const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i | o], o);
+        if (up) v[i] = got; else v[i | o] = got;
+      }
+  }
+  // v[i] is now output lane % 16 of the half warp's token i
+  const int col = n + (lane & 15), first = t_warp + (lane & 16);
+  if (col >= p.N) return;
+  OUT* y = (OUT*)p.y + (size_t)first * p.ldy + col;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (first + i < p.T) {
+      if constexpr (EPI == EPI_ACCUM_F32) atomicAdd(y + (size_t)i * p.ldy, v[i]);
+      else y[(size_t)i * p.ldy] = from_f32<OUT>(v[i]);
+    }
+}
+
+// Scales of the W weight rows from n on (what lies behind the last one is not used)
+template <int W>
+__device__ __forceinline__ void scales(const Int8Params& p, int n, float (&s)[W]) {
+  const int end = n < p.N ? p.N : 2 * p.N;               // (with SwiGLU up rows follow the gate rows)
+  if (p.vec) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(p.sw + min(n + i, end - 4)));
+      s[i] = q.x; s[i + 1] = q.y; s[i + 2] = q.z; s[i + 3] = q.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) if (n + i < p.N) y[i] = from_f32<OUT>(v[i]);
+    for (int i = 0; i < W; ++i) s[i] = __ldg(p.sw + min(n + i, end - 1));
   }
 }
 
@@ -104,22 +141,36 @@ __device__ __forceinline__ void tile_out(const Int8Params& p, uint32_t taddr, in
   if (t_warp >= p.T) return;
   const float sx = t < p.T ? p.sx[t] : 0.f;
   const int grp = (warp - 2) >> 2;
-#pragma unroll 1
-  for (int c = grp * (F / 2); c < (grp + 1) * (F / 2); c += CH) {
-    const int n = n0 + c;
-    if (n >= p.N) break;
-    uint32_t a[CH], b[DUAL ? CH : 1];
-    tmem_cols<CH>(taddr + c, a);
-    if constexpr (DUAL) tmem_cols<CH>(taddr + F + c, b);
+  auto numbers = [&](int c, int n, auto& v) {            // finished outputs c, c + 1 ... of the tile
+    constexpr int W = sizeof(v) / sizeof(float);
+    uint32_t a[W], b[DUAL ? W : 1];
+    tmem_cols<W>(taddr + c, a);
+    if constexpr (DUAL) tmem_cols<W>(taddr + F + c, b);
+    float sa[W], sb[DUAL ? W : 1];
+    scales(p, n, sa);
+    if constexpr (DUAL) scales(p, n + p.N, sb);
     tmem_ld_wait();
-    float v[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int ni = min(n + i, p.N - 1);
-      v[i] = (float)(int)a[i] * sx * __ldg(p.sw + ni);
-      if constexpr (DUAL) v[i] = silu_gate(v[i], (float)(int)b[i] * sx * __ldg(p.sw + p.N + ni), sizeof(OUT) == 4);
+    for (int i = 0; i < W; ++i) {
+      v[i] = (float)(int)a[i] * sx * sa[i];
+      if constexpr (DUAL) v[i] = silu_gate(v[i], (float)(int)b[i] * sx * sb[i], sizeof(OUT) == 4);
     }
-    if (t < p.T) emit_row<EPI, OUT, CH>(p, t, n, v);
+  };
+  const int end = min((grp + 1) * (F / 2), p.N - n0);
+  if (p.vec) {
+#pragma unroll 1
+    for (int c = grp * (F / 2); c < end; c += CH) {
+      float v[CH];
+      numbers(c, n0 + c, v);
+      if (t < p.T) emit_row<EPI, OUT, CH>(p, t, n0 + c, v);
+    }
+  } else {
+#pragma unroll 1
+    for (int c = grp * (F / 2); c < end; c += 16) {
+      float v[16];
+      numbers(c, n0 + c, v);
+      emit_turned<EPI, OUT>(p, t_warp, n0 + c, v, lane);
+    }
   }
 }
 
@@ -245,6 +296,151 @@ int8_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, C::TMEM_COLS); }
+}
+
+// ---------------------------------------------------------------------------- many tokens, two SMs a tile
+// The persistent scheme on pairs of CTAs (a cluster of two, cta_group::2): a tile is 256 tokens x 256 weight rows; each CTA of a pair loads its own
+// 128 tokens and its own half of the weight rows (SwiGLU: the gate rows in the even CTA, the up rows in the odd one) and keeps the accumulator
+// of its own tokens. The even CTA issues the MMAs, which read both CTAs' shared memory. A block of K takes 32 KB into and out of an SM's
+// shared memory where a tile of 128 x 256 on one SM takes 48: 0.36 us a block for twice the work of that kernel's 0.45. 512 tokens, 2 x 14,336 x 4,096
+// 56.6 -> 48.0 us (2.5 of the 3.3 Pop/s that twice the library's bfloat16 rate would be), 2,048 tokens 3.1 Pop/s with the tokens' quantising; with 16 blocks
+// of K a tile's start and end weigh more: 2,048 tokens, 2 x 8,192 x 2,048 51.7 -> 50.4, scales read four at a time 48.
+// Hand-overs as on the pairs of tc_gemm.cu: both CTAs' bytes are counted by the even CTA's `full` barrier, commits go to both CTAs' `empty`
+// and `acc_full`, both CTAs' epilogue warps arrive at the even CTA's `acc_empty`; both meet before TMEM is freed.
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+struct PairCfg {
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BM * BK, STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 6;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES;
+};
+constexpr long long PAIR_WAIT_CYCLES = 1000000000LL;     // about half a second
+
+template <int EPI, typename OUT>
+__global__ void __launch_bounds__(THREADS_TC, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Int8Params p) {
+  constexpr bool DUAL = EPI == EPI_SWIGLU;
+  constexpr int F = DUAL ? 128 : 256;                    // features a tile
+  typedef PairCfg C;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[C::STAGES];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+  __shared__ int never_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int rank = (int)cluster_rank();
+  const bool leader = rank == 0;
+  const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const int t_tiles = (p.T + 2 * BM - 1) / (2 * BM), n_tiles = (p.N + F - 1) / F;
+  const int tiles = t_tiles * n_tiles;
+  const int n_kb = (p.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }
+    abort_flag = 0;
+    never_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) { prefetch_tensormap(&tmap_w); prefetch_tensormap(&tmap_x); }
+  if (warp == 1) { tmem_alloc_pair(&tmem_base_slot, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cluster_sync_all();          // the peer's barriers exist before anything is signalled there
+  pdl_launch();
+  const uint32_t tmem_base = tmem_base_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      constexpr uint32_t stage_bytes = 2u * C::STAGE_BYTES;            // of both CTAs
+      const int mine = (tiles - pair_id + n_pairs - 1) / n_pairs * n_kb;
+      const int pre = min(mine, C::STAGES);
+      const uint32_t st0 = smem_u32(smem), even0 = map_to_rank(smem_u32(full_bar), 0);
+      auto weights = [&](int s, int tile, int kb) {
+        const int n0 = tile / t_tiles * F;
+        tma_load_2d_pair(st0 + s * C::STAGE_BYTES + C::A_BYTES, &tmap_w, even0 + 8 * s, kb * BK, DUAL ? n0 + rank * p.N : n0 + rank * BM);
+      };
+      auto tokens = [&](int s, int tile, int kb) {
+        tma_load_2d_pair(st0 + s * C::STAGE_BYTES, &tmap_x, even0 + 8 * s, kb * BK, tile % t_tiles * 2 * BM + rank * BM);
+      };
+      for (int i = 0; i < pre; ++i) {                    // (see the kernel above: weights need not wait)
+        if (leader) mbar_expect_tx(&full_bar[i], stage_bytes);
+        weights(i, pair_id + i / n_kb * n_pairs, i % n_kb);
+      }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) tokens(i, pair_id + i / n_kb * n_pairs, i % n_kb);
+      int it = pre, tile = pair_id + pre / n_kb * n_pairs, kb = pre % n_kb;
+      for (; it < mine; ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&empty_bar[s], (uint32_t)(it / C::STAGES - 1) & 1u, &abort_flag, PAIR_WAIT_CYCLES)) {
+          abort_flag = 1; record_failure(p.err, 5, rank); break;
+        }
+        if (leader) mbar_expect_tx(&full_bar[s], stage_bytes);
+        weights(s, tile, kb);
+        tokens(s, tile, kb);
+        if (++kb == n_kb) { kb = 0; tile += n_pairs; }
+      }
+      if (abort_flag && leader)                          // let copies already issued land before the shared memory is given back
+        for (int i = max(0, it - C::STAGES); i < it; ++i)
+          mbar_wait(&full_bar[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, &never_flag, 200000000LL);
+    }
+  } else if (warp == 1) {
+    if (elect_one() && leader) {
+      constexpr uint32_t idesc = umma_idesc_i8(2 * BM, 256);
+      const uint64_t d0 = umma_desc_sw128(smem_u32(smem));
+      int it = 0, ti = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < tiles && ok; tile += n_pairs, ++ti) {
+        const int buf = ti & 1, use = ti >> 1;
+        if (use > 0 && !mbar_wait(&acc_empty[buf], (uint32_t)(use - 1) & 1u, &abort_flag, PAIR_WAIT_CYCLES)) {
+          abort_flag = 1; record_failure(p.err, 6); ok = false; break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem_base + (uint32_t)(buf * 256);
+        for (int kb = 0; kb < n_kb; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&full_bar[s], (uint32_t)(it / C::STAGES) & 1u, &abort_flag, PAIR_WAIT_CYCLES)) { abort_flag = 1; record_failure(p.err, 2); ok = false; break; }
+          tc_fence_after();
+          const uint64_t da = d0 + (uint64_t)(s * (C::STAGE_BYTES >> 4)), db = da + (uint64_t)(C::A_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_i8_pair(acc, da + (uint64_t)(k * UMMA_K / 16), db + (uint64_t)(k * UMMA_K / 16), idesc, kb > 0 || k > 0);
+          umma_commit_pair_both(smem_u32(&empty_bar[s]));
+        }
+        if (ok) umma_commit_pair_both(smem_u32(&acc_full[buf]));
+      }
+    }
+  } else {
+    const uint32_t drained = map_to_rank(smem_u32(&acc_empty[0]), 0);
+    pdl_wait();
+    int ti = 0;
+    for (int tile = pair_id; tile < tiles; tile += n_pairs, ++ti) {
+      const int buf = ti & 1, use = ti >> 1;
+      bool got = mbar_wait(&acc_full[buf], (uint32_t)use & 1u, &abort_flag, PAIR_WAIT_CYCLES);
+      if (!got) { abort_flag = 1; record_failure(p.err, 3, rank); }
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(buf * 256);
+      tile_out<256, EPI, OUT>(p, taddr, tile % t_tiles * 2 * BM + rank * BM, tile / t_tiles * F, warp, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(drained + (uint32_t)(buf * 8));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();          // both CTAs are done with each other's shared memory, barriers and TMEM
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem_base, 512); }
 }
 
 // ---------------------------------------------------------------------------- few tiles: ranges of K
@@ -385,14 +581,16 @@ int8_split_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       int a[16], b[DUAL ? 16 : 1];
       add_up(c, a);
       if constexpr (DUAL) add_up(part + c, b);
-      float v[16];
+      float v[16], sa[16], sb[DUAL ? 16 : 1];
+      scales(p, n, sa);
+      if constexpr (DUAL) scales(p, n + p.N, sb);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int ni = min(n + i, p.N - 1);
-        v[i] = (float)a[i] * sx * __ldg(p.sw + ni);
-        if constexpr (DUAL) v[i] = silu_gate(v[i], (float)b[i] * sx * __ldg(p.sw + p.N + ni), sizeof(OUT) == 4);
+        v[i] = (float)a[i] * sx * sa[i];
+        if constexpr (DUAL) v[i] = silu_gate(v[i], (float)b[i] * sx * sb[i], sizeof(OUT) == 4);
       }
-      if (t < p.T) emit_row<EPI, OUT, 16>(p, t, n, v);
+      if (!p.vec) emit_turned<EPI, OUT>(p, t - lane, n, v, lane);
+      else if (t < p.T) emit_row<EPI, OUT, 16>(p, t, n, v);
     }
   }
   tc_fence_before();
@@ -448,20 +646,60 @@ int launch_tc(const void* x, const void* w, Int8Params p, int sm_count, cudaStre
   return launch_ex(int8_tc_kernel<BN, EPI, OUT>, dim3((unsigned)(tiles < sm_count ? tiles : sm_count)), dim3(THREADS_TC), C::SMEM_BYTES, s, 1, mx, mw, p);
 }
 
-// Weight rows a tile and ranges of K, by the time in us of the CTA with the most to do: 0.26 a block of K, tile after tile, or of its range and 2.5 and
-// a us for 40 KB of the exchange; a wide tile's epilogue 0.002 a row.
+template <int EPI, typename OUT>
+int launch_pair(const void* x, const void* w, Int8Params p, int sm_count, cudaStream_t s) {
+  static bool configured[64] = {};
+  if (allow_dynamic_smem(int8_pair_kernel<EPI, OUT>, PairCfg::SMEM_BYTES, configured)) return -5;
+  constexpr int F = EPI == EPI_SWIGLU ? 128 : 256;
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, x, p.T, p.K, BM);
+  if (!rc) rc = make_map(&mw, w, EPI == EPI_SWIGLU ? 2ll * p.N : p.N, p.K, BM);
+  if (rc) return rc;
+  const long long tiles = (long long)((p.T + 2 * BM - 1) / (2 * BM)) * ((p.N + F - 1) / F);
+  if (tiles > 1073741823LL) return ERR_TOO_LARGE;
+  const long long pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(THREADS_TC);
+  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = 2; attrs[0].val.clusterDim.y = 1; attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int8_pair_kernel<EPI, OUT>, mx, mw, p);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+  return 0;
+}
+
+// Weight rows a tile (512: pairs of CTAs, 256 x 256) and ranges of K, by an estimate of the time in us: the blocks of K of the CTA with the most
+// of them, `block` each (how many tokens hardly matters, nor how many CTAs are busy), a start and an end, and with ranges the
+// exchange of an accumulator. Fitted to 20 sizes of 32 to 2,048 tokens, each timed at every width and number of ranges; the choice was the best of
+// them, or within 8 % of it. Best | widths 64, 128, 256, pairs without ranges, us: 64 tokens, 2,048 x 8,192 7.9 (64 rows, 4 ranges) | 15.9, 18.1, 28.9;
+// 256 tokens of it 11.0 (128, 4) | 16.5, 19.3, 31.2, 27.0; 2,048 tokens of it 29.4 (pairs) | 55.7, 35.5, 31.1, 29.4; 2,048 tokens, 2 x 8,192 x 2,048
+// 50.4 (pairs) | 102, 64.3, 51.7, 50.4; 512 tokens, 2 x 14,336 x 4,096 48.0 (pairs) | 92.3, 60.9, 56.6, 48.0.
 void plan(int epi, int T, int N, int K, int sm_count, int& bn, int& splits) {
   const int half = epi == EPI_SWIGLU ? 2 : 1, rows = half * N, box = T >= BM ? BM : (T + 7) / 8 * 8;
-  const long long t_tiles = (T + BM - 1) / BM, n_kb = (K + BK - 1) / BK;
+  const long long n_kb = (K + BK - 1) / BK;
   double best = 1e30;
-  for (int b = 256; b >= 64; b >>= 1)
+  auto offer = [&](int b, int z, long long rounds, double block, double rest) {
+    const double cost = (double)(rounds * ((n_kb + z - 1) / z)) * block + rest;
+    if (cost < best) { best = cost; bn = b; splits = z; }
+  };
+  for (int b = 64; b <= 256; b <<= 1)
     for (int z = 1; z <= 4; z <<= 1) {
-      const long long tiles = t_tiles * ((rows + b - 1) / b);
+      const long long tiles = (long long)((T + BM - 1) / BM) * ((rows + b - 1) / b);
       if (z > 1 && (b / half / z < 16 || n_kb < 4 * z || tiles * z > sm_count)) break;
-      const long long rounds = (tiles * z + sm_count - 1) / sm_count;
-      const double cost = 0.26 * (double)(rounds * ((n_kb + z - 1) / z)) + (z > 1 ? 2.5 + 1e-4 * b * box : 0.0) + 0.002 * (double)(rounds * b);
-      if (cost < best) { best = cost; bn = b; splits = z; }
+      const double exchange = z > 1 ? 0.5 * z + 1.2e-4 * b * box * (z - 1) / z : 0.0;
+      offer(b, z, (tiles * z + sm_count - 1) / sm_count, b == 64 ? 0.215 : b == 128 ? 0.28 : 0.45, 1.8 + 0.005 * b + exchange);
     }
+  if (T > BM && sm_count >= 2) {
+    const long long tiles = (long long)((T + 2 * BM - 1) / (2 * BM)) * ((rows + 255) / 256), pairs = sm_count / 2;
+    offer(512, 1, (tiles + pairs - 1) / pairs, 0.375, 4.5);
+  }
 }
 
 template <int EPI, typename OUT>
@@ -469,6 +707,7 @@ int launch_epi(const void* x, const void* w, Int8Params p, int sm_count, cudaStr
   int bn = 64;
   plan(EPI, p.T, p.N, p.K, sm_count, bn, p.splits);
   switch (bn) {
+    case 512: return launch_pair<EPI, OUT>(x, w, p, sm_count, s);
     case 256: return launch_tc<256, EPI, OUT>(x, w, p, sm_count, s);
     case 128: return launch_tc<128, EPI, OUT>(x, w, p, sm_count, s);
     default: return launch_tc<64, EPI, OUT>(x, w, p, sm_count, s);
@@ -494,7 +733,7 @@ RLLM_API int rllm_int8_gemm(int epi, int out_dt, const void* x, const float* sx,
   if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
   if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
   const int size = epi == EPI_STORE_F32 || epi == EPI_ACCUM_F32 || out_dt == DT_F32 ? 4 : 2;
-  const Int8Params p = {sx, sw, y, ldy, !((uintptr_t)y & 15) && ldy * size % 16 == 0, T, N, K, 0, 1, err};
+  const Int8Params p = {sx, sw, y, ldy, !(((uintptr_t)y | (uintptr_t)sw) & 15) && ldy * size % 16 == 0 && N % 4 == 0, T, N, K, 0, 1, err};
   cudaStream_t s = (cudaStream_t)stream;
   if (epi == EPI_STORE_F32) return launch_epi<EPI_STORE_F32, float>(x, w, p, sm_count, s);
   if (epi == EPI_ACCUM_F32) return launch_epi<EPI_ACCUM_F32, float>(x, w, p, sm_count, s);

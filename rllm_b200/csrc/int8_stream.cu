@@ -5,7 +5,7 @@
 // m16n8k16 in half precision: weights are the A operand, tokens the B operand, the contraction index permuted alike on both sides so
 // that the 16 bytes that a lane reads are fragments. (The instruction's 8-bit form takes some 200 cycles here: 1 token of 14,336 numbers
 // with 4,096 outputs 34 us.) A code is an exact half number, 1024 + (code + 128) by one byte permutation for two of them, less 1152; a piece's
-// sum, below 2^22, is exact in float and added to the whole numbers of the pieces before. The warps' sums meet in shared memory in any
+// sum, below 2^22, is exact in float. The warps' sums meet in shared memory in any
 // order.
 // The tokens are quantised here, by every CTA for itself while its first weights are on their way: a lane's fragments are 16 numbers of
 // a token at a time, of which it needs the row's largest; the warps' maxima (and sums of squares, with an RMSNorm in front) meet once in
@@ -102,8 +102,8 @@ __device__ __forceinline__ void load16(const StreamParams& p, const void* xrow, 
   }
 }
 
-// TILES: 2 with SwiGLU; NCH: pieces of K a warp has
-template <bool F32, int TILES, int KB, int NCH>
+// TILES: 2 with SwiGLU
+template <bool F32, int TILES, int KB>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_stream_kernel(const StreamParams p) {
   typedef StreamCfg<KB> C;
@@ -117,12 +117,12 @@ int8_stream_kernel(const StreamParams p) {
   const int my_jobs = p.njobs > (int)blockIdx.x ? (p.njobs - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
   pdl_launch();
 
-  int pj = 0, ptile = 0, pci = 0, pslot = 0;
+  int pj = 0, ptile = 0, pslot = 0;
   const int crow = lane / UNITS, cunit = lane % UNITS;
   auto produce = [&]() {
     if (pj < my_jobs) {
       const int n0 = (blockIdx.x + pj * gridDim.x) * 16;
-      const int k = (warp * NCH + pci) * SCK + 16 * cunit;
+      const int k = warp * SCK + 16 * cunit;
       const int8_t* src = p.w + (size_t)(n0 + (ptile ? p.N : 0) + crow) * p.K + k;
       const uint32_t dst = ring + pslot * C::CHUNK + crow * SCK + ((cunit ^ ((crow & 1) << 2)) << 4);      // odd rows: units' bit 2 flipped
 #pragma unroll
@@ -130,7 +130,7 @@ int8_stream_kernel(const StreamParams p) {
         const bool there = k < p.K && n0 + crow + STEP * i < p.N;
         copy16(dst + i * 512, there ? src + (size_t)(STEP * i) * p.K : p.w, there);
       }
-      if (++pci == NCH) { pci = 0; if (++ptile == TILES) { ptile = 0; ++pj; } }
+      if (++ptile == TILES) { ptile = 0; ++pj; }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     pslot = pslot + 1 == RING ? 0 : pslot + 1;
@@ -140,26 +140,18 @@ int8_stream_kernel(const StreamParams p) {
   for (int i = 0; i < RING; ++i) produce();
   pdl_wait();
 
-  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[piece][step] words of codes + 128
-  constexpr bool KEEP = NCH == 1;                         // the numbers stay in registers between the two looks
-  uint32_t b[NCH][KB][4];
+  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[step] words of codes + 128
+  uint32_t b[KB][4];
   {
     const int tok = min(g, p.T - 1);                      // tokens beyond the last one: its codes again, never stored
     const uint8_t* xr = (const uint8_t*)p.x + (size_t)(p.rows ? p.rows[tok] : tok) * p.ldx * (F32 ? 4 : 2);
-    float keep[KEEP ? KB : 1][16], mx = 0.f, ss = 0.f, bad = 0.f;
-    auto look = [&](int c, float (&v)[KB][16]) {
+    float v[KB][16], mx = 0.f, ss = 0.f, bad = 0.f;
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) load16<F32>(p, xr, (warp * NCH + c) * SCK + 64 * kb + 16 * t, v[kb], ss);
+    for (int kb = 0; kb < KB; ++kb) load16<F32>(p, xr, warp * SCK + 64 * kb + 16 * t, v[kb], ss);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { mx = fmaxf(mx, fabsf(v[kb][i])); bad = fmaf(v[kb][i], 0.f, bad); }
-    };
-    if constexpr (KEEP) look(0, keep);
-    else {
-#pragma unroll 1
-      for (int c = 0; c < NCH; ++c) { float v[KB][16]; look(c, v); }
-    }
+      for (int i = 0; i < 16; ++i) { mx = fmaxf(mx, fabsf(v[kb][i])); bad = fmaf(v[kb][i], 0.f, bad); }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -182,21 +174,16 @@ int8_stream_kernel(const StreamParams p) {
     const Rounding rd(codes ? s : 1.f);
     if (warp == 0 && t == 0) s_scale[g] = whole ? s : __int_as_float(0x7fc00000);
 #pragma unroll
-    for (int ci = 0; ci < NCH; ++ci)
+    for (int kb = 0; kb < KB; ++kb) {
+      if (p.g) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        float fresh[16], unused = 0.f;
-        if (!KEEP) load16<F32>(p, xr, (warp * NCH + ci) * SCK + 64 * kb + 16 * t, fresh, unused);
-        float (&v)[16] = KEEP ? keep[KEEP ? kb : 0] : fresh;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (p.g) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] *= rstd;
-        }
-        if (codes) codes8<16>(v, rd, w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[ci][kb][i] = w[i] ^ 0x80808080u;
+        for (int i = 0; i < 16; ++i) v[kb][i] *= rstd;
       }
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      if (codes) codes8<16>(v[kb], rd, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[kb][i] = w[i] ^ 0x80808080u;
+    }
   }
 
   int cslot = 0;
@@ -206,35 +193,28 @@ int8_stream_kernel(const StreamParams p) {
     for (int jb = 0; jb < nb; ++jb) {
 #pragma unroll
       for (int tile = 0; tile < TILES; ++tile) {
-        int acc[4] = {0, 0, 0, 0};
+        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+        __syncwarp();
+        const uint32_t src = ring + cslot * C::CHUNK + frag_off;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ci = 0; ci < NCH; ++ci) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
-          __syncwarp();
-          const uint32_t src = ring + cslot * C::CHUNK + frag_off;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
+          uint32_t lo[4], hi[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(at));
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * SCK));
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
-            uint32_t lo[4], hi[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(at));
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * SCK));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u;
-              const uint32_t a0 = halves(u, false), a1 = halves(v, false), a2 = halves(u, true), a3 = halves(v, true);
-              mma_f16(sum, a0, a1, a2, a3, halves(b[ci][kb][i], false), halves(b[ci][kb][i], true));
-            }
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u;
+            mma_f16(sum, halves(u, false), halves(v, false), halves(u, true), halves(v, true), halves(b[kb][i], false), halves(b[kb][i], true));
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] += __float2int_rn(sum[i]);
-          cslot = cslot + 1 == RING ? 0 : cslot + 1;
-          __syncwarp();                                   // every lane has read the slot that is refilled now
-          produce();
         }
+        cslot = cslot + 1 == RING ? 0 : cslot + 1;
+        __syncwarp();                                     // every lane has read the slot that is refilled now
+        produce();
         int* r = red + (size_t)((jb * TILES + tile) * WARPS + warp) * (16 * SNT);
-        *reinterpret_cast<int2*>(r + g * SNT + sum_col(g, 2 * t)) = make_int2(acc[0], acc[1]);
-        *reinterpret_cast<int2*>(r + (g + 8) * SNT + sum_col(g + 8, 2 * t)) = make_int2(acc[2], acc[3]);
+        *reinterpret_cast<int2*>(r + g * SNT + sum_col(g, 2 * t)) = make_int2(__float2int_rn(sum[0]), __float2int_rn(sum[1]));
+        *reinterpret_cast<int2*>(r + (g + 8) * SNT + sum_col(g + 8, 2 * t)) = make_int2(__float2int_rn(sum[2]), __float2int_rn(sum[3]));
       }
     }
     __syncthreads();
@@ -260,27 +240,26 @@ int8_stream_kernel(const StreamParams p) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool F32, int TILES, int KB, int NCH>
+template <bool F32, int TILES, int KB>
 int launch_stream(const StreamParams& p, int sm_count, cudaStream_t s) {
   typedef StreamCfg<KB> C;
   static bool configured[64] = {};
-  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, KB, NCH>, C::SMEM_BYTES, configured)) return -5;
-  return launch_ex(int8_stream_kernel<F32, TILES, KB, NCH>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(THREADS), C::SMEM_BYTES, s, 1, p);
+  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, KB>, C::SMEM_BYTES, configured)) return -5;
+  return launch_ex(int8_stream_kernel<F32, TILES, KB>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(THREADS), C::SMEM_BYTES, s, 1, p);
 }
 
-// What the kernel takes: fragments of all of K in registers, two pieces a warp; rows that 16-byte loads read, a norm in front of float ones
-// only. (Beyond 8,192 numbers a CTA has too much to quantise: 8 tokens, 14,336 to 4,096 29 us, on tcgen05 with ranges of K 22. With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
+// What the kernel takes: fragments of all of K in registers; rows that 16-byte loads read, a norm in front of float ones only. (Beyond 4,096
+// numbers a CTA has too much to quantise: 8 tokens, 8,192 to 2,048 12.9 us, on tcgen05 with ranges of K 11; 14,336 to 4,096 29 and 17. With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
 // tcgen05 behind a kernel that quantises 11.)
 bool streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g) {
-  if (T > SNT || xk % 8 || xk > WARPS * 2 * 256 || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
+  if (T > SNT || xk % 8 || xk > WARPS * 256 || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
   return x_dt == DT_F32 ? ldx % 4 == 0 : ldx % 8 == 0 && !g;
 }
 
 template <bool F32, int TILES>
 int launch_stream_k(const StreamParams& p, int sm_count, cudaStream_t s) {
-  if (p.K <= WARPS * 128) return launch_stream<F32, TILES, 2, 1>(p, sm_count, s);
-  if (p.K <= WARPS * 256) return launch_stream<F32, TILES, 4, 1>(p, sm_count, s);
-  return launch_stream<F32, TILES, 4, 2>(p, sm_count, s);
+  if (p.K <= WARPS * 128) return launch_stream<F32, TILES, 2>(p, sm_count, s);
+  return launch_stream<F32, TILES, 4>(p, sm_count, s);
 }
 
 }  // namespace

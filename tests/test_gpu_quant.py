@@ -143,6 +143,37 @@ def test_product(T, N, K, dtype):
     assert ((out.cpu().double() - total).abs() <= e * want.abs() + 2.0 ** -24 * total.abs() * 1.01).all()
 
 
+# tiles of two SMs: ends of tokens, outputs and K inside a tile, in either of the two, one tile a pair and several
+@pytest.mark.parametrize("T,N,K", [(1000, 4601, 4112), (700, 6000, 2500), (2049, 2000, 4100), (1400, 4096, 4112), (300, 9001, 4500),
+                                   (4097, 2200, 2060), (1030, 9000, 2000)])
+def test_products_of_many_tokens(T, N, K):
+    import ctypes
+    from rllm_b200.kernels import build
+    lib, bn, splits = build.load_library("quant"), ctypes.c_int(), ctypes.c_int()
+    x, w, px, pw = product_inputs(T, N, K, torch.bfloat16)
+    want, o = plain_product(px, pw), ops()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for epi in (o.EPI_STORE, o.EPI_STORE_F32, o.EPI_ACCUM_F32):
+        assert lib.rllm_int8_plan(epi, T, N, K, sms, ctypes.byref(bn), ctypes.byref(splits)) == 0 and bn.value == 512
+    e = 3 * 2.0 ** -24 * 1.01                       # (as in test_product)
+    for dt in DT.values():
+        y = quant().linear_int8(x, w, o.EPI_STORE, out_dtype=dt).cpu().double()
+        assert ((y - want).abs() <= (e + HALF[dt]) * want.abs()).all()
+    res = rnd(T, N, seed=5)
+    out = res.to(DEV)
+    quant().linear_int8(x, w, o.EPI_ACCUM_F32, out)
+    total = res.double() + want
+    assert ((out.cpu().double() - total).abs() <= e * want.abs() + 2.0 ** -24 * total.abs() * 1.01).all()
+    if N % 2 == 0:
+        assert lib.rllm_int8_plan(o.EPI_SWIGLU, T, N // 2, K, sms, ctypes.byref(bn), ctypes.byref(splits)) == 0 and bn.value == 512
+        g, u = want.chunk(2, dim=1)
+        want = g / (1 + torch.exp(-g)) * u
+        e = (3 * (1 + g.abs()) + 3 + 2 * 2 + 2 * 2 + 2) * 2.0 ** -24 * 2             # (as in test_product_swiglu)
+        for dt in DT.values():
+            y = quant().linear_int8(x, w, o.EPI_SWIGLU, out_dtype=dt).cpu().double()
+            assert ((y - want).abs() <= (e + HALF[dt]) * want.abs() + 1e-30).all()
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("T,N,K", SIZES)
 def test_product_swiglu(T, N, K, dtype):
