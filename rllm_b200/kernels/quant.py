@@ -47,7 +47,13 @@ class Int8Rows:
     [rows]."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, width: int):
-        self.codes, self.scales, self.width = codes, scales, int(width)
+        width = int(width)
+        if (codes.dtype != torch.int8 or codes.dim() != 2 or not codes.is_contiguous() or width < 1 or codes.shape[1] != (width + 15) // 16 * 16
+                or scales.dtype != torch.float32 or scales.shape != codes.shape[:1] or not scales.is_contiguous()
+                or scales.device != codes.device):
+            raise ops.KernelError(f"rows in 8 bits: codes must be contiguous int8 [rows, {width} rounded up to a multiple of 16], scales "
+                                  "contiguous float32 [rows] beside them")
+        self.codes, self.scales, self.width = codes, scales, width
 
     @property
     def shape(self):
@@ -300,7 +306,7 @@ def decode_supported(q: torch.Tensor, hd: int, scale: float) -> bool:
 def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
                          window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: about how many keys a sequence has
-    (for the number of ranges only); `splits`: that many ranges of keys (1 to 8, 16), None: by `decode_splits`."""
+    (for the number of ranges only); `splits`: that many ranges of keys (1 to 16), None: by `decode_splits`."""
     k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
     S = kv_lens.numel()
     _queries(q, nh, nkv, hd, S)
@@ -315,6 +321,10 @@ def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, 
         splits = decode_splits(S * nkv * -(-G // 16), seen, sms, hd)
     if out is None:
         out = q.new_empty((S, nh * hd))
+    else:
+        _here(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype or out.stride(1) != 1 or (S > 1 and out.stride(0) < nh * hd):
+            raise ops.KernelError(f"attention_kv4_decode: out must be bfloat16 [{S}, {nh * hd}] with unit inner stride and rows side by side")
     ops._check(ops._fn("quant", "rllm_kv4_decode")(
         q.data_ptr(), q.stride(0), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr(), out.stride(0),
         kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), S, nh, nkv, hd, page_size, float(scale), int(window or 0),
@@ -355,7 +365,8 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
         row = r0
         for s in range(s0, s1):
             n = ctx.q_lens_host[s]
-            if not _portions(q, tensors, ctx, block_table, nh, scale, window, (s, s + 1, row, row + n, False, n, ctx.kv_lens_host[s]), out, scratch):
+            keys = ctx.kv_lens_host[s] if ctx.kv_lens_host else most
+            if not _portions(q, tensors, ctx, block_table, nh, scale, window, (s, s + 1, row, row + n, False, n, keys), out, scratch):
                 return False
             row += n
         return True

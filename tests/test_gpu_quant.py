@@ -462,6 +462,112 @@ def test_a_nan_key_is_seen_where_it_is_visible_only():
     assert torch.isfinite(y).all()
 
 
+@pytest.mark.parametrize("window", [None, 333])
+@pytest.mark.parametrize("nh,nkv,hd,lens", [(8, 2, 64, [1, 700, 64, 2049]), (12, 1, 128, [1500, 3]), (40, 8, 64, [130]), (4, 4, 128, [900, 0])])
+def test_every_number_of_ranges(nh, nkv, hd, lens, window):
+    """The ranges that the keys are cut into do not show: any number of them, on any step, and a hint of the lengths that is wrong."""
+    t, table, _, held = make_cache(lens, nkv, hd, 16, seed=7)
+    S, scale = len(lens), hd ** -0.5
+    q = rnd(S, nh * hd, seed=3, dtype=torch.bfloat16, scale=1.5).to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    room = torch.full((S, nh * hd + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    for splits in (None, 1, 2, 3, 4, 5, 6, 7, 8, 16):
+        for hint in ((1, 100000) if splits is None else (max(lens),)):
+            room.fill_(7.0)
+            quant().attention_kv4_decode(q, t, lens_d, table, nh, scale, window, hint, splits, out=room[:, : nh * hd])
+            assert (room[:, nh * hd:] == 7.0).all()
+            for s, n in enumerate(lens):
+                got = room[s, : nh * hd].cpu().double().view(1, nh, hd)
+                if n == 0:
+                    assert not got.any()
+                    continue
+                want, mag, big = Q.attention(q[s].cpu().view(1, nh, hd), held[s][0], held[s][1], scale, window)
+                tol = bound(torch.bfloat16, want, mag, big, hd, n, False)
+                assert ((got - want).abs() <= tol).all(), (splits, hint, s, float(((got - want).abs() / tol).max()))
+    for splits in (0, -1, 17):
+        with pytest.raises(ops().KernelError):
+            quant().attention_kv4_decode(q, t, lens_d, table, nh, scale, window, max(lens), splits)
+
+
+def test_portions_one_by_one_and_without_scratch(monkeypatch):
+    """Portions whose numbers do not fit the scratch at once go one by one; where there is no room for one they are attended over in 4 bits."""
+    lens, q_lens, nh, nkv, hd = [700, 20, 640, 577], [100, 1, 200, 64], 8, 2, 64
+    t, table, _, _ = make_cache(lens, nkv, hd, 16)
+    q = rnd(sum(q_lens), nh * hd, seed=2, dtype=torch.bfloat16).to(DEV)
+    call = lambda: run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, 0.125, None)
+    y, (be, ctx, cache) = call()
+    monkeypatch.setattr(quant(), "READ_BYTES", 1)
+    assert torch.equal(call()[0], y)                       # (the same kernels over the same numbers)
+    ctx.per_forward.clear()
+    ctx.kv_lens_host = None
+    assert torch.equal(be.attention(q, cache, ctx, nh, 0.125, None), y)
+    simt = quant().attention_kv4(q, t, ctx, table, nh, 0.125, None, True, lambda size, make: None)
+    assert torch.equal(simt, quant().attention_kv4_simt(q, t, ctx.token_seq, ctx.positions, table, nh, 0.125))
+
+
+def test_calls_of_nothing():
+    q, o = quant(), ops()
+    none = torch.zeros(0, 128, device=DEV, dtype=torch.bfloat16)
+    w = q.quantize_matrix(rnd(40, 128, dtype=torch.bfloat16).to(DEV))
+    assert q.quantize_rows(none).shape == (0, 128) and q.linear(none, w).shape == (0, 40) and q.linear(none, w, o.EPI_SWIGLU).shape == (0, 20)
+    assert q.linear_int8(q.quantize_rows(none), w, o.EPI_STORE_F32).shape == (0, 40)
+    x = rnd(3, 128, dtype=torch.bfloat16).to(DEV)
+    assert q.linear(x, w, rows=torch.zeros(0, dtype=torch.int32, device=DEV)).shape == (0, 40)
+    t, table, _, _ = make_cache([20], 2, 64, 16)
+    i32 = torch.zeros(0, dtype=torch.int32, device=DEV)
+    before = {n: a.clone() for n, a in t.items()}
+    q.kv4_store(none, none, t, i32)
+    assert all(torch.equal(a.view(torch.uint8), before[n].view(torch.uint8)) for n, a in t.items())
+    assert q.attention_kv4_simt(none, t, i32, i32, table, 2, 1.0).shape == (0, 128)
+    assert q.attention_kv4_decode(none, t, i32, table, 2, 1.0, None, 1).shape == (0, 128)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T", [1, 8, 40, 700])
+def test_captured_and_replayed(T):
+    """A layer's calls, captured together on a stream of their own, replayed over new inputs: the same numbers as launch by launch. Two graphs
+    replayed at once on two streams do not disturb one another."""
+    q, o, nh, nkv, hd = quant(), ops(), 8, 2, 64
+    lens = [64 + 5 * (i % 40) for i in range(min(T, 40))]
+    t, table, slots, _ = make_cache(lens, nkv, hd, 16)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    last = torch.tensor([int(s[-1]) for s in slots], dtype=torch.int32, device=DEV)
+    w = [q.quantize_matrix(rnd(n, k, seed=n, dtype=torch.bfloat16).to(DEV)) for n, k in ((12 * 64, 512), (512, 512), (2 * 1024, 512), (512, 1024))]
+    S = len(lens)
+
+    def layer(x, cache):
+        qkv = q.linear(x, w[0])
+        q.kv4_store(qkv[:S, 512: 640], qkv[:S, 640:], cache, last)
+        a = q.attention_kv4_decode(qkv[:S, :512], cache, lens_d, table, nh, 0.125, None, 300)
+        h = q.linear(torch.cat([a, x[S:]]), w[1], o.EPI_STORE_F32)
+        f = q.linear(x, w[2], o.EPI_SWIGLU)
+        q.linear(f, w[3], o.EPI_ACCUM_F32, h)
+        return h
+
+    caches = [{n: a.clone() for n, a in t.items()} for _ in range(2)]
+    xs = [rnd(T, 512, seed=i, dtype=torch.bfloat16).to(DEV) for i in range(4)]
+    want = [layer(x, {n: a.clone() for n, a in t.items()}).clone() for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ins = [torch.zeros_like(xs[0]) for _ in range(2)]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            outs.append(layer(ins[i], caches[i]))
+        graphs.append(g)
+    for a, b in ((0, 1), (2, 3), (1, 0)):
+        for i, n in enumerate((a, b)):
+            ins[i].copy_(xs[n])
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[a]) and torch.equal(outs[1], want[b])
+
+
 def test_cache_calls_refuse():
     q, o = quant(), ops()
     t, table, slots, _ = make_cache([20], 2, 64, 16)
@@ -475,7 +581,12 @@ def test_cache_calls_refuse():
                  lambda: q.kv4_store(x.half(), x.half(), t, sl),
                  lambda: q.kv4_read(t, table, lens, 100), lambda: q.kv4_read(t, table.long(), lens, 20),
                  lambda: q.attention_kv4_simt(torch.zeros(1, 3 * 64, device=DEV), t, i32, i32, table, 3, 1.0),
-                 lambda: q.attention_kv4_simt(torch.zeros(1, 100, device=DEV), t, i32, i32, table, 2, 1.0)):
+                 lambda: q.attention_kv4_simt(torch.zeros(1, 100, device=DEV), t, i32, i32, table, 2, 1.0),
+                 lambda: q.attention_kv4_decode(x[:1], t, lens, table, 2, 0.0, None, 20),
+                 lambda: q.attention_kv4_decode(x[:1].float(), t, lens, table, 2, 1.0, None, 20),
+                 lambda: q.attention_kv4_decode(x[:1], t, lens, table, 2, 1.0, None, 20, out=x[:1].float()),
+                 lambda: q.attention_kv4_decode(x[:1], t, lens, table, 2, 1.0, None, 20, out=x[:2]),
+                 lambda: q.attention_kv4_decode(x[:1], t, lens, table, 2, 1.0, None, 20, out=x[:1].cpu())):
         with pytest.raises(o.KernelError):
             call()
 
@@ -563,6 +674,14 @@ def test_generate_and_graphs(dirs):
         llm.engine.check()
         llm.engine.cache.check()
     assert outs[0] == outs[1]
+
+
+def test_the_command_line_runs_it(dirs, capsys):
+    from rllm_b200 import cli
+    args = ["run", "--model", str(dirs["D"]), "--prompt-ids", "3,7,11,2", "--max-tokens", "5", "--temperature", "0"]
+    for more in ([], ["--kv-quant", "int4"], ["--weight-quant", "int8"], ["--kv-quant", "int4", "--weight-quant", "int8"]):
+        assert not cli.main(args + more)
+        assert capsys.readouterr().out.strip()
 
 
 def test_the_cache_takes_less(dirs):

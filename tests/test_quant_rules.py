@@ -79,6 +79,16 @@ def test_no_cpu_path():
             call()
 
 
+def test_rows_are_checked_when_made():
+    codes, scales = torch.zeros(4, 48, dtype=torch.int8), torch.zeros(4)
+    assert quant.Int8Rows(codes, scales, 40).shape == (4, 40) and quant.Int8Matrix(codes, scales, 48).dequantize().shape == (4, 48)
+    for c, s, width in ((codes, scales, 49), (codes, scales, 32), (codes, scales, 0), (codes.short(), scales, 48), (codes[0], scales, 48),
+                        (codes, scales[:3], 48), (codes, scales.double(), 48), (codes[:, :32], scales, 32), (codes, scales[:, None], 48),
+                        (codes, torch.zeros(8)[::2], 48)):
+        with pytest.raises(ops.KernelError, match="rows in 8 bits"):
+            quant.Int8Rows(c, s, width)
+
+
 def test_the_plain_forms_themselves():
     g = torch.Generator().manual_seed(3)
     x = torch.randn(5, 3, 128, generator=g)
