@@ -132,6 +132,7 @@ struct PfParams {
   float scale_log2e;
   // HALF_V: values are half numbers times 2^e, one e per page and kv head: [page * nkv + kv head]; a page is a multiple of a tile's keys
   const int* vexp;
+  int parts;             // HALF_V: CTAs of a cluster that share an item's keys; with more than one a CTA has one item
   int* err;
 };
 
@@ -288,7 +289,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     fence_barrier_init();
   }
   __syncthreads();
-  if (abort_flag) break;                                // a wait ran out in an earlier item: the kernel's output is void anyway
+  const bool shared = MODE == HALF_V && p.parts > 1;    // (its CTAs meet at the item's end, whatever happens before)
+  if (abort_flag && !shared) break;                     // a wait ran out in an earlier item: the kernel's output is void anyway
 
   const int q0 = p.cu_q[seq];
   const int q_len = p.cu_q[seq + 1] - q0;
@@ -311,6 +313,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const int p_max = kv_len - q_len + min(q_len - 1, (tile[g] * PM + PM - 1) / G);
       n_t[g] = active ? n_kept + (p_max + 1 - kv_begin + PN - 1) / PN : 0;
     }
+  }
+  if (shared) {
+    // this CTA's range of the tiles: as many steps as the others', a tile that both row tiles see being two
+    const int both = min(n_t[0], n_t[1]), steps = n_t[0] + n_t[1], z = (int)blockIdx.z;
+    auto cut = [&](int x) { return x <= 2 * both ? (x + 1) / 2 : x - both; };
+    const int from = cut(steps * z / p.parts), to = cut(steps * (z + 1) / p.parts);
+    kv_begin += from * PN;
+#pragma unroll
+    for (int g = 0; g < RT; ++g) n_t[g] = max(0, min(n_t[g], to) - from);
   }
   auto tile_first = [&](int t) { return t < n_kept ? t * PN : kv_begin + (t - n_kept) * PN; };   // first key of tile t of the list
   const int n_tiles = max(n_t[0], n_t[1]);
@@ -730,6 +741,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     if (ok && wait_on(&pv_full[g], (uint32_t)(n_mine - 1) & 1u, 25, n_mine)) {
       tc_fence_after();
+      if (shared) {                                        // the row's maximum and sum wait in the row tile's Q, which is done with
+        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(q_s + (uint32_t)(g * C::Q_BYTES + 4096 + r * 8)), "f"(m), "f"(l) : "memory");
+      } else {
       float inv = sig ? 1.f : (l > 0.f ? 1.f / l : 0.f);
       if (p.gate && valid) inv *= 1.f / (1.f + __expf(-p.gate[(size_t)(q0 + tok) * p.gate_ld + head]));
       const bf16* gh = nullptr;
@@ -777,10 +791,77 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
       }
       tc_fence_before();
+      }
     }
   } else if (TMA) {
     if (lane == 0) mbar_arrive(&q_full);                  // a row tile beyond the sequence's rows: nothing to bring
   }
+  }
+  if constexpr (MODE == HALF_V) {
+    if (shared) {
+      // The ranges' outputs meet: every CTA finishes a part of the item's rows, and is sent the others' sums of those (not divided), over its
+      // K and V stages, and their maxima and denominators, over Q. [CTA][four columns][row] x 16 bytes: a warp's rows lie side by side. (Left
+      // in each CTA's own shared memory and read from there, the exchange took 15 us of a launch.)
+      const int rows = RT * PM / p.parts;                  // 128 or 64: a warp's 32 rows go to one CTA
+      static_assert(RT * PM * VD * 4 <= KVS * (C::K_BYTES + C::V_BYTES) && RT * PM * 8 <= RT * C::Q_BYTES, "the parts lie over the stages");
+      __syncwarp();
+      cluster_sync_all();                                  // nobody multiplies or copies any more
+      if constexpr (SOFTMAX) {
+        const int x = (warp - SOFTMAX_WARP0) * 32 + lane;  // this thread's row of the item (warps 4.. have row tile 0's quadrants 0..3)
+        const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + C::O_COL + (uint32_t)(x / PM) * VD;
+        const int owner = x / rows, at = x % rows;
+        const bool there = n_t[x / PM] > 0;                // the range has keys of this row tile
+        const uint32_t to = map_to_rank(k_s + (uint32_t)(((int)blockIdx.z * (VD / 4) * rows + at) * 16), owner);
+#pragma unroll
+        for (int c = 0; c < VD / 32; ++c) {
+          uint32_t ov[32];
+          if (there) { tmem_ld32(from + 32 * c, ov); tmem_ld_wait(); }
+          else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            st_cluster_v4(to + (uint32_t)((8 * c + i) * rows * 16), __uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]),
+                          __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
+        }
+        const uint32_t ml = map_to_rank(q_s + (uint32_t)(((int)blockIdx.z * rows + at) * 8), owner);
+        const float* own = reinterpret_cast<const float*>(smem + (x / PM) * C::Q_BYTES + 4096 + x % PM * 8);
+        st_cluster_f32(ml, there ? own[0] : -INFINITY);
+        st_cluster_f32(ml + 4, there ? own[1] : 0.f);
+        tc_fence_before();
+      }
+      __syncwarp();
+      cluster_sync_all();                                  // every part has landed
+      if constexpr (SOFTMAX) {
+        const float* ml = reinterpret_cast<const float*>(smem);
+        const float4* parts = reinterpret_cast<const float4*>(smem + RT * C::Q_BYTES);
+        for (int i = threadIdx.x - SOFTMAX_WARP0 * 32; i < rows * (VD / 16); i += RT * PM) {
+          const int at = i % rows, col = i / rows * 4, x = (int)blockIdx.z * rows + at, row = tile[x / PM] * PM + x % PM;
+          if (row >= rows_total) continue;
+          float M = -INFINITY, L = 0.f, o[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+          for (int y = 0; y < p.parts; ++y) M = fmaxf(M, ml[2 * (y * rows + at)]);
+          for (int y = 0; y < p.parts; ++y) {
+            const float my = ml[2 * (y * rows + at)], f = my == -INFINITY ? 1.f : fast_exp2(my - M);      // (-inf: nothing seen, or NaN only)
+            L = fmaf(ml[2 * (y * rows + at) + 1], f, L);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float4 q = parts[(y * (VD / 4) + col + c) * rows + at];
+              o[4 * c] = fmaf(q.x, f, o[4 * c]); o[4 * c + 1] = fmaf(q.y, f, o[4 * c + 1]);
+              o[4 * c + 2] = fmaf(q.z, f, o[4 * c + 2]); o[4 * c + 3] = fmaf(q.w, f, o[4 * c + 3]);
+            }
+          }
+          const float inv = L > 0.f ? 1.f / L : 0.f;
+          uint4* dst = reinterpret_cast<uint4*>(p.out + (size_t)(q0 + row / G) * p.out_stride + (size_t)(kvh * G + row % G) * VD + 4 * col);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            dst[h] = make_uint4(pack_bf16(o[8 * h] * inv, o[8 * h + 1] * inv), pack_bf16(o[8 * h + 2] * inv, o[8 * h + 3] * inv),
+                                pack_bf16(o[8 * h + 4] * inv, o[8 * h + 5] * inv), pack_bf16(o[8 * h + 6] * inv, o[8 * h + 7] * inv));
+        }
+      }
+    }
   }
   }   // items
   };
@@ -850,11 +931,12 @@ int cache_map(CUtensorMap* out, const void* ptr, long long planes, int page_size
 }
 
 template <int KD, int VD, bool TMA, bool CAP, int MODE>
-int launch_pf_c(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mr, const PfParams& p, int ctas, cudaStream_t s) {
+int launch_pf_c(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mr, const PfParams& p, int ctas, cudaStream_t s) {      // ctas: clusters
   static bool configured[64] = {};
   constexpr int smem = Shape<KD, VD, CAP>::SMEM_BYTES;
   if (allow_dynamic_smem(attn_prefill_tc_kernel<KD, VD, TMA, CAP, MODE>, smem, configured)) return -5;
-  return launch_ex(attn_prefill_tc_kernel<KD, VD, TMA, CAP, MODE>, dim3(ctas), dim3(THREADS), smem, s, 1, mk, mv, mr, p);
+  const int z = MODE == HALF_V ? p.parts : 1;
+  return launch_ex(attn_prefill_tc_kernel<KD, VD, TMA, CAP, MODE>, dim3(ctas, 1, z), dim3(THREADS), smem, s, z, mk, mv, mr, p);
 }
 
 template <int HD, bool TMA>
@@ -900,14 +982,15 @@ int multiprocessors(int asked, int& sms) {
 // max_q_len: the longest portion in the batch (sizes the list of work items). Head sizes 64 and 128.
 // chunk > 0: a query sees only the keys of its own block of `chunk` positions (blocks counted from position 0);
 // sinks: float [nh] or null; gate: float logits [T, gate_ld] or null (see PfParams); keep_first, sigmoid: see PfParams.
-// softcap > 0: bounded scores. cross, long_from, vexp (values in half precision, pages of a power of two from 128 keys): see PfParams. sm_count: CTAs to launch at most (0: asked from the device).
+// softcap > 0: bounded scores. cross, long_from, vexp (values in half precision, pages of a power of two from 128 keys): see PfParams. parts: CTAs
+// that may share an item's keys (1, 2 or 4, with vexp; taken where every item's then have an SM each, else 1). sm_count: CTAs to launch at most (0: asked from the device).
 RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* kcache, const void* vcache,
                                        void* out, int out_stride, const int* cu_q, const int* kv_lens,
                                        const int* block_table, int bt_stride, int num_seqs, int max_q_len,
                                        int num_pages, int nh, int nkv, int hd, int page_size, float scale, int window,
                                        int chunk, const float* sinks, const float* gate, int gate_ld,
                                        int keep_first, int sigmoid, float softcap, int long_from, float* cross, const int* vexp,
-                                       int* err, int sm_count, void* stream) {
+                                       int parts, int* err, int sm_count, void* stream) {
   if (num_seqs <= 0 || max_q_len <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || keep_first < 0 || scale <= 0.f)
     return ERR_BAD_SIZE;
@@ -916,6 +999,7 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
   if (long_from > 0 && !cross) return ERR_BAD_SIZE;
   if (cross && (softcap > 0.f || sigmoid || gate || ((uintptr_t)cross & 15))) return ERR_BAD_SIZE;
   if (vexp && (cross || softcap > 0.f || sigmoid || sinks || page_size % 128)) return ERR_BAD_SIZE;
+  if (parts != 1 && ((parts != 2 && parts != 4) || !vexp || gate || keep_first)) return ERR_BAD_SIZE;
   PfParams p = {};
   p.long_from = long_from; p.cross = cross; p.vexp = vexp;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.kc = (const bf16*)kcache; p.vc = (const bf16*)vcache;
@@ -934,6 +1018,7 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
   if (int rc = multiprocessors(sm_count, sms)) return rc;
   p.fold = p.window <= 0 && p.chunk <= 0 && p.row_pairs > 1 && items <= sms;
   const int ctas = items < sms ? (int)items : sms;
+  p.parts = items * parts <= sms ? parts : 1;
   // pages of a power of two from 8 keys up (whole 1 KB swizzle atoms) come by tensor copies
   const bool tma = p.page_shift >= 3 && (long long)num_pages * nkv <= 2147483647LL;
   CUtensorMap mk, mv;

@@ -444,7 +444,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------- few tiles: ranges of K
-// Four MMAs on a block of K take 0.26 us whatever the tile's width (32 weight rows or 256), so a CTA's time goes with its blocks. Where the tiles
+// A CTA's time goes with its blocks of K, 0.22 us each with 64 weight rows and 0.45 with 256, however few its tokens. Where the tiles
 // leave most SMs idle and K is long, a tile is shared by the CTAs of a cluster, each with a range of K. The parts are whole numbers, so
 // their sum does not depend on the cut. Rank r finishes the r-th part of the tile's features: every rank pushes its accumulator's
 // columns to their owners through distributed shared memory, into the stage ring, which is idle once all ranks' products are

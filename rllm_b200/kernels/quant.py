@@ -350,6 +350,20 @@ def _runs(ctx) -> list:
     return runs
 
 
+def portion_parts(items: int, keys: int, hd: int, sm_count: int) -> int:
+    """CTAs that share a work item's keys (256 rows of a kv head, 1, 2 or 4 CTAs) where the items leave SMs idle: by the time in us, 0.0139 a
+    key at heads of 64 and 0.0185 at 128, and 4 + 1/16 a CTA for where the ranges meet, 4 more for many clusters of 4. One | two | four, us with the
+    keys' reading: 512 rows over 2,012 keys (32 / 8 heads of 128) 54.5 | 50.7; 512 over 600 25.4 | 28.5; 128 over 4,000 92 | 63 | 48; 64 over
+    4,000 (heads of 64) 67 | 43 | 32; 512 over 8,000 122 | 74."""
+    best, cost = 1, keys * (0.0139 if hd == 64 else 0.0185)
+    for z in (2, 4):
+        n = items * z
+        c = keys * (0.0139 if hd == 64 else 0.0185) / z + 4 + n / 16 + (4 if z == 4 and n > 64 else 0)
+        if n <= sm_count and c < cost:
+            best, cost = z, c
+    return best
+
+
 def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch) -> bool:
     """Attention of a run of portions (bfloat16, heads of 64 or 128): the keys and values that they see are read into scratch, in pages of
     READ_PAGE places, and the kernels of the cache of whole numbers attend over those. A portion's rows share the keys, so the
@@ -386,7 +400,9 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
         cu.data_ptr(), vexp.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
     a = (q, k, v, cu, kv_lens, table.view(S, width))
     if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(q, k):
-        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out, vexp=vexp)
+        items = -(-longest * (nh // nkv) // 256) * nkv * S
+        parts = portion_parts(items, min(most, window + longest) if window else most, hd, sm100.init(q.device).sm_count)
+        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out, vexp=vexp, parts=parts)
     else:
         sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out, vexp=vexp)
     return True

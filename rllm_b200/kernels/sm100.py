@@ -33,7 +33,7 @@ ops.register_signatures("sm100", {
     "rllm_attention_fa_v16": [_P, c_int, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                               c_int, c_int, c_float, c_int, c_int, _P, _P, _P],
     "rllm_attention_prefill_tc": [_P, c_int, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
-                                  c_int, c_int, c_float, c_int, c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, _P, _P, c_int, _P],
+                                  c_int, c_int, c_float, c_int, c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, _P, c_int, _P, c_int, _P],
     "rllm_attention_prefill_dense": [_P, c_int, c_int, _P, c_longlong, c_int, _P, _P, c_longlong, c_int, c_int, _P, c_int, c_longlong, _P,
                                      c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, c_int, c_int, c_int, _P, c_int, _P],
     "rllm_attention_decode_per_sm": [c_int, c_int, c_int],
@@ -435,7 +435,7 @@ def _extras(chunk, sinks, gate, nh, rows):
 
 def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_len, nh, scale, window, out=None,
                          chunk=None, sinks=None, gate=None, keep_first=0, sigmoid=False, softcap=None, long_from=0,
-                         cross=None, vexp=None):
+                         cross=None, vexp=None, parts=1):
     """Prefill attention on the tcgen05 tensor cores (bf16, head size 64 or 128): tiles of 128 rows x
     128 (64) keys, both products with their accumulators in TMEM. `chunk`: a query sees only the keys of its
     own block of that many positions; `sinks` float [nh]: exp(sink) joins a row's denominator; `gate` float
@@ -444,7 +444,8 @@ def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_le
     bounded, softcap * tanh(score / softcap). `cross` float32 [T, nh, nkv, hd]: every query head meets every kv head's
     values and the float outputs go there (pages of a power of two from 8 keys on; no gate, bound or sigmoid); sequences with
     fewer than `long_from` rows are then left out. `vexp` int32 [pages, kv heads]: the values are half numbers times 2^vexp (float16
-    vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid)."""
+    vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid); `parts`: that many CTAs (1, 2 or 4) may then share a
+    work item's keys, where all of them find an SM."""
     if not prefill_tc_supported(q, kcache):
         raise ops.KernelError("attention_prefill_tc: bfloat16, head size 64 or 128, rows 16-byte aligned")
     _check_vexp(vexp, kcache, vcache, 128)
@@ -461,7 +462,7 @@ def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_le
         cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.numel(),
         max_q_len, kcache.shape[0], nh, nkv, hd, page_size, float(scale), int(window or 0),
         *_extras(chunk, sinks, gate, nh, q.shape[0]), int(keep_first or 0), int(bool(sigmoid)), float(softcap or 0.0), int(long_from),
-        None if cross is None else cross.data_ptr(), None if vexp is None else vexp.data_ptr(), st.err.data_ptr(), st.sm_count, ops._stream())
+        None if cross is None else cross.data_ptr(), None if vexp is None else vexp.data_ptr(), int(parts), st.err.data_ptr(), st.sm_count, ops._stream())
     ops._check(rc, "attention_prefill_tc")
     return out if cross is None else cross
 

@@ -494,6 +494,7 @@ def test_portions_one_by_one_and_without_scratch(monkeypatch):
     lens, q_lens, nh, nkv, hd = [700, 20, 640, 577], [100, 1, 200, 64], 8, 2, 64
     t, table, _, _ = make_cache(lens, nkv, hd, 16)
     q = rnd(sum(q_lens), nh * hd, seed=2, dtype=torch.bfloat16).to(DEV)
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: 2)        # (how many ranges of keys there are goes with the run's items)
     call = lambda: run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, 0.125, None)
     y, (be, ctx, cache) = call()
     monkeypatch.setattr(quant(), "READ_BYTES", 1)
@@ -503,6 +504,27 @@ def test_portions_one_by_one_and_without_scratch(monkeypatch):
     assert torch.equal(be.attention(q, cache, ctx, nh, 0.125, None), y)
     simt = quant().attention_kv4(q, t, ctx, table, nh, 0.125, None, True, lambda size, make: None)
     assert torch.equal(simt, quant().attention_kv4_simt(q, t, ctx.token_seq, ctx.positions, table, nh, 0.125))
+
+
+@pytest.mark.parametrize("parts", [1, 2, 4])
+@pytest.mark.parametrize("lens,q_lens,nh,nkv,hd,window", [
+    ([700], [64], 8, 2, 64, None), ([520], [32], 8, 2, 128, None), ([1500, 513], [200, 130], 8, 2, 64, None), ([2000], [300], 4, 1, 128, 700),
+    ([600], [600], 8, 2, 64, None), ([900], [257], 8, 2, 128, None), ([1030, 520], [33, 520], 16, 2, 64, 100)])
+def test_portions_share_their_keys(lens, q_lens, nh, nkv, hd, window, parts, monkeypatch):
+    """Ranges of a work item's keys in CTAs of their own: every number of them, ranges that a row tile sees nothing of, rows in short of a tile."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: parts)
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1)
+    back = [max(0, (L - n - window + 1) // 16) if window else 0 for L, n in zip(lens, q_lens)]
+    t, table, _, held = make_cache(lens, nkv, hd, 16, seed=9, given_back=back)
+    q = rnd(sum(q_lens), nh * hd, seed=6, dtype=torch.bfloat16, scale=1.5).to(DEV)
+    scale, row = hd ** -0.5, 0
+    y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, scale, window)
+    for s, n in enumerate(q_lens):
+        want, mag, big = Q.attention(q[row: row + n].cpu().view(n, nh, hd), held[s][0], held[s][1], scale, window)
+        got = y[row: row + n].cpu().double().view(n, nh, hd)
+        row += n
+        tol = bound(torch.bfloat16, want, mag, big, hd, lens[s], True)
+        assert ((got - want).abs() <= tol).all(), (s, float(((got - want).abs() / tol).max()))
 
 
 def test_calls_of_nothing():

@@ -79,6 +79,15 @@ def test_no_cpu_path():
             call()
 
 
+def test_ranges_of_keys_find_an_sm_each():
+    for items in (1, 8, 16, 37, 38, 64, 74, 75, 148, 149, 5000):
+        for keys in (1, 300, 600, 1200, 4000, 60000):
+            for hd in (64, 128):
+                z = quant.portion_parts(items, keys, hd, 148)
+                assert z in (1, 2, 4) and (z == 1 or items * z <= 148) and (z == 1 or keys >= 256)
+    assert quant.portion_parts(8, 4000, 64, 148) == 4 and quant.portion_parts(64, 2012, 128, 148) == 2
+
+
 def test_rows_are_checked_when_made():
     codes, scales = torch.zeros(4, 48, dtype=torch.int8), torch.zeros(4)
     assert quant.Int8Rows(codes, scales, 40).shape == (4, 40) and quant.Int8Matrix(codes, scales, 48).dequantize().shape == (4, 48)
