@@ -749,6 +749,10 @@ RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long
                               const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int sm_count,
                               void* stream);
 
+RLLM_API int rllm_int8_streams_codes(int epi, int T, int N, int K, int sm_count);
+RLLM_API int rllm_int8_stream_codes(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
+                                    int T, int N, int K, int sm_count, void* stream);
+
 // y = x w^T from numbers x [*, xk] (as rllm_quantize_rows takes them): in one kernel for few tokens, else quantised into codes [T, K] and scales [T]
 // first. Without scratch (codes null) a product that wants it is not run: 1000000.
 RLLM_API int rllm_int8_linear(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
@@ -759,5 +763,7 @@ RLLM_API int rllm_int8_linear(int epi, int out_dt, int x_dt, const void* x, long
     return rllm_int8_stream(epi, out_dt, x_dt, x, ldx, rows, g, g_dt, eps, w, sw, y, ldy, T, N, xk, K, sm_count, stream);
   if (codes == nullptr) return 1000000;
   const int rc = rllm_quantize_rows(x_dt, x, ldx, rows, g, g_dt, eps, codes, K, scales, T, xk, 1, stream);
+  if (!rc && rllm_int8_streams_codes(epi, T, N, K, sm_count))
+    return rllm_int8_stream_codes(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, sm_count, stream);
   return rc ? rc : rllm_int8_gemm(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, err, sm_count, stream);
 }

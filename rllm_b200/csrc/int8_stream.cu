@@ -27,6 +27,7 @@ struct StreamParams {
   const void* x; long long ldx;
   const int* rows;                   // row of x that token t is made from, or null
   const void* g; int g_is_bf16; float eps;      // norm weight, or null
+  const float* sx;                   // CODES: x holds codes, these are their scales
   int xk;                            // numbers of a row of x (K without what pads it)
   const int8_t* w; const float* sw;
   void* y; long long ldy;
@@ -103,11 +104,15 @@ __device__ __forceinline__ void load16(const StreamParams& p, const void* xrow, 
   }
 }
 
-// TILES: 2 with SwiGLU
-template <bool F32, int TILES, int KB>
+// IN: bfloat16, float or codes; TILES: 2 with SwiGLU; NCH: pieces of K a warp has (codes only). A warp's sum is exact in float up to 1,024 products
+// of codes: 64 KB NCH at most.
+enum : int { NUMBERS = 0, FLOATS = 1, CODES = 2 };
+template <int IN, int TILES, int KB, int NCH>
 __global__ void __launch_bounds__(THREADS, 1)
 int8_stream_kernel(const StreamParams p) {
+  static_assert(NCH * KB <= 16 && (NCH == 1 || IN == CODES), "sums of a warp are exact; numbers are quantised in one piece");
   typedef StreamCfg<KB> C;
+  constexpr bool F32 = IN == FLOATS;
   constexpr int RING = C::RING, SCK = C::SCK, BATCH = SUMS / TILES;
   constexpr int UNITS = SCK / 16, STEP = 32 / UNITS;      // 16-byte units of a row, rows a copy instruction brings
   extern __shared__ __align__(128) uint8_t stream_smem[];
@@ -118,12 +123,12 @@ int8_stream_kernel(const StreamParams p) {
   const int my_jobs = p.njobs > (int)blockIdx.x ? (p.njobs - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
   pdl_launch();
 
-  int pj = 0, ptile = 0, pslot = 0;
+  int pj = 0, ptile = 0, pci = 0, pslot = 0;
   const int crow = lane / UNITS, cunit = lane % UNITS;
   auto produce = [&]() {
     if (pj < my_jobs) {
       const int n0 = (blockIdx.x + pj * gridDim.x) * 16;
-      const int k = warp * SCK + 16 * cunit;
+      const int k = (warp * NCH + pci) * SCK + 16 * cunit;
       const int8_t* src = p.w + (size_t)(n0 + (ptile ? p.N : 0) + crow) * p.K + k;
       const uint32_t dst = ring + pslot * C::CHUNK + crow * SCK + ((cunit ^ ((crow & 1) << 2)) << 4);      // odd rows: units' bit 2 flipped
 #pragma unroll
@@ -131,7 +136,7 @@ int8_stream_kernel(const StreamParams p) {
         const bool there = k < p.K && n0 + crow + STEP * i < p.N;
         copy16(dst + i * 512, there ? src + (size_t)(STEP * i) * p.K : p.w, there);
       }
-      if (++ptile == TILES) { ptile = 0; ++pj; }
+      if (++pci == NCH) { pci = 0; if (++ptile == TILES) { ptile = 0; ++pj; } }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     pslot = pslot + 1 == RING ? 0 : pslot + 1;
@@ -141,10 +146,20 @@ int8_stream_kernel(const StreamParams p) {
   for (int i = 0; i < RING; ++i) produce();
   pdl_wait();
 
-  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[step] words of codes + 128
-  uint32_t b[KB][4];
-  {
-    const int tok = min(g, p.T - 1);                      // tokens beyond the last one: its codes again, never stored
+  // ---- the tokens: their rows' largest numbers, then their codes as fragments: b[piece][step] words of codes + 128
+  uint32_t b[NCH][KB][4];
+  const int tok = min(g, p.T - 1);                        // tokens beyond the last one: its codes again, never stored
+  if constexpr (IN == CODES) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int k = (warp * NCH + c) * SCK + 64 * kb + 16 * t;
+        const uint4 q = k < p.K ? __ldcg(reinterpret_cast<const uint4*>((const int8_t*)p.x + (size_t)tok * p.ldx + k)) : make_uint4(0u, 0u, 0u, 0u);
+        b[c][kb][0] = q.x ^ 0x80808080u; b[c][kb][1] = q.y ^ 0x80808080u; b[c][kb][2] = q.z ^ 0x80808080u; b[c][kb][3] = q.w ^ 0x80808080u;
+      }
+    if (warp == 0 && t == 0) s_scale[g] = __ldcg(p.sx + tok);
+  } else {
     const uint8_t* xr = (const uint8_t*)p.x + (size_t)(p.rows ? p.rows[tok] : tok) * p.ldx * (F32 ? 4 : 2);
     float v[KB][16], mx = 0.f, ss = 0.f, bad = 0.f;
 #pragma unroll
@@ -183,7 +198,7 @@ int8_stream_kernel(const StreamParams p) {
       uint32_t w[4] = {0u, 0u, 0u, 0u};
       if (codes) codes8<16>(v[kb], rd, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[kb][i] = w[i] ^ 0x80808080u;
+      for (int i = 0; i < 4; ++i) b[0][kb][i] = w[i] ^ 0x80808080u;
     }
   }
 
@@ -194,25 +209,28 @@ int8_stream_kernel(const StreamParams p) {
     for (int jb = 0; jb < nb; ++jb) {
 #pragma unroll
       for (int tile = 0; tile < TILES; ++tile) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
-        __syncwarp();
-        const uint32_t src = ring + cslot * C::CHUNK + frag_off;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
-          uint32_t lo[4], hi[4];
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(at));
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * SCK));
+        for (int ci = 0; ci < NCH; ++ci) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+          __syncwarp();
+          const uint32_t src = ring + cslot * C::CHUNK + frag_off;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u;
-            mma_f16(sum, halves(u, false), halves(v, false), halves(u, true), halves(v, true), halves(b[kb][i], false), halves(b[kb][i], true));
+          for (int kb = 0; kb < KB; ++kb) {
+            const uint32_t at = src + ((((uint32_t)(4 * kb + t)) ^ frag_key) << 4);
+            uint32_t lo[4], hi[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]) : "r"(at));
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]) : "r"(at + 8 * SCK));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t u = lo[i] ^ 0x80808080u, v = hi[i] ^ 0x80808080u, c = b[ci][kb][i];
+              mma_f16(sum, halves(u, false), halves(v, false), halves(u, true), halves(v, true), halves(c, false), halves(c, true));
+            }
           }
+          cslot = cslot + 1 == RING ? 0 : cslot + 1;
+          __syncwarp();                                   // every lane has read the slot that is refilled now
+          produce();
         }
-        cslot = cslot + 1 == RING ? 0 : cslot + 1;
-        __syncwarp();                                     // every lane has read the slot that is refilled now
-        produce();
         int* r = red + (size_t)((jb * TILES + tile) * WARPS + warp) * (16 * SNT);
         *reinterpret_cast<int2*>(r + g * SNT + sum_col(g, 2 * t)) = make_int2(__float2int_rn(sum[0]), __float2int_rn(sum[1]));
         *reinterpret_cast<int2*>(r + (g + 8) * SNT + sum_col(g + 8, 2 * t)) = make_int2(__float2int_rn(sum[2]), __float2int_rn(sum[3]));
@@ -241,26 +259,26 @@ int8_stream_kernel(const StreamParams p) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <bool F32, int TILES, int KB>
+template <int IN, int TILES, int KB, int NCH>
 int launch_stream(const StreamParams& p, int sm_count, cudaStream_t s) {
   typedef StreamCfg<KB> C;
   static bool configured[64] = {};
-  if (allow_dynamic_smem(int8_stream_kernel<F32, TILES, KB>, C::SMEM_BYTES, configured)) return -5;
-  return launch_ex(int8_stream_kernel<F32, TILES, KB>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(THREADS), C::SMEM_BYTES, s, 1, p);
+  if (allow_dynamic_smem(int8_stream_kernel<IN, TILES, KB, NCH>, C::SMEM_BYTES, configured)) return -5;
+  return launch_ex(int8_stream_kernel<IN, TILES, KB, NCH>, dim3(p.njobs < sm_count ? p.njobs : sm_count), dim3(THREADS), C::SMEM_BYTES, s, 1, p);
 }
 
 // What the kernel takes: fragments of all of K in registers; rows that 16-byte loads read, a norm in front of float ones only. (Beyond 4,096
-// numbers a CTA has too much to quantise: 8 tokens, 8,192 to 2,048 12.9 us, on tcgen05 with ranges of K 11; 14,336 to 4,096 29 and 17. With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
+// numbers a CTA has too much to quantise: 8 tokens, 8,192 to 2,048 12.9 us, behind a kernel that makes the codes 8.2; 14,336 to 4,096 29 and 17.
+// With two groups of 8 tokens every CTA had twice as much to quantise: 16 tokens of 2,048 with a gate/up pair of 8,192 17.7 us, on
 // tcgen05 behind a kernel that quantises 11.)
 bool streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g) {
   if (T > SNT || xk % 8 || xk > WARPS * 256 || ((uintptr_t)x & 15) || ((uintptr_t)g & 15)) return false;
   return x_dt == DT_F32 ? ldx % 4 == 0 : ldx % 8 == 0 && !g;
 }
 
-template <bool F32, int TILES>
+template <int IN, int TILES>
 int launch_stream_k(const StreamParams& p, int sm_count, cudaStream_t s) {
-  if (p.K <= WARPS * 128) return launch_stream<F32, TILES, 2>(p, sm_count, s);
-  return launch_stream<F32, TILES, 4>(p, sm_count, s);
+  return p.K <= WARPS * 128 ? launch_stream<IN, TILES, 2, 1>(p, sm_count, s) : launch_stream<IN, TILES, 4, 1>(p, sm_count, s);
 }
 
 }  // namespace
@@ -279,8 +297,25 @@ RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long
     return ERR_BAD_SIZE;
   if ((uintptr_t)w & 15) return ERR_BAD_ALIGN;
   const bool out_f32 = out_dt == DT_F32 || epi == EPI_STORE_F32;
-  const StreamParams p = {x, ldx, rows, g, g_dt == DT_BF16, eps, xk, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi, out_f32};
+  const StreamParams p = {x, ldx, rows, g, g_dt == DT_BF16, eps, nullptr, xk, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi, out_f32};
   cudaStream_t s = (cudaStream_t)stream;
-  if (x_dt == DT_F32) return epi == EPI_SWIGLU ? launch_stream_k<true, 2>(p, sm_count, s) : launch_stream_k<true, 1>(p, sm_count, s);
-  return epi == EPI_SWIGLU ? launch_stream_k<false, 2>(p, sm_count, s) : launch_stream_k<false, 1>(p, sm_count, s);
+  if (x_dt == DT_F32) return epi == EPI_SWIGLU ? launch_stream_k<FLOATS, 2>(p, sm_count, s) : launch_stream_k<FLOATS, 1>(p, sm_count, s);
+  return epi == EPI_SWIGLU ? launch_stream_k<NUMBERS, 2>(p, sm_count, s) : launch_stream_k<NUMBERS, 1>(p, sm_count, s);
+}
+
+// The same from codes x [T, K] and scales sx [T], where every slab of 16 weight rows has an SM of its own: T up to 8, K up to 8,192, no SwiGLU.
+// Behind the kernel that makes the codes, on whose time the weights arrive: 8,192 to 2,048, 1 token 8.9 us on tcgen05 with ranges of K,
+// here 7.1 (8 tokens 9.2 and 8.2). With more slabs than SMs, or longer rows, tcgen05 is ahead: 14,336 to 4,096 16.3 and 22.5, 8,200 to 8,192 17.7 and 34.7.
+RLLM_API int rllm_int8_streams_codes(int epi, int T, int N, int K, int sm_count) {
+  return T <= SNT && K <= WARPS * 512 && epi != EPI_SWIGLU && (N + 15) / 16 <= sm_count;
+}
+RLLM_API int rllm_int8_stream_codes(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
+                                    int T, int N, int K, int sm_count, void* stream) {
+  if (T <= 0 || N <= 0) return 0;
+  if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
+  if (K <= 0 || K % 16 || ldy < N || epi < 0 || epi > 3 || !rllm_int8_streams_codes(epi, T, N, K, sm_count)) return ERR_BAD_SIZE;
+  if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
+  const StreamParams p = {x, K, nullptr, nullptr, 0, 0.f, sx, K, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi,
+                          out_dt == DT_F32 || epi == EPI_STORE_F32};
+  return launch_stream<CODES, 1, 4, 2>(p, sm_count, (cudaStream_t)stream);
 }
