@@ -61,8 +61,9 @@ def set_weight_quant(model, weight_quant: str) -> None:
     for p in model.parts():
         for name in p.int8_params:
             w = getattr(p, name)
-            with torch.cuda.device(w.device):
-                setattr(p, name, quant.quantize_matrix(w))
+            if not isinstance(w, quant.Int8Matrix):        # (a model may be given to a second engine)
+                with torch.cuda.device(w.device):
+                    setattr(p, name, quant.quantize_matrix(w))
             seen = True
     if not seen:
         raise ValueError(f"weight_quant {weight_quant!r}: no part of this model has matrices that can be held in 8 bits")

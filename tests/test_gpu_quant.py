@@ -706,6 +706,16 @@ def test_the_command_line_runs_it(dirs, capsys):
         assert capsys.readouterr().out.strip()
 
 
+def test_a_second_engine_of_the_same_model(dirs):
+    from rllm_b200.engine import Entry, load_engine
+    from rllm_b200.engine.factory import make_engine
+    a = load_engine(dirs["D"], device=DEV, num_pages=16, kv_quant="int4", weight_quant="int8")
+    b = make_engine(a.model, num_pages=16, dtype="bfloat16", device=DEV, kv_quant="int4", weight_quant="int8")
+    toks = tiny.random_prompt(40, P.read_model_dir(dirs["D"])[0]["vocab_size"], 3)
+    x, y = (e.step([Entry("a", toks, [39])]).clone() for e in (a, b))
+    assert torch.equal(x, y)
+
+
 def test_the_cache_takes_less(dirs):
     from rllm_b200.engine import load_engine
     a, b = (load_engine(dirs["D"], device=DEV, num_pages=8, kv_quant=k) for k in ("none", "int4"))
