@@ -14,7 +14,7 @@ from dataclasses import replace
 
 import torch
 
-from . import ops
+from . import ops, quant
 
 
 # Rows that a step's longest portion has where attention over latents runs over expanded keys and values, and rows from which
@@ -150,10 +150,7 @@ class Backend:
         # weights whose height is no multiple of 4 (a gate row per head, say) stay on the CUDA cores
         return self._sm100 is not None and w.shape[0] % 4 == 0 and self._sm100.gemm_supported(x, w)
 
-    @property
-    def _quant(self):
-        from . import quant
-        return quant
+    _quant = quant
 
     def quantize_weight(self, w):
         """A weight [N, K] in 8 bits with a scale per output channel; the products below take it in place of the tensor."""

@@ -37,7 +37,8 @@ HEAD_SIZES = (64, 128, 192, 256)
 
 def _here(t: torch.Tensor, name: str) -> None:
     """The launch goes to the current device's current stream: a tensor of another device would be read from there."""
-    if not t.is_cuda or t.get_device() != ops._raw_device():
+    d = t.get_device()                                     # -1: the CPU
+    if d < 0 or d != ops._raw_device():
         ops._cuda(t, name)
         raise ops.KernelError(f"{name} is on {t.device}, the current device is cuda:{ops._raw_device()}")
 
@@ -199,7 +200,7 @@ def _kv4(tensors: dict) -> tuple:
         raise ops.KernelError(f"a cache held in 4 bits has heads of {HEAD_SIZES}, not {hd}")
     here, scales = ops._raw_device(), (pages, nkv, page_size, hd // 32)
     for t, want, dt in ((k4, shape, torch.uint8), (v4, shape, torch.uint8), (ks, scales, torch.bfloat16), (vs, scales, torch.bfloat16)):
-        if t.dtype != dt or t.shape != want or not t.is_contiguous() or not t.is_cuda or t.get_device() != here:
+        if t.dtype != dt or t.shape != want or not t.is_contiguous() or t.get_device() != here:
             raise ops.KernelError(f"a cache held in 4 bits: codes must be contiguous uint8 {tuple(shape)} and scales bfloat16 {scales}, on the "
                                   f"current CUDA device (cuda:{here})")
     return k4, ks, v4, vs, pages, nkv, page_size, hd
@@ -307,29 +308,35 @@ def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, 
                          window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: about how many keys a sequence has
     (for the number of ranges only); `splits`: that many ranges of keys (1 to 16), None: by `decode_splits`."""
-    k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
-    S = kv_lens.numel()
+    kv = _kv4(tensors)
+    S, nkv, hd = kv_lens.numel(), kv[5], kv[7]
     _queries(q, nh, nkv, hd, S)
     if not decode_supported(q, hd, scale):
         raise ops.KernelError("attention_kv4_decode: bfloat16, heads of 64 or 128, rows of q on 16 bytes, a scale above 0")
     _i32(kv_lens, "kv_lens", S)
     _table(block_table, S)
-    G = nh // nkv
-    sms = sm100.init(q.device).sm_count
-    if splits is None:
-        seen = min(max_kv_len, window) if window else max_kv_len
-        splits = decode_splits(S * nkv * -(-G // 16), seen, sms, hd)
     if out is None:
         out = q.new_empty((S, nh * hd))
     else:
         _here(out, "out")
         if out.shape != q.shape or out.dtype != q.dtype or out.stride(1) != 1 or (S > 1 and out.stride(0) < nh * hd):
             raise ops.KernelError(f"attention_kv4_decode: out must be bfloat16 [{S}, {nh * hd}] with unit inner stride and rows side by side")
-    ops._check(ops._fn("quant", "rllm_kv4_decode")(
-        q.data_ptr(), q.stride(0), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr(), out.stride(0),
-        kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), S, nh, nkv, hd, page_size, float(scale), int(window or 0),
-        int(splits), sms, ops._stream()), "attention_kv4_decode")
+    _decode(q, kv, kv_lens, block_table, nh, scale, window, max_kv_len, splits, out, 0, 0, S)
     return out
+
+
+def _decode(q, kv, kv_lens, block_table, nh, scale, window, max_kv_len, splits, out, row, seq, S) -> None:
+    """The launch, for S sequences from `seq` on, whose rows of q and out begin at `row` (views of them would cost as much as the launch)."""
+    k4, ks, v4, vs, pages, nkv, page_size, hd = kv
+    sms = sm100.init(q.device).sm_count
+    if splits is None:
+        seen = min(max_kv_len, window) if window else max_kv_len
+        splits = decode_splits(S * nkv * -(-(nh // nkv) // 16), seen, sms, hd)
+    q_ld, out_ld, bt_ld = q.stride(0), out.stride(0), block_table.stride(0)
+    ops._check(ops._fn("quant", "rllm_kv4_decode")(
+        q.data_ptr() + 2 * row * q_ld, q_ld, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, out.data_ptr() + 2 * row * out_ld,
+        out_ld, kv_lens.data_ptr() + 4 * seq, block_table.data_ptr() + 4 * seq * bt_ld, bt_ld, S, nh, nkv, hd, page_size, float(scale),
+        int(window or 0), int(splits), sms, ops._stream()), "attention_kv4_decode")
 
 
 def _runs(ctx) -> list:
@@ -364,7 +371,7 @@ def portion_parts(items: int, keys: int, hd: int, sm_count: int) -> int:
     return best
 
 
-def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch) -> bool:
+def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> bool:
     """Attention of a run of portions (bfloat16, heads of 64 or 128): the keys and values that they see are read into scratch, in pages of
     READ_PAGE places, and the kernels of the cache of whole numbers attend over those. A portion's rows share the keys, so the
     numbers are made once instead of in every row tile. Keys are rounded to bfloat16, what the queries' product takes; values (12
@@ -372,7 +379,7 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
     0.0026 of its norm from the exact one, with half precision 0.0018, of which 0.0017 is the output's own rounding. False where the
     memory left does not hold the scratch."""
     s0, s1, r0, r1, _, longest, most = run
-    k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
+    k4, ks, v4, vs, pages, nkv, page_size, hd = kv
     S, width, T = s1 - s0, -(-most // READ_PAGE), r1 - r0
     size = S * width * nkv * READ_PAGE * hd * 2
     if S > 1 and 2 * size > READ_BYTES:            # one by one, then
@@ -380,7 +387,7 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
         for s in range(s0, s1):
             n = ctx.q_lens_host[s]
             keys = ctx.kv_lens_host[s] if ctx.kv_lens_host else most
-            if not _portions(q, tensors, ctx, block_table, nh, scale, window, (s, s + 1, row, row + n, False, n, keys), out, scratch):
+            if not _portions(q, kv, ctx, block_table, nh, scale, window, (s, s + 1, row, row + n, False, n, keys), out, scratch):
                 return False
             row += n
         return True
@@ -391,12 +398,12 @@ def _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch
     v = v.view(torch.float16)
     table, vexp, cu = q.new_empty(S * width * (1 + nkv) + S + 1, dtype=torch.int32).split((S * width, S * width * nkv, S + 1))
     whole = S == ctx.num_seqs                      # (a view costs the host as much as half a launch)
-    kv_lens, bt = (ctx.kv_lens, block_table) if whole else (ctx.kv_lens[s0:s1], block_table[s0:s1])
+    kv_lens = ctx.kv_lens if whole else ctx.kv_lens[s0:s1]
     if not whole:
         q, out = q[r0:r1], out[r0:r1]
     ops._check(ops._fn("quant", "rllm_kv4_read")(
-        ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, bt.data_ptr(), bt.stride(0), kv_lens.data_ptr(),
-        ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+        ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr() + 4 * s0 * block_table.stride(0),
+        block_table.stride(0), kv_lens.data_ptr(), ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), table.data_ptr(),
         cu.data_ptr(), vexp.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
     a = (q, k, v, cu, kv_lens, table.view(S, width))
     if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(q, k):
@@ -420,12 +427,15 @@ def attention_kv4(q: torch.Tensor, tensors: dict, ctx, block_table: torch.Tensor
         # a captured step's bound serves contexts from half of it up
         keys = ctx.max_kv_len * 3 // 4 if ctx.graph_safe else ctx.max_kv_len
         return attention_kv4_decode(q, tensors, ctx.kv_lens, block_table, nh, scale, window, max(keys, 1))
-    _queries(q, nh, tensors["k4"].shape[1], hd, ctx.num_tokens)
+    kv = _kv4(tensors)
+    _queries(q, nh, kv[5], hd, ctx.num_tokens)
+    _i32(ctx.kv_lens, "kv_lens", ctx.num_seqs)
+    _table(block_table, ctx.num_seqs)
     out = q.new_empty((q.shape[0], nh * hd))
     for run in _runs(ctx):
         s0, s1, r0, r1, single, _, most = run
         if single:
-            attention_kv4_decode(q[r0:r1], tensors, ctx.kv_lens[s0:s1], block_table[s0:s1], nh, scale, window, most, out=out[r0:r1])
-        elif not _portions(q, tensors, ctx, block_table, nh, scale, window, run, out, scratch):
+            _decode(q, kv, ctx.kv_lens, block_table, nh, scale, window, most, None, out, r0, s0, s1 - s0)
+        elif not _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch):
             return simt()
     return out
