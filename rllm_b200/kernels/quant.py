@@ -307,12 +307,14 @@ def decode_supported(q: torch.Tensor, hd: int, scale: float) -> bool:
 def attention_kv4_decode(q: torch.Tensor, tensors: dict, kv_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
                          window: int | None, max_kv_len: int, splits: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over 4 bits for one bfloat16 query row per sequence, heads of 64 or 128. `max_kv_len`: about how many keys a sequence has
-    (for the number of ranges only); `splits`: that many ranges of keys (1 to 16), None: by `decode_splits`."""
+    (for the number of ranges only); `splits`: that many ranges of keys (1 to 8, 16), None: by `decode_splits`."""
     kv = _kv4(tensors)
     S, nkv, hd = kv_lens.numel(), kv[5], kv[7]
     _queries(q, nh, nkv, hd, S)
     if not decode_supported(q, hd, scale):
         raise ops.KernelError("attention_kv4_decode: bfloat16, heads of 64 or 128, rows of q on 16 bytes, a scale above 0")
+    if splits is not None and splits not in (1, 2, 3, 4, 5, 6, 7, 8, 16):
+        raise ops.KernelError(f"attention_kv4_decode: 1 to 8 or 16 ranges of keys, not {splits}")
     _i32(kv_lens, "kv_lens", S)
     _table(block_table, S)
     if out is None:

@@ -484,7 +484,7 @@ def test_every_number_of_ranges(nh, nkv, hd, lens, window):
                 want, mag, big = Q.attention(q[s].cpu().view(1, nh, hd), held[s][0], held[s][1], scale, window)
                 tol = bound(torch.bfloat16, want, mag, big, hd, n, False)
                 assert ((got - want).abs() <= tol).all(), (splits, hint, s, float(((got - want).abs() / tol).max()))
-    for splits in (0, -1, 17):
+    for splits in (0, -1, 9, 15, 17):
         with pytest.raises(ops().KernelError):
             quant().attention_kv4_decode(q, t, lens_d, table, nh, scale, window, max(lens), splits)
 
