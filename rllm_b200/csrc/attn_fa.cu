@@ -18,7 +18,7 @@
 // reference's prefill kernel attends inside the chunk only (attention.cu:573-618); here a
 // portion also sees what earlier steps left in the cache.
 // Cache layout: [page][kv head][offset in page][HD].
-#include "common.cuh"
+#include "quant.cuh"
 #include <cuda_fp16.h>
 using namespace rllm;
 
@@ -78,12 +78,12 @@ struct FaParams {
   float* part_ml;     // [(token * nh + head) * splits + z][2]
   long long part_rows;   // rows the two buffers above have: a row index beyond it (a cu_q that names more
                          // tokens than the caller said) is skipped, never written
-  // V16: values are half numbers times 2^e, with one e per page and kv head; a page is a multiple of BN keys
+  // V16: values are half numbers, or bfloat16, times 2^e, a word per page and kv head (quant.cuh); a page is a multiple of BN keys
   const int* vexp;       // [page * nkv + kv head]
 };
 
 // V16: a value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
-// that meet the half values are those of the sum itself and stay within half's range; the denominator's part is given it back.
+// that meet the values, in the values' type, are those of the sum itself and stay within half's range; the denominator's part is given it back.
 template <int HD, int NWARPS, bool V16>
 __global__ void __launch_bounds__(NWARPS * 32)
 fa_paged_kernel(const FaParams p) {
@@ -210,7 +210,8 @@ fa_paged_kernel(const FaParams p) {
 
     if (w_active && j0 <= wpos_max && j0 + BN - 1 >= wlo_min) {
       const int page_v = V16 ? bt[pshift >= 0 ? (j0 >> pshift) : j0 / p.page_size] : -1;
-      const int ve = V16 && page_v >= 0 ? p.vexp[page_v * p.nkv + kvh] : 0;
+      const int word = V16 && page_v >= 0 ? p.vexp[page_v * p.nkv + kvh] : 0, ve = value_exponent(word);
+      const bool halves = V16 && !value_wide(word);
       const float vef = (float)ve, vback = V16 ? __int_as_float((127 - ve) << 23) : 1.f;
       // ---- scores S = Q K^T : 16 rows x 64 keys; the K fragments of a k-step are fetched together
       float s[BN / 8][4];
@@ -276,18 +277,21 @@ fa_paged_kernel(const FaParams p) {
           if (V16) {
             lA = fmaf(p0 + p1 + p4 + p5, vback, lA);
             lB = fmaf(p2 + p3 + p6 + p7, vback, lB);
-            a[0] = pack_f16(p0, p1); a[1] = pack_f16(p2, p3);
-            a[2] = pack_f16(p4, p5); a[3] = pack_f16(p6, p7);
           } else {
             lA += p0 + p1 + p4 + p5;
             lB += p2 + p3 + p6 + p7;
+          }
+          if (halves) {
+            a[0] = pack_f16(p0, p1); a[1] = pack_f16(p2, p3);
+            a[2] = pack_f16(p4, p5); a[3] = pack_f16(p6, p7);
+          } else {
             a[0] = pack_bf16(p0, p1); a[1] = pack_bf16(p2, p3);
             a[2] = pack_bf16(p4, p5); a[3] = pack_bf16(p6, p7);
           }
         }
 #pragma unroll
         for (int dp = 0; dp < DTILES / 2; ++dp) {
-          if (V16) {
+          if (halves) {
             mma_f16(o[2 * dp], a, vb[dp][0], vb[dp][1]);
             mma_f16(o[2 * dp + 1], a, vb[dp][2], vb[dp][3]);
           } else {
@@ -420,7 +424,7 @@ RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, 
                 nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, nullptr, stream);
 }
 
-// The same with values in half precision times 2^vexp[page * nkv + kv head]; pages of a multiple of 64 keys.
+// The same with values of 16 bits times a power of two, vexp[page * nkv + kv head] (quant.cuh: value_word); pages of a multiple of 64 keys.
 RLLM_API int rllm_attention_fa_v16(const void* q, int q_stride, const void* kcache, const void* vcache, const int* vexp, void* out,
                                    int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
                                    int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,

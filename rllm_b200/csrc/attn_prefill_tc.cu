@@ -54,7 +54,7 @@
 // reference's prefill kernel a portion also sees what earlier steps left in the cache.
 // Every mbarrier wait is bounded; a wait that runs out records an error word and the CTA leaves
 // in an orderly way (TMEM freed).
-#include "common.cuh"
+#include "quant.cuh"
 #include "sm100.cuh"
 #include <cuda_fp16.h>
 #include <mutex>
@@ -134,7 +134,7 @@ struct PfParams {
   const bf16* q2; long long q2_stride; int q2_head;
   const bf16* gate_h; int gate_h_ld, gate_cols;   // logits [T, gate_h_ld] or null: a column per head, or (gate_cols) per output
   float scale_log2e;
-  // HALF_V: values are half numbers times 2^e, one e per page and kv head: [page * nkv + kv head]; a page is a multiple of a tile's keys
+  // HALF_V: values are 16-bit numbers times 2^e, a word per page and kv head (quant.cuh): [page * nkv + kv head]; a page is a multiple of a tile's keys
   const int* vexp;
   int parts;             // HALF_V: CTAs of a cluster that share an item's keys; with more than one a CTA has one item
   int* err;
@@ -215,8 +215,8 @@ __device__ __forceinline__ void softcap_poly2(uint32_t& x0, uint32_t& x1, float 
 // CAP: scores are bounded (p.cap).
 // MODE PLAIN: pages. CROSS: pages, every head over every kv head's values, float outputs (PfParams). DENSE: keys and values in
 // rows, by tensor copies of whole tiles.
-// HALF_V: pages whose values are half numbers times a power of two a page (PfParams); the weights that meet them are half numbers
-// too. A value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
+// HALF_V: pages whose values are half numbers, or bfloat16 where half's range is too small, times a power of two a page (PfParams); the weights
+// that meet them are of the same type. A value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
 // are those of the sum itself and stay within half's range; the denominator's part is given it back.
 enum : int { PLAIN = 0, CROSS = 1, DENSE_ROWS = 2, HALF_V = 3 };
 template <int KD, int VD, bool TMA, bool CAP, int MODE>
@@ -232,6 +232,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __shared__ __align__(8) uint64_t kv_full[KVS], kv_empty[KVS], s_full[SB], s_free[SB], p_full[RT], pv_full[RT], q_full;
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
+  __shared__ int tile_wide[RT];        // HALF_V: is P of the row tile's step bfloat16? Written in front of `p_full`, when the PV before is complete
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* smem = (uint8_t*)(((uintptr_t)pf_smem_raw + 1023) & ~(uintptr_t)1023);
@@ -351,8 +352,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   if constexpr (!SOFTMAX) {
   // ---- the products. Step k is (row tile g, K tile t); its S lands in accumulator acc_of(k, g), used for the turn_of(k, t)-th time.
   constexpr uint32_t id_s = idesc(PM, PN, false);
-  // 64 output values at a time; HALF_V: both operands' type field says half
-  constexpr uint32_t id_pv = idesc(PM, 64, true) & (MODE == HALF_V ? ~((7u << 7) | (7u << 10)) : ~0u);
+  // 64 output values at a time; HALF_V: both operands' type field says half, or bfloat16 where the page is
+  constexpr uint32_t id_bf16 = idesc(PM, 64, true), id_half = id_bf16 & ~((7u << 7) | (7u << 10));
   auto step = [&](int k, int& g, int& t) {
     if (k < 2 * n_both) { g = k & 1; t = k >> 1; } else { g = g_long; t = n_both + (k - 2 * n_both); }
   };
@@ -391,6 +392,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       abort_flag = 1; record_failure(p.err, 23, t); ok = false; return;
     }
     tc_fence_after();
+    const uint32_t id_pv = MODE == HALF_V && !*(volatile int*)&tile_wide[g] ? id_half : id_bf16;
     const uint64_t dv = dv0 + (uint64_t)((t % NST) * (C::V_BYTES >> 4));
     const uint32_t acc = tmem_base + C::O_COL + (uint32_t)g * VD, pa = tmem_base + (BESIDE ? C::P_COL + (uint32_t)g * (PN / 2) : C::S_COL + (uint32_t)(k % SB) * PN);
 #pragma unroll
@@ -597,11 +599,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const int j0 = tile_first(t);
       const int k = t < n_both ? 2 * t + g : 2 * n_both + (t - n_both);
       const int sa = BESIDE ? g : k % SB;
-      int ve = 0;                                          // the tile's values' power of two
+      int word = 0;                                        // the tile's values' power of two and type
       if (MODE == HALF_V) {
         const int page = p.block_table[(size_t)seq * p.bt_stride + (j0 >> p.page_shift)];
-        if (page >= 0) ve = p.vexp[page * p.nkv + kvh];
+        if (page >= 0) word = p.vexp[page * p.nkv + kvh];
       }
+      const int ve = value_exponent(word);
       const uint32_t s_addr = lane_addr + C::S_COL + (uint32_t)sa * PN;          // this step's S accumulator
       const uint32_t p_addr = BESIDE ? lane_addr + C::P_COL + (uint32_t)g * (PN / 2) : s_addr;
       if (!wait_on(&s_full[sa], (uint32_t)(BESIDE ? t : k / SB) & 1u, 24, t)) { ok = false; break; }
@@ -709,34 +712,41 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       uint64_t lq[4];                                     // eight partial sums side by side, added up in a fixed order
 #pragma unroll
       for (int i = 0; i < 4; ++i) lq[i] = f32x2(0.f, 0.f);
+      auto weigh = [&](auto type) {                       // float(): bfloat16, __half(): half numbers
+        constexpr bool HALVES = std::is_same<decltype(type), __half>::value;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        uint32_t pk[16];
-        if (sig) {
-          // sigmoid(x) = 1 / (1 + 2^(-x log2 e)); hidden keys hold -inf: 1 / (1 + inf) = 0
+        for (int c = 0; c < NC; ++c) {
+          uint32_t pk[16];
+          if (MODE != HALF_V && sig) {
+            // sigmoid(x) = 1 / (1 + 2^(-x log2 e)); hidden keys hold -inf: 1 / (1 + inf) = 0
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e0 = fast_rcp(1.f + fast_exp2(-fmaf(__uint_as_float(v[c][2 * i]), sl, sb)));
-            const float e1 = fast_rcp(1.f + fast_exp2(-fmaf(__uint_as_float(v[c][2 * i + 1]), sl, sb)));
-            pk[i] = pack_bf16(e0, e1);
+            for (int i = 0; i < 16; ++i) {
+              const float e0 = fast_rcp(1.f + fast_exp2(-fmaf(__uint_as_float(v[c][2 * i]), sl, sb)));
+              const float e1 = fast_rcp(1.f + fast_exp2(-fmaf(__uint_as_float(v[c][2 * i + 1]), sl, sb)));
+              pk[i] = pack_bf16(e0, e1);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float e0, e1;
+              split2(fma2(f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, use2), e0, e1);
+              e0 = fast_exp2(e0); e1 = fast_exp2(e1);       // hidden keys hold -inf: 0
+              lq[i & 3] = add2(lq[i & 3], f32x2(e0, e1));
+              pk[i] = HALVES ? pack_f16(e0, e1) : pack_bf16(e0, e1);
+            }
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float e0, e1;
-            split2(fma2(f32x2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sl2, use2), e0, e1);
-            e0 = fast_exp2(e0); e1 = fast_exp2(e1);         // hidden keys hold -inf: 0
-            lq[i & 3] = add2(lq[i & 3], f32x2(e0, e1));
-            pk[i] = MODE == HALF_V ? pack_f16(e0, e1) : pack_bf16(e0, e1);
-          }
+          tmem_st16(p_addr + 16 * c, pk);
         }
-        tmem_st16(p_addr + 16 * c, pk);
-      }
+      };
+      if (MODE == HALF_V && !value_wide(word)) weigh(__half()); else weigh(float());       // (a branch in every piece: a prompt of 2,048 43.8 -> 49.9 us)
       tmem_st_wait();
       if (!BESIDE && !moves && !pv_before()) { ok = false; break; }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g]);
+      if (lane == 0) {
+        if (MODE == HALF_V) *(volatile int*)&tile_wide[g] = value_wide(word);
+        mbar_arrive(&p_full[g]);
+      }
       float ls[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(lq[i], ls[2 * i], ls[2 * i + 1]);
@@ -986,7 +996,7 @@ int multiprocessors(int asked, int& sms) {
 // max_q_len: the longest portion in the batch (sizes the list of work items). Head sizes 64 and 128.
 // chunk > 0: a query sees only the keys of its own block of `chunk` positions (blocks counted from position 0);
 // sinks: float [nh] or null; gate: float logits [T, gate_ld] or null (see PfParams); keep_first, sigmoid: see PfParams.
-// softcap > 0: bounded scores. cross, long_from, vexp (values in half precision, pages of a power of two from 128 keys): see PfParams. parts: CTAs
+// softcap > 0: bounded scores. cross, long_from, vexp (values of 16 bits times powers of two, pages of a power of two from 128 keys): see PfParams. parts: CTAs
 // that may share an item's keys (1, 2 or 4, with vexp; taken where every item's then have an SM each, else 1). sm_count: CTAs to launch at most (0: asked from the device).
 RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* kcache, const void* vcache,
                                        void* out, int out_stride, const int* cu_q, const int* kv_lens,

@@ -98,12 +98,33 @@ __device__ __forceinline__ void store4h(void* p, const float (&v)[4]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {       // of both halves
+  asm("max.u16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
+}
+__device__ __forceinline__ uint32_t block_max2(uint32_t v) {
+  __shared__ uint32_t red[THREADS / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max2(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 32; ++w) v = max2(v, red[w]);
+  return v;
+}
+
 // Places i * out_page .. of sequence s go to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind
 // the sequence's last token are zeros, and so are those in pages it does not hold. A CTA takes one kv head's part of a page. With `cu_q` (attention
 // of portions) pages that no query of the step sees are left out; table_out says which are there, cu_out counts the portions' rows
 // from zero.
-// vexp: the values are half numbers times 2^vexp[page * nkv + kv head], with the largest of the page's scales between 1 and 2 of these
-// powers. (A value has 12 significant bits: half numbers hold 11 of them, bfloat16 8.)
+// vexp: the values are 16-bit numbers times a power of two a page and kv head (`value_word`). A value has 12 significant bits: half numbers hold 11
+// of them, bfloat16 8, but half numbers have few powers of two. So a page whose scales lie within 2^6 of each other is half numbers, its
+// largest scale between 1 and 2; any other is bfloat16, its smallest scale (but not less than 2^-40 of its largest) between 1 and 2. The power
+// joins the scores where the weights are made: with the smallest scale no group of such a page, be it one a row's weight lies
+// wholly on, raises a row's maximum by more than it adds to the sum, so that the other pages' weights, in half precision, keep their bits.
+// A page of zeros adds nothing and so has the lowest power.
 // UNITS: pieces (place, block of 64 dimensions) that a thread has at once, eight lanes together: 8 are a page of 128 places of 128 dimensions.
 // (With place after place, each behind its page's number, 2,012 keys of 8 heads of 128 took 11.5 us to read, now 7.6.)
 template <typename T, int UNITS>
@@ -159,14 +180,23 @@ kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restr
       two[e] = there[e] ? __ldcg(reinterpret_cast<const uint32_t*>(sc + row * (c.hd >> 5)) + b) : 0u;
     }
     float down = 1.f;
+    bool wide = false;
     if (half) {                                          // (the page is one turn of the loop)
-      __shared__ float red[32];
-      float mx = 0.f;
+      // the largest scale's bits, and 0x7fff less the smallest's, as two maxima in a word
+      uint32_t ends = 0u;
 #pragma unroll
-      for (int e = 0; e < UNITS; ++e) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(two[e])), fabsf(bf16_hi(two[e]))));      // (fmaxf drops a NaN)
-      mx = block_max(mx, red);
-      const int e = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -100), 120) : 0;
-      if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = e;
+      for (int e = 0; e < UNITS; ++e)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t b = (g ? two[e] >> 16 : two[e]) & 0x7fffu;
+          if (there[e] && b < 0x7f80u) ends = max2(ends, b | (0x7fffu - b) << 16);        // (a NaN is one in any format)
+        }
+      ends = block_max2(ends);
+      const int top = (int)(ends >> 7 & 0xffu) - 127, low = (int)((0x7fffu - (ends >> 16)) >> 7 & 0xffu) - 127;
+      const bool zeros = (ends & 0xffffu) == 0u;
+      wide = !zeros && (low < top - 6 || top < -VALUE_EXPONENTS || top > VALUE_EXPONENTS);
+      const int e = min(max(zeros ? -VALUE_EXPONENTS : wide ? max(low, top - 40) : top, -VALUE_EXPONENTS), VALUE_EXPONENTS);
+      if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = value_word(e, wide);
       down = __int_as_float((127 - e) << 23);
     }
 #pragma unroll
@@ -181,7 +211,7 @@ kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restr
         for (int i4 = 0; i4 < 4; ++i4) { x0[i4] = (float)code4(word[e], i4) * d0; x1[i4] = (float)code4(word[e], 4 + i4) * d1; }
       }
       T* o = dst + (size_t)r * c.hd + 64 * b + 4 * w;
-      if (half) { store4h(o, x0); store4h(o + 32, x1); }
+      if (half && !wide) { store4h(o, x0); store4h(o + 32, x1); }
       else { store4(o, x0); store4(o + 32, x1); }
     }
   }
@@ -221,7 +251,7 @@ RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk,
 
 // The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, out_page, hd] float or bf16 (rounded once). kv_lens int32
 // [num_seqs], none above width * out_page; block_table int32 with an entry for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
-// [num_seqs + 1], and vexp [num_seqs * width, nkv] (bf16 only: v is then half numbers; out_page * hd / 64 between 32 and 256) for attention of portions, or null.
+// [num_seqs + 1], and vexp [num_seqs * width, nkv] (bf16 only: v is then 16-bit numbers as `value_word` says; out_page * hd / 64 between 32 and 256) for attention of portions, or null.
 RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
                            const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, int out_page, void* k,
                            void* v, int* table_out, int* cu_out, int* vexp, int nkv, int page_size, int hd, void* stream) {

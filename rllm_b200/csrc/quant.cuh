@@ -72,4 +72,11 @@ __device__ __forceinline__ int code4(uint32_t word, int i) { return (int)((word 
 __device__ __forceinline__ float bf16_lo(uint32_t two) { return __uint_as_float(two << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
 
+// How a page of values is held in the scratch of portions (kv4_read_kernel writes it, the portions' kernels read it): 16-bit numbers times
+// 2^e, half numbers or, `wide`, bfloat16. One word a page and kv head.
+__host__ __device__ __forceinline__ int value_word(int e, bool wide) { return 2 * e + (wide ? 1 : 0); }
+__host__ __device__ __forceinline__ int value_exponent(int word) { return word >> 1; }
+__host__ __device__ __forceinline__ bool value_wide(int word) { return word & 1; }
+constexpr int VALUE_EXPONENTS = 48;           // e lies between -48 and 48
+
 }  // namespace rllm

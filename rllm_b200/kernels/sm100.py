@@ -379,7 +379,7 @@ def attention_splits(num_seqs: int, nkv: int, max_rows: int, max_kv_len: int, sm
 def attention_fa(q, kcache, vcache, cu_q, kv_lens, block_table, num_tokens, max_q_len, max_kv_len, nh,
                  scale, window, splits=None, out=None, vexp=None):
     """Tiled tensor-core attention over the paged cache (bf16, head size 64 or 128). `vexp` int32 [pages, kv heads]: the values
-    are half numbers times 2^vexp (float16 vcache, pages of a multiple of 64 keys)."""
+    are half numbers times 2^(vexp >> 1), or with vexp odd bfloat16 ones (float16 vcache, pages of a multiple of 64 keys)."""
     st = init(q.device)
     _, nkv, page_size, hd = kcache.shape
     _check_vexp(vexp, kcache, vcache, 64)
@@ -443,8 +443,8 @@ def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_le
     the window says; `sigmoid`: no softmax, a visible key's weight is sigmoid(score + sinks[head]); `softcap`: scores
     bounded, softcap * tanh(score / softcap). `cross` float32 [T, nh, nkv, hd]: every query head meets every kv head's
     values and the float outputs go there (pages of a power of two from 8 keys on; no gate, bound or sigmoid); sequences with
-    fewer than `long_from` rows are then left out. `vexp` int32 [pages, kv heads]: the values are half numbers times 2^vexp (float16
-    vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid); `parts`: that many CTAs (1, 2 or 4) may then share a
+    fewer than `long_from` rows are then left out. `vexp` int32 [pages, kv heads]: the values are half numbers times
+    2^(vexp >> 1), or with vexp odd bfloat16 ones (float16 vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid); `parts`: that many CTAs (1, 2 or 4) may then share a
     work item's keys, where all of them find an SM."""
     if not prefill_tc_supported(q, kcache):
         raise ops.KernelError("attention_prefill_tc: bfloat16, head size 64 or 128, rows 16-byte aligned")

@@ -1,0 +1,125 @@
+"""Attention over a cache held in 4 bits whose values are of very different sizes: places, groups of 32 dimensions, pages, and rows whose weight lies
+wholly on small ones. Against the plain 64-bit form, number by number: `bound` is a share of sum_j p_j |v_j| of each dimension, so that a
+dimension of small values is held to its own size."""
+import math
+
+import pytest
+import torch
+
+import plain_quant as Q
+from test_gpu_quant import DEV, bound, quant, rnd, run_attention
+
+pytestmark = pytest.mark.gpu
+
+SIZES = ("like", "places", "groups", "pages", "both", "zero_pages", "zero_places", "zero_groups", "small", "large")
+
+
+def powers(kind, n, nkv, hd, gen):
+    """What the values of a sequence are multiplied by, [n, nkv, hd / 32]: powers of two and zeros."""
+    one = torch.ones(n, nkv, hd // 32, dtype=torch.float64)
+    draw = lambda *shape: 2.0 ** torch.randint(-14, 15, shape, generator=gen).double()
+    if kind == "places":
+        return one * draw(n, 1, 1)
+    if kind == "groups":
+        return one * draw(1, nkv, hd // 32)
+    if kind == "pages":
+        return one * draw(-(-n // 128), 1, 1).repeat_interleave(128, 0)[:n]
+    if kind == "both":
+        return one * draw(n, 1, 1) * draw(1, nkv, hd // 32)
+    if kind == "zero_pages":                                   # and the others small
+        return one * 2.0 ** -30 * (torch.arange(n) // 128 % 2).double()[:, None, None]
+    if kind == "zero_places":
+        return one * (torch.arange(n) % 3 > 0).double()[:, None, None]
+    if kind == "zero_groups":
+        return one * (torch.randint(0, 3, one.shape, generator=gen) > 0).double()
+    return one * {"like": 1.0, "small": 2.0 ** -60, "large": 2.0 ** 60}[kind]
+
+
+def make(kind, lens, nkv, hd, page=16, seed=0, sink=None):
+    """As `make_cache` of the tests beside, values times `powers`. `sink`: every key at these places is the query's own direction."""
+    gen = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    t = {n: torch.full((sum(need), nkv, page, hd // 2), 0x5a, dtype=torch.uint8) for n in ("k4", "v4")}
+    t.update({n: torch.full((sum(need), nkv, page, hd // 32), math.nan, dtype=torch.bfloat16) for n in ("ks", "vs")})
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    order = torch.randperm(sum(need), generator=gen).tolist()
+    held = []
+    for s, n in enumerate(lens):
+        mine = [order.pop() for _ in range(need[s])]
+        table[s, : need[s]] = torch.tensor(mine, dtype=torch.int32)
+        at = torch.tensor([mine[j // page] for j in range(n)]), torch.arange(n) % page
+        kv = []
+        for name in "kv":
+            x = torch.randn(n, nkv, hd, generator=gen, dtype=torch.float64)
+            if name == "v":
+                x = (x.unflatten(-1, (-1, 32)) * powers(kind, n, nkv, hd, gen)[..., None]).flatten(-2)
+            elif sink is not None:
+                x[[j for j in sink if j < n]] = 3.0
+            c, d = Q.groups4(x)
+            t[name + "4"][at[0], :, at[1]] = Q.pack4(c)
+            t[name + "s"][at[0], :, at[1]] = d.bfloat16()
+            kv.append((c.unflatten(-1, (-1, 32)) * d[..., None]).flatten(-2))
+        held.append(kv)
+    return {n: x.to(DEV) for n, x in t.items()}, table.to(DEV), held
+
+
+def check(y, q, held, lens, q_lens, nh, hd, scale, window, read_bf16):
+    row = 0
+    for s, n in enumerate(q_lens):
+        want, mag, big = Q.attention(q[row: row + n].cpu().view(n, nh, hd), held[s][0], held[s][1], scale, window)
+        got = y[row: row + n].cpu().double().view(n, nh, hd)
+        row += n
+        tol = bound(torch.bfloat16, want, mag, big, hd, lens[s], read_bf16)
+        far = ((got - want).abs() - tol).max()
+        assert torch.isfinite(got).all() and far <= 0, (s, float(far), float(((got - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("parts", [0, 1, 2, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", SIZES)
+def test_portions(kind, hd, parts, monkeypatch):
+    """`parts` 0: the kernel of short portions; else that many CTAs share an item's keys. Bound: weights and values rounded to bfloat16, half a
+    step each, as `bound` has it for portions; a page in half precision is well within."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: max(parts, 1))
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if parts else 1 << 30)
+    lens, q_lens, nh, nkv = [700, 300], [64, 40], 8, 2
+    t, table, held = make(kind, lens, nkv, hd, seed=hd + parts)
+    q = rnd(sum(q_lens), nh * hd, seed=6, dtype=torch.bfloat16, scale=1.5).to(DEV)
+    for window in (None, 200):
+        y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, hd ** -0.5, window)
+        check(y, q, held, lens, q_lens, nh, hd, hd ** -0.5, window, True)
+
+
+@pytest.mark.parametrize("parts", [0, 2])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["places", "zero_places", "zero_pages", "both"])
+def test_portions_whose_weight_lies_on_few_keys(kind, hd, parts, monkeypatch):
+    """Queries that a few keys draw nearly all of the weight from: small ones beside large ones, zeros among them."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: max(parts, 1))
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if parts else 1 << 30)
+    lens, q_lens, nh, nkv = [700], [64], 4, 1
+    t, table, held = make(kind, lens, nkv, hd, seed=3 * hd + parts, sink=(0, 1, 2, 130, 131, 132, 400))
+    q = (0.5 + 0.1 * rnd(64, nh * hd, seed=6)).bfloat16().to(DEV)
+    y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, 16 / hd, None)
+    check(y, q, held, lens, q_lens, nh, hd, 16 / hd, None, True)
+
+
+@pytest.mark.parametrize("parts", [0, 1])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_portions_of_like_values_keep_half_precision(hd, parts, monkeypatch):
+    """Values of one size are half numbers, and so are the weights: with 2^-11 of half a step where bfloat16 has 2^-8. Queries and keys are codes times
+    powers of two, so that reading keys as bfloat16 is exact, and few keys share the weight, so that roundings do not average out."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: 1)
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if parts else 1 << 30)
+    L, n, nh, nkv = 600, 128, 4, 1
+    t, table, held = make("like", [L], nkv, hd, seed=hd, sink=())
+    t["ks"].copy_(torch.where(torch.isnan(t["ks"]), t["ks"], torch.full_like(t["ks"], 0.25)))
+    held[0][0] = Q.groups4(held[0][0])[0] * 0.25           # the codes' keys; twelve bits of a value stay
+    q = rnd(n, nh * hd, seed=2, scale=1.0).bfloat16().to(DEV)
+    y, _ = run_attention(q, t, table, [L], [n], nh, nkv, hd, 16, 4 * hd ** -0.5, None)
+    want, mag, big = Q.attention(q.cpu().view(n, nh, hd), held[0][0], held[0][1], 4 * hd ** -0.5, None)
+    got = y.cpu().double().view(n, nh, hd)
+    # the output's own rounding, half a step of weight and value in half precision (2^-11 each), scores as `bound` has them
+    e = torch.expm1(2 * (big * (hd + 6) * 2.0 ** -23 + 1e-5))[..., None] + (L + 16) * 2.0 ** -23 + 2 * 2.0 ** -11
+    tol = mag * e * 1.02 + 2.0 ** -8 * want.abs() * 1.02
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
