@@ -17,9 +17,9 @@
 //   * O^T = V^T P^T, dimensions within a group on the rows; the contraction is over (key, group) pairs, so that a register is again a word's
 //     nibble of both halves, and a column's weights are zero for the group that is not its own: columns 0-3 become the
 //     output's first 32 dimensions of a block, columns 4-7 the second. The scale of a (key, group) goes onto the weight in float, before its
-//     one rounding, to half precision (bfloat16 cost 0.0016 of the output's norm); so that the product stays in half's range, the running
-//     maximum is that of score + log2 of the key's largest value scale, weights themselves being float of any size. movmatrix
-//     turns the rounded weights from rows of keys into the columns that the second product takes.
+//     one rounding, to half precision (bfloat16 cost 0.0016 of the output's norm). So that the product stays in half's range whatever the
+//     sizes of a group's scales, each group of 32 dimensions has a running maximum of score + log2 of its scale beside the scores' own, and
+//     its sums are against that one. movmatrix turns the rounded weights from rows of keys into the columns that the second product takes.
 //   * Which key a row of the fragment stands for is free, as long as both products agree, and is chosen so that neither product's reads of
 //     shared memory meet a bank twice.
 //   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which is as good as 1, and
@@ -352,12 +352,18 @@ kv4_decode_kernel(const Kv4Params p) {
 
   float o[NQ][2 * BL][4];                                // [block, half of a group]: rows dimensions, columns queries (see below)
   float m[NQ][2], l[NQ][2];
+  float top[NQ][2][BL];                                  // what the sums of this lane's columns' group in each block are against (log2)
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
 #pragma unroll
     for (int i = 0; i < 2 * BL; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
-    m[x][0] = m[x][1] = -INFINITY;
-    l[x][0] = l[x][1] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[x][e] = -INFINITY;
+      l[x][e] = 0.f;
+#pragma unroll
+      for (int b = 0; b < BL; ++b) top[x][e][b] = -INFINITY;
+    }
   }
   // a scale of this lane's columns' group out of the two, as float; where the weights of the keys 2 qi and 2 qi + 1 go
   const uint32_t pick = qi & 2 ? 0x3244u : 0x1044u, put0 = hi_cols ? 0x1044u : 0x4410u, put1 = hi_cols ? 0x3244u : 0x4432u;
@@ -428,36 +434,53 @@ kv4_decode_kernel(const Kv4Params p) {
         }
       }
       // ---- weights
-      uint32_t sc[2][2][BL];                             // the value scales of rows quad and quad + 8
-      float big[2][2];                                   // log2 of the largest of a row
+      float sc[2][2][BL], big[2][2][BL];                 // the value scales of rows quad and quad + 8 in this lane's group, their log2
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = 0.f;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int b = 0; b < BL; ++b) {
-            sc[f][e][b] = lds32(sa + st + C::SCALES + (32 * half + 16 * f + 8 * e) * (HD / 16) + 4 * b);
-            x = fmaxf(x, fmaxf(fabsf(bf16_lo(sc[f][e][b])), fabsf(bf16_hi(sc[f][e][b]))));      // (drops a NaN)
+            sc[f][e][b] = scale_of(lds32(sa + st + C::SCALES + (32 * half + 16 * f + 8 * e) * (HD / 16) + 4 * b));
+            big[f][e][b] = exponent_of(fabsf(sc[f][e][b]));
           }
-          big[f][e] = exponent_of(x);
-        }
+      auto risen = [](float now, float old) { return now == old ? 1.f : fast_exp2(old - now); };
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        float mx0 = fmaxf(fmaxf(s[0][x][0] + big[0][0], s[0][x][2] + big[0][1]), fmaxf(s[1][x][0] + big[1][0], s[1][x][2] + big[1][1]));
-        float mx1 = fmaxf(fmaxf(s[0][x][1] + big[0][0], s[0][x][3] + big[0][1]), fmaxf(s[1][x][1] + big[1][0], s[1][x][3] + big[1][1]));
-        if (__any_sync(0xffffffffu, mx0 > m[x][0] + 8.f || mx1 > m[x][1] + 8.f)) {
+        float mx[2], tx[2][BL];
+        bool rises = false;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = fmaxf(fmaxf(s[0][x][e], s[0][x][2 + e]), fmaxf(s[1][x][e], s[1][x][2 + e]));
+          rises = rises || mx[e] > m[x][e] + 8.f;
+#pragma unroll
+          for (int b = 0; b < BL; ++b) {
+            tx[e][b] = fmaxf(fmaxf(s[0][x][e] + big[0][0][b], s[0][x][2 + e] + big[0][1][b]),
+                             fmaxf(s[1][x][e] + big[1][0][b], s[1][x][2 + e] + big[1][1][b]));
+            rises = rises || tx[e][b] > top[x][e][b] + 8.f;
           }
-          mx0 = fmaxf(mx0, m[x][0]); mx1 = fmaxf(mx1, m[x][1]);
-          const float c0 = m[x][0] == mx0 ? 1.f : fast_exp2(m[x][0] - mx0), c1 = m[x][1] == mx1 ? 1.f : fast_exp2(m[x][1] - mx1);
-          m[x][0] = mx0; m[x][1] = mx1;
-          l[x][0] *= c0; l[x][1] *= c1;
+        }
+        if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
-          for (int t = 0; t < 2 * BL; ++t) { o[x][t][0] *= c0; o[x][t][1] *= c1; o[x][t][2] *= c0; o[x][t][3] *= c1; }
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+#pragma unroll
+              for (int b = 0; b < BL; ++b) tx[e][b] = fmaxf(tx[e][b], __shfl_xor_sync(0xffffffffu, tx[e][b], d));
+            }
+            mx[e] = fmaxf(mx[e], m[x][e]);
+            l[x][e] *= risen(mx[e], m[x][e]);
+            m[x][e] = mx[e];
+#pragma unroll
+            for (int b = 0; b < BL; ++b) {
+              tx[e][b] = fmaxf(tx[e][b], top[x][e][b]);
+              const float c = risen(tx[e][b], top[x][e][b]);
+              top[x][e][b] = tx[e][b];
+#pragma unroll
+              for (int u = 0; u < 2; ++u) { o[x][2 * b + u][e] *= c; o[x][2 * b + u][2 + e] *= c; }
+            }
+          }
         }
         const float u0 = m[x][0] == -INFINITY ? 0.f : m[x][0], u1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
 #pragma unroll
@@ -468,6 +491,14 @@ kv4_decode_kernel(const Kv4Params p) {
           l[x][1] += s[f][x][1] + s[f][x][3];
         }
       }
+      // from the scores' maximum to the group's (a maximum of -inf: no key yet, or NaN scores only)
+      float up[NQ][2][BL];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int b = 0; b < BL; ++b) up[x][e][b] = m[x][e] == -INFINITY ? 1.f : fast_exp2(m[x][e] - top[x][e][b]);
       // ---- values: the keys of weights 2 qi, 2 qi + 1, 2 qi + 8 and 2 qi + 9 are qi, qi + 4, qi + 8 and qi + 12
 #pragma unroll
       for (int f = 0; f < 2; ++f)
@@ -476,13 +507,14 @@ kv4_decode_kernel(const Kv4Params p) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {                  // rows 0-7, then 8-15
             const int k0 = 32 * half + 16 * f + 8 * e;
-            const float d = scale_of(sc[f][e][b]);
+            const float d = sc[f][e][b];
             uint32_t ca[4], cb[4];
             codes_f16(lds32(va[b] + st + k0 * ROW), ca);
             codes_f16(lds32(vb[b] + st + k0 * ROW), cb);
 #pragma unroll
             for (int x = 0; x < NQ; ++x) {
-              const uint32_t w = turn8x8(pack2(s[f][x][2 * e] * d, s[f][x][2 * e + 1] * d));
+              // (the weight times its power first: below 2^8 over the scale, so that nothing overflows on the way)
+              const uint32_t w = turn8x8(pack2(s[f][x][2 * e] * up[x][0][b] * d, s[f][x][2 * e + 1] * up[x][1][b] * d));
               const uint32_t b0 = __byte_perm(w, 0u, put0), b1 = __byte_perm(w, 0u, put1);
               // rows quad and quad + 8 are dimensions 4 quad + 2 u and 4 quad + 2 u + 1 of the columns' group
 #pragma unroll
@@ -518,9 +550,12 @@ kv4_decode_kernel(const Kv4Params p) {
       if (lane < 2) { w_m[warp * 16 + query] = m[x][e]; w_l[warp * 16 + query] = l[x][e]; }
       if (query < nq) {
 #pragma unroll
-        for (int t = 0; t < 2 * BL; ++t)
+        for (int t = 0; t < 2 * BL; ++t) {
+          // the groups' sums against the scores' maximum, in two steps that stay in range where the sums are zero
+          const float c = m[x][e] == -INFINITY ? 1.f : fast_exp2(0.5f * (top[x][e][t >> 1] - m[x][e]));
           *reinterpret_cast<float2*>(w_o + ((size_t)warp * 4 * NQ + query) * HD + 64 * (t >> 1) + 32 * (qi >> 1) + 4 * quad + 2 * (t & 1)) =
-              make_float2(o[x][t][e], o[x][t][2 + e]);
+              make_float2(o[x][t][e] * c * c, o[x][t][2 + e] * c * c);
+        }
       }
     }
   }

@@ -123,3 +123,29 @@ def test_portions_of_like_values_keep_half_precision(hd, parts, monkeypatch):
     e = torch.expm1(2 * (big * (hd + 6) * 2.0 ** -23 + 1e-5))[..., None] + (L + 16) * 2.0 ** -23 + 2 * 2.0 ** -11
     tol = mag * e * 1.02 + 2.0 ** -8 * want.abs() * 1.02
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (12, 2, 64), (8, 1, 128), (12, 1, 128)])
+@pytest.mark.parametrize("kind", SIZES)
+def test_single_tokens(kind, nh, nkv, hd):
+    """Keys are codes and so exact; the bound has half a step of bfloat16 for a weight, where half precision has 2^-11."""
+    lens = [700, 33, 1]
+    t, table, held = make(kind, lens, nkv, hd, seed=hd + nh)
+    q = rnd(3, nh * hd, seed=6, dtype=torch.bfloat16, scale=1.5).to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for window in (None, 200):
+        for splits in (1, 4, 16):
+            y = quant().attention_kv4_decode(q, t, lens_d, table, nh, hd ** -0.5, window, 700, splits)
+            check(y, q, held, lens, [1, 1, 1], nh, hd, hd ** -0.5, window, False)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["places", "zero_places", "zero_pages", "both"])
+def test_single_tokens_whose_weight_lies_on_few_keys(kind, hd):
+    lens, nh, nkv = [700], 4, 1
+    t, table, held = make(kind, lens, nkv, hd, seed=3 * hd, sink=(0, 1, 2, 130, 131, 132, 400))
+    q = (0.5 + 0.1 * rnd(1, nh * hd, seed=6)).bfloat16().to(DEV)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for splits in (1, 3, 8):
+        y = quant().attention_kv4_decode(q, t, lens_d, table, nh, 16 / hd, None, 700, splits)
+        check(y, q, held, lens, [1], nh, hd, 16 / hd, None, False)
