@@ -21,6 +21,7 @@ struct Int8Params {
   int T, N, K;                       // N: outputs (of one half with SwiGLU); K: bytes a row, a multiple of 16
   int box;                           // token rows a copy brings
   int splits;                        // ranges of K
+  int w_fixed;                       // nothing in front of this kernel writes the weight
   int* err;
 };
 
@@ -109,19 +110,19 @@ __device__ __forceinline__ void emit_turned(const Int8Params& p, int t_warp, int
     }
 }
 
-// Scales of the W weight rows from n on (what lies behind the last one is not used)
+// Scales of the W weight rows from n on (what lies behind the last one is not used). Plain loads: the kernel in front may have written them.
 template <int W>
 __device__ __forceinline__ void scales(const Int8Params& p, int n, float (&s)[W]) {
   const int end = n < p.N ? p.N : 2 * p.N;               // (with SwiGLU up rows follow the gate rows)
   if (p.vec) {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(p.sw + min(n + i, end - 4)));
+      const float4 q = *reinterpret_cast<const float4*>(p.sw + min(n + i, end - 4));
       s[i] = q.x; s[i + 1] = q.y; s[i + 2] = q.z; s[i + 3] = q.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) s[i] = __ldg(p.sw + min(n + i, end - 1));
+    for (int i = 0; i < W; ++i) s[i] = p.sw[min(n + i, end - 1)];
   }
 }
 
@@ -218,7 +219,8 @@ int8_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       const uint64_t pol_x = policy_evict_last();    // the token tiles are read by every weight tile
       const uint32_t bytes = (uint32_t)(C::B_BYTES + p.box * BK);
       const uint32_t st0 = smem_u32(smem);
-      // the first stages' weights need not wait for the kernel in front: what writes a weight's codes lets no kernel start before it ends
+      // the first stages' weights need not wait for the kernel in front, unless it, or one before it, may still write them
+      if (!p.w_fixed) pdl_wait();
       const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * n_kb;
       const int pre = min(mine, C::STAGES);
       auto weights = [&](int s, int tile, int kb) {
@@ -373,7 +375,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       auto tokens = [&](int s, int tile, int kb) {
         tma_load_2d_pair(st0 + s * C::STAGE_BYTES, &tmap_x, even0 + 8 * s, kb * BK, tile % t_tiles * 2 * BM + rank * BM);
       };
-      for (int i = 0; i < pre; ++i) {                    // (see the kernel above: weights need not wait)
+      if (!p.w_fixed) pdl_wait();                        // (see the kernel above)
+      for (int i = 0; i < pre; ++i) {
         if (leader) mbar_expect_tx(&full_bar[i], stage_bytes);
         weights(i, pair_id + i / n_kb * n_pairs, i % n_kb);
       }
@@ -495,6 +498,7 @@ int8_split_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         tma_load_2d(dst, &tmap_w, full, kb * BK, n0);
         if (DUAL) tma_load_2d(dst + F * BK, &tmap_w, full, kb * BK, p.N + n0);
       };
+      if (!p.w_fixed) pdl_wait();
       for (int i = 0; i < pre; ++i) { mbar_expect_tx(&full_bar[i], bytes); weights(i, kb0 + i); }
       pdl_wait();
       for (int i = 0; i < pre; ++i) tma_load_2d(st0 + i * C::STAGE_BYTES, &tmap_x, smem_u32(&full_bar[i]), (kb0 + i) * BK, t0);
@@ -725,15 +729,16 @@ RLLM_API int rllm_int8_plan(int epi, int T, int N, int K, int sm_count, int* bn,
 }
 
 // x int8 [T, K] with scales sx [T]; w int8 [N, K] (SwiGLU: [2 N, K], gate rows first) with scales sw; K a multiple of 16, both
-// 16-byte aligned. y [T, N] in out_dt (epilogues 0 and 3) or float (1, 2: added), row stride ldy.
+// 16-byte aligned. y [T, N] in out_dt (epilogues 0 and 3) or float (1, 2: added), row stride ldy. w_fixed: w's codes are not written by work
+// that may still be running, so that they are read before the kernel in front has ended.
 RLLM_API int rllm_int8_gemm(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
-                            int T, int N, int K, int* err, int sm_count, void* stream) {
+                            int T, int N, int K, int w_fixed, int* err, int sm_count, void* stream) {
   if (T <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 16 || K > 131072 || ldy < N || epi < 0 || epi > 3 || N > (1 << 30)) return ERR_BAD_SIZE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
   if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
   const int size = epi == EPI_STORE_F32 || epi == EPI_ACCUM_F32 || out_dt == DT_F32 ? 4 : 2;
-  const Int8Params p = {sx, sw, y, ldy, !(((uintptr_t)y | (uintptr_t)sw) & 15) && ldy * size % 16 == 0 && N % 4 == 0, T, N, K, 0, 1, err};
+  const Int8Params p = {sx, sw, y, ldy, !(((uintptr_t)y | (uintptr_t)sw) & 15) && ldy * size % 16 == 0 && N % 4 == 0, T, N, K, 0, 1, w_fixed, err};
   cudaStream_t s = (cudaStream_t)stream;
   if (epi == EPI_STORE_F32) return launch_epi<EPI_STORE_F32, float>(x, w, p, sm_count, s);
   if (epi == EPI_ACCUM_F32) return launch_epi<EPI_ACCUM_F32, float>(x, w, p, sm_count, s);
@@ -746,24 +751,24 @@ RLLM_API int rllm_quantize_rows(int dt, const void* x, long long ldx, const int*
                                 long long ldc, float* scales, int T, int K, int early, void* stream);
 RLLM_API int rllm_int8_streams(int T, int xk, int x_dt, const void* x, long long ldx, const void* g);
 RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
-                              const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int sm_count,
+                              const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int w_fixed, int sm_count,
                               void* stream);
 
 RLLM_API int rllm_int8_streams_codes(int epi, int T, int N, int K, int sm_count);
 RLLM_API int rllm_int8_stream_codes(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
-                                    int T, int N, int K, int sm_count, void* stream);
+                                    int T, int N, int K, int w_fixed, int sm_count, void* stream);
 
 // y = x w^T from numbers x [*, xk] (as rllm_quantize_rows takes them): in one kernel for few tokens, else quantised into codes [T, K] and scales [T]
 // first. Without scratch (codes null) a product that wants it is not run: 1000000.
 RLLM_API int rllm_int8_linear(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
                               void* codes, float* scales, const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk,
-                              int K, int* err, int sm_count, void* stream) {
+                              int K, int w_fixed, int* err, int sm_count, void* stream) {
   if (T <= 0 || N <= 0) return 0;
   if (rllm_int8_streams(T, xk, x_dt, x, ldx, g))
-    return rllm_int8_stream(epi, out_dt, x_dt, x, ldx, rows, g, g_dt, eps, w, sw, y, ldy, T, N, xk, K, sm_count, stream);
+    return rllm_int8_stream(epi, out_dt, x_dt, x, ldx, rows, g, g_dt, eps, w, sw, y, ldy, T, N, xk, K, w_fixed, sm_count, stream);
   if (codes == nullptr) return 1000000;
   const int rc = rllm_quantize_rows(x_dt, x, ldx, rows, g, g_dt, eps, codes, K, scales, T, xk, 1, stream);
   if (!rc && rllm_int8_streams_codes(epi, T, N, K, sm_count))
-    return rllm_int8_stream_codes(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, sm_count, stream);
-  return rc ? rc : rllm_int8_gemm(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, err, sm_count, stream);
+    return rllm_int8_stream_codes(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, w_fixed, sm_count, stream);
+  return rc ? rc : rllm_int8_gemm(epi, out_dt, codes, scales, w, sw, y, ldy, T, N, K, w_fixed, err, sm_count, stream);
 }

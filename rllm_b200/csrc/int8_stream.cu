@@ -33,6 +33,7 @@ struct StreamParams {
   void* y; long long ldy;
   int T, N, K, njobs;
   int epi, out_f32;
+  int w_fixed;                       // nothing in front of this kernel writes the weight
 };
 
 constexpr int SNT = 8;
@@ -141,7 +142,8 @@ int8_stream_kernel(const StreamParams p) {
     asm volatile("cp.async.commit_group;" ::: "memory");
     pslot = pslot + 1 == RING ? 0 : pslot + 1;
   };
-  // the weights need not wait for the kernel in front: what writes a weight's codes lets no kernel start before it ends
+  // the weights need not wait for the kernel in front, unless it, or one before it, may still write them
+  if (!p.w_fixed) pdl_wait();
 #pragma unroll
   for (int i = 0; i < RING; ++i) produce();
   pdl_wait();
@@ -248,10 +250,10 @@ int8_stream_kernel(const StreamParams p) {
         s0 += part[0];
         if (TILES == 2) s1 += part[WARPS * 16 * SNT];
       }
-      const float sx = s_scale[tok], v = (float)s0 * sx * __ldg(p.sw + n);
+      const float sx = s_scale[tok], v = __fmul_rn((float)s0 * sx, p.sw[n]);      // (rounded before it is added, as in int8_gemm.cu)
       const size_t o = (size_t)tok * p.ldy + n;
       if (p.epi == EPI_ACCUM_F32) { ((float*)p.y)[o] += v; continue; }
-      const float out = TILES == 2 ? silu_gate(v, (float)s1 * sx * __ldg(p.sw + p.N + n), p.out_f32) : v;
+      const float out = TILES == 2 ? silu_gate(v, (float)s1 * sx * p.sw[p.N + n], p.out_f32) : v;
       if (p.out_f32) ((float*)p.y)[o] = out; else ((bf16*)p.y)[o] = __float2bfloat16_rn(out);
     }
     if (batch0 + BATCH < my_jobs) __syncthreads();        // the sums are read before the next batch overwrites them
@@ -289,7 +291,7 @@ RLLM_API int rllm_int8_streams(int T, int xk, int x_dt, const void* x, long long
 // x [*, xk] float or bf16 (x_dt) with row stride ldx, rows int32 [T] or null, g norm weight [xk] (g_dt) or null; the rest as for
 // rllm_int8_gemm, K what xk is padded to.
 RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
-                              const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int sm_count,
+                              const void* w, const float* sw, void* y, long long ldy, int T, int N, int xk, int K, int w_fixed, int sm_count,
                               void* stream) {
   if (T <= 0 || N <= 0) return 0;
   if ((out_dt != DT_F32 && out_dt != DT_BF16) || (x_dt != DT_F32 && x_dt != DT_BF16)) return ERR_BAD_DTYPE;
@@ -297,7 +299,7 @@ RLLM_API int rllm_int8_stream(int epi, int out_dt, int x_dt, const void* x, long
     return ERR_BAD_SIZE;
   if ((uintptr_t)w & 15) return ERR_BAD_ALIGN;
   const bool out_f32 = out_dt == DT_F32 || epi == EPI_STORE_F32;
-  const StreamParams p = {x, ldx, rows, g, g_dt == DT_BF16, eps, nullptr, xk, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi, out_f32};
+  const StreamParams p = {x, ldx, rows, g, g_dt == DT_BF16, eps, nullptr, xk, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi, out_f32, w_fixed};
   cudaStream_t s = (cudaStream_t)stream;
   if (x_dt == DT_F32) return epi == EPI_SWIGLU ? launch_stream_k<FLOATS, 2>(p, sm_count, s) : launch_stream_k<FLOATS, 1>(p, sm_count, s);
   return epi == EPI_SWIGLU ? launch_stream_k<NUMBERS, 2>(p, sm_count, s) : launch_stream_k<NUMBERS, 1>(p, sm_count, s);
@@ -310,12 +312,12 @@ RLLM_API int rllm_int8_streams_codes(int epi, int T, int N, int K, int sm_count)
   return T <= SNT && K <= WARPS * 512 && epi != EPI_SWIGLU && (N + 15) / 16 <= sm_count;
 }
 RLLM_API int rllm_int8_stream_codes(int epi, int out_dt, const void* x, const float* sx, const void* w, const float* sw, void* y, long long ldy,
-                                    int T, int N, int K, int sm_count, void* stream) {
+                                    int T, int N, int K, int w_fixed, int sm_count, void* stream) {
   if (T <= 0 || N <= 0) return 0;
   if (out_dt != DT_F32 && out_dt != DT_BF16) return ERR_BAD_DTYPE;
   if (K <= 0 || K % 16 || ldy < N || epi < 0 || epi > 3 || !rllm_int8_streams_codes(epi, T, N, K, sm_count)) return ERR_BAD_SIZE;
   if (((uintptr_t)x | (uintptr_t)w) & 15) return ERR_BAD_ALIGN;
   const StreamParams p = {x, K, nullptr, nullptr, 0, 0.f, sx, K, (const int8_t*)w, sw, y, ldy, T, N, K, (N + 15) / 16, epi,
-                          out_dt == DT_F32 || epi == EPI_STORE_F32};
+                          out_dt == DT_F32 || epi == EPI_STORE_F32, w_fixed};
   return launch_stream<CODES, 1, 4, 2>(p, sm_count, (cudaStream_t)stream);
 }

@@ -194,8 +194,7 @@ int launch_rows(const RowArgs& a, int T_, cudaStream_t s) {
 }  // namespace
 
 // x [*, K] float or bf16 with row stride ldx; rows int32 [T] or null; g norm weight [K] (g_dt) or null. codes int8 [T, ldc], ldc a
-// multiple of 16 that holds K, zeros behind K; scales float [T]. early 0 for a weight: the products read its codes before they wait for
-// the kernel in front of them.
+// multiple of 16 that holds K, zeros behind K; scales float [T]. early: the next kernel in the stream may begin before this one has ended.
 RLLM_API int rllm_quantize_rows(int dt, const void* x, long long ldx, const int* rows, const void* g, int g_dt, float eps,
                                 void* codes, long long ldc, float* scales, int T, int K, int early, void* stream) {
   if (T <= 0) return 0;

@@ -18,10 +18,10 @@ from . import ops, sm100
 _P = c_void_p
 ops.register_signatures("quant", {
     "rllm_quantize_rows": [c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, c_longlong, _P, c_int, c_int, c_int, _P],
-    "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, _P, c_int, _P],
+    "rllm_int8_gemm": [c_int, c_int, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P, c_int, _P],
     "rllm_int8_plan": [c_int, c_int, c_int, c_int, c_int, _P, _P],
     "rllm_int8_linear": [c_int, c_int, c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int,
-                         c_int, _P, c_int, _P],
+                         c_int, c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
     "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int,
                       c_int, _P],
@@ -74,7 +74,26 @@ class Int8Rows:
 
 
 class Int8Matrix(Int8Rows):
-    """A weight [N, K] in 8 bits, a scale per output channel: the backend's products take it where they take a tensor."""
+    """A weight [N, K] in 8 bits, a scale per output channel: the backend's products take it where they take a tensor. A product copies the codes
+    of a `settled` matrix before the kernel in front of it has ended; those of any other, one put together from tensors or written
+    to since, only then."""
+    _settled = None
+
+    def settle(self) -> "Int8Matrix":
+        """Waits for the work that writes the codes; they are not to be written after. (Nothing is waited for, and the matrix is not settled,
+        while a graph is captured.)"""
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.device).synchronize()
+            self._settled = self._version()
+        return self
+
+    def _version(self):
+        return -1 if self.codes.is_inference() else self.codes._version       # (what torch counts a tensor's writes by)
+
+    @property
+    def settled(self) -> bool:
+        n = self._settled
+        return n is not None and (n == -1 or n == self.codes._version)
 
 
 def _rows(x: torch.Tensor, norm: tuple | None, rows: torch.Tensor | None):
@@ -113,8 +132,8 @@ def quantize_rows(x: torch.Tensor, norm: tuple | None = None, rows: torch.Tensor
 
 
 def quantize_matrix(w: torch.Tensor) -> Int8Matrix:
-    """A weight [N, K] in 8 bits, a scale per row (output channel)."""
-    return quantize_rows(w, cls=Int8Matrix)
+    """A weight [N, K] in 8 bits, a scale per row (output channel). Done when it returns (`Int8Matrix.settle`)."""
+    return quantize_rows(w, cls=Int8Matrix).settle()
 
 
 def _output(T: int, K: int, w: Int8Matrix, epilogue: int, out: torch.Tensor | None, out_dtype: torch.dtype, device):
@@ -157,7 +176,7 @@ def linear_int8(x: Int8Rows, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: 
     st = sm100.init(x.codes.device)
     ops._check(ops._fn("quant", "rllm_int8_gemm")(
         epilogue, ops._dt(out, "out"), x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-        max(out.stride(0), N), T, N, x.codes.shape[1], st.err.data_ptr(), st.sm_count, ops._stream()), "linear_int8")
+        max(out.stride(0), N), T, N, x.codes.shape[1], int(w.settled), st.err.data_ptr(), st.sm_count, ops._stream()), "linear_int8")
     return out
 
 
@@ -173,11 +192,11 @@ def linear(x: torch.Tensor, w: Int8Matrix, epilogue: int = ops.EPI_STORE, out: t
     device = x.device
     N, out = _output(T, K, w, epilogue, out, out_dtype, device)
     st = sm100.init(device)
-    KP = w.codes.shape[1]
+    KP, fixed = w.codes.shape[1], int(w.settled)
     fn = ops._fn("quant", "rllm_int8_linear")
     call = lambda codes, scales: fn(
         epilogue, ops._dt(out, "out"), dt, x.data_ptr(), x.stride(0), ops._ptr(rows), g, g_dt, eps, codes, scales, w.codes.data_ptr(),
-        w.scales.data_ptr(), out.data_ptr(), max(out.stride(0), N), T, N, K, KP, st.err.data_ptr(), st.sm_count, ops._stream())
+        w.scales.data_ptr(), out.data_ptr(), max(out.stride(0), N), T, N, K, KP, fixed, st.err.data_ptr(), st.sm_count, ops._stream())
     rc = call(None, None) if T <= STREAM_TOKENS else _NEEDS_SCRATCH
     launches = 1
     if rc == _NEEDS_SCRATCH:

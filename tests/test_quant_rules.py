@@ -107,3 +107,16 @@ def test_the_plain_forms_themselves():
     far = (Q.fake4(x) - x).abs().unflatten(-1, (-1, 32)) / d.abs()[..., None]
     assert float(far.max()) <= 1.0 + 8 * 2 ** -8 and float(far.median()) < 0.5
     assert float((Q.fake8(x[0]) - x[0]).abs().max()) <= float(x[0].abs().max()) / 254 * (1 + 1e-6)
+
+
+def test_a_matrix_is_settled_by_its_maker_only():
+    """Products read a settled matrix before the kernel in front of them has ended: one put together by a caller, or written to since, is not."""
+    m = quant.Int8Matrix(torch.zeros(4, 48, dtype=torch.int8), torch.zeros(4), 48)
+    assert not m.settled
+    m._settled = m._version()
+    assert m.settled
+    m.codes[0, 0] = 1
+    assert not m.settled
+    with torch.inference_mode():
+        n = quant.Int8Matrix(torch.zeros(4, 48, dtype=torch.int8), torch.zeros(4), 48)
+    assert not n.settled and n._version() == -1
