@@ -10,7 +10,7 @@ from ..config import config_from_dict, load_config
 from ..kernels.backend import Backend
 from ..parts.base import KV4CacheSpec, cache_kind_of
 from ..weights import init_random_weights, load_weights
-from .step import Engine
+from .step import Engine, any_engine
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
            "float32": torch.float32, "fp32": torch.float32, "f32": torch.float32}
@@ -29,44 +29,60 @@ KV_QUANT = ("none", "int4")
 WEIGHT_QUANT = ("none", "int8")
 
 
-def set_kv_quant(model, kv_quant: str) -> None:
-    """"int4": every layer's keys and values are held in 4 bits (`KV4CacheSpec`); a model with another paged cache is refused.
-    Before the cache is made."""
+def _may_change(model, what: str, asked: str, has: str) -> bool:
+    """Is the model to be changed from the form that it `has` to the one asked for? Its parts are what every engine of it runs, with their captured
+    steps: the form is chosen before the first, and never taken back."""
+    if asked == has:
+        return False
+    if has != "none":
+        raise ValueError(f"{what} {asked!r}: this model has been given {what} {has!r}, which cannot be taken back; load it again")
+    if any_engine(model):
+        raise ValueError(f"{what} {asked!r}: another engine runs this model with {what} 'none'; load it again for this one")
+    return True
+
+
+def set_kv_quant(model, kv_quant: str) -> list:
+    """"int4": every layer's keys and values are held in 4 bits (`KV4CacheSpec`); a model with another paged cache is refused and left as it
+    was, and so is one that an engine runs otherwise. Before the cache is made. Returns the parts that were changed."""
     if kv_quant not in KV_QUANT:
         raise ValueError(f"kv_quant must be one of {KV_QUANT}, got {kv_quant!r}")
-    if kv_quant == "none":
-        return
-    specs = [s for s in model.cache_specs() if s is not None and cache_kind_of(s).paged]
     able = [p for p in model.parts() if hasattr(p, "use_kv4")]
+    if not _may_change(model, "kv_quant", kv_quant, "int4" if any(p.kv4 for p in able) else "none"):
+        return []
+    specs = [s for s in model.cache_specs() if s is not None and cache_kind_of(s).paged]
     if not able:
         raise ValueError(f"kv_quant {kv_quant!r}: this model has no cache of keys and values that can be held in 4 bits"
                          + (f" (it has {sorted({type(s).__name__ for s in specs})})" if specs else ""))
-    for p in able:
-        p.use_kv4()
-    left = sorted({type(s).__name__ for s in model.cache_specs()
-                   if s is not None and cache_kind_of(s).paged and not isinstance(s, KV4CacheSpec)})
-    if left:
-        raise ValueError(f"kv_quant {kv_quant!r}: layers with {left} cannot be held in 4 bits")
+    try:
+        for p in able:
+            p.use_kv4()
+        left = sorted({type(s).__name__ for s in model.cache_specs()
+                       if s is not None and cache_kind_of(s).paged and not isinstance(s, KV4CacheSpec)})
+        if left:
+            raise ValueError(f"kv_quant {kv_quant!r}: layers with {left} cannot be held in 4 bits")
+    except ValueError:
+        for p in able:
+            p.kv4 = False
+        raise
+    return able
 
 
 def set_weight_quant(model, weight_quant: str) -> None:
     """"int8": the matrices that the parts declare (`Part.int8_params`) are held in 8 bits with a scale per output channel, and their
-    inputs are quantised per token. Embedding and output head stay as they are. After the weights are bound."""
+    inputs are quantised per token. Embedding and output head stay as they are. A model that an engine runs otherwise is refused. After the weights are bound."""
     if weight_quant not in WEIGHT_QUANT:
         raise ValueError(f"weight_quant must be one of {WEIGHT_QUANT}, got {weight_quant!r}")
-    if weight_quant == "none":
-        return
     from ..kernels import quant
-    seen = False
-    for p in model.parts():
-        for name in p.int8_params:
-            w = getattr(p, name)
-            if not isinstance(w, quant.Int8Matrix):        # (a model may be given to a second engine)
-                with torch.cuda.device(w.device):
-                    setattr(p, name, quant.quantize_matrix(w))
-            seen = True
-    if not seen:
+    held = [(p, n) for p in model.parts() for n in p.int8_params]
+    has = any(isinstance(getattr(p, n), quant.Int8Matrix) for p, n in held)
+    if not _may_change(model, "weight_quant", weight_quant, "int8" if has else "none"):
+        return
+    if not held:
         raise ValueError(f"weight_quant {weight_quant!r}: no part of this model has matrices that can be held in 8 bits")
+    for p, name in held:
+        w = getattr(p, name)
+        with torch.cuda.device(w.device):
+            setattr(p, name, quant.quantize_matrix(w))
 
 
 def default_num_pages(model, page_size: int, dtype: torch.dtype, device, weights_bytes: int = 0,
@@ -86,8 +102,13 @@ def make_engine(model, dtype, device="cuda:0", page_size: int = 16, num_pages: i
                 weight_quant: str = "none") -> Engine:
     """`model` must already hold its weights on `device`."""
     dtype = parse_dtype(dtype)
-    set_kv_quant(model, kv_quant)
-    set_weight_quant(model, weight_quant)
+    changed = set_kv_quant(model, kv_quant)
+    try:
+        set_weight_quant(model, weight_quant)
+    except ValueError:
+        for p in changed:
+            p.kv4 = False
+        raise
     backend = Backend(dtype, device)
     if num_pages is None:
         if max_tokens is not None:

@@ -16,8 +16,10 @@ the cache are the same either way.
 """
 from __future__ import annotations
 
+import gc
 import logging
 import os
+import weakref
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -60,9 +62,20 @@ class MetaLayout:
         return buf[o: o + n]
 
 
+def any_engine(model) -> bool:
+    """Is there an engine that runs this model?"""
+    if not getattr(model, "engines", None):
+        return False
+    gc.collect()                      # (an engine and its captured steps refer to one another)
+    return bool(model.engines)
+
+
 class Engine:
     def __init__(self, model, backend, cache: CacheManager, use_graphs: bool | None = None):
         self.model, self.backend, self.cache = model, backend, cache
+        if not hasattr(model, "engines"):
+            model.engines = weakref.WeakSet()
+        model.engines.add(self)
         self.device = backend.device
         self.vocab = model.vocab_size
         # device words: [0] a kernel's bounded wait ran out, [1] a token id outside the table,
