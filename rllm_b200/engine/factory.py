@@ -69,7 +69,8 @@ def set_kv_quant(model, kv_quant: str) -> list:
 
 def set_weight_quant(model, weight_quant: str) -> None:
     """"int8": the matrices that the parts declare (`Part.int8_params`) are held in 8 bits with a scale per output channel, and their
-    inputs are quantised per token. Embedding and output head stay as they are. A model that an engine runs otherwise is refused. After the weights are bound."""
+    inputs are quantised per token. Embedding and output head stay as they are; a model whose layers have other matrices is refused, and so is one
+    that an engine runs otherwise. After the weights are bound."""
     if weight_quant not in WEIGHT_QUANT:
         raise ValueError(f"weight_quant must be one of {WEIGHT_QUANT}, got {weight_quant!r}")
     from ..kernels import quant
@@ -79,6 +80,10 @@ def set_weight_quant(model, weight_quant: str) -> None:
         return
     if not held:
         raise ValueError(f"weight_quant {weight_quant!r}: no part of this model has matrices that can be held in 8 bits")
+    left = sorted({f"{type(p).__name__}.{q.attr}" for b in model.blocks for p in b.walk() for q in p.params()
+                   if len(q.shape) > 1 and q.role == "matrix" and q.attr not in p.int8_params})
+    if left:
+        raise ValueError(f"weight_quant {weight_quant!r}: {', '.join(left)} cannot be held in 8 bits")
     for p, name in held:
         w = getattr(p, name)
         with torch.cuda.device(w.device):

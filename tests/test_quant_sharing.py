@@ -119,3 +119,12 @@ def test_an_engine_is_known_while_it_lives():
     del a, b
     gc.collect()
     assert not any_engine(m)
+
+
+def test_a_model_that_would_be_quantised_in_part_is_refused(on_cpu):
+    """Livovik's shared expert is a SwiGLU like Llama's; its attention and its routed experts have matrices of their own kinds."""
+    from livovik_tiny import LA
+    m = model_of(LA)
+    with pytest.raises(ValueError, match="SinkGQAttention.*cannot be held in 8 bits"):
+        set_weight_quant(m, "int8")
+    assert not on_cpu
