@@ -88,14 +88,16 @@ def set_weight_quant(model, weight_quant: str) -> None:
         w = getattr(p, name)
         with torch.cuda.device(w.device):
             setattr(p, name, quant.quantize_matrix(w))
+            del w
+            torch.cuda.empty_cache()           # its memory goes back to the device, before the next one's codes are cut out of it
 
 
 def default_num_pages(model, page_size: int, dtype: torch.dtype, device, weights_bytes: int = 0,
                       fraction: float = 0.75) -> int:
     """Pages that fit in `fraction` of the free device memory (the reference takes 75 % of
     what is left after the weights, src/model/config.rs:1195-1226, clamped there to
-    [256, 8192] blocks; here only a floor is kept)."""
-    free, _ = torch.cuda.mem_get_info(device)
+    [256, 8192] blocks; here only a floor is kept). What torch keeps of freed tensors is free too."""
+    free = torch.cuda.mem_get_info(device)[0] + torch.cuda.memory_reserved(device) - torch.cuda.memory_allocated(device)
     per_page = CacheManager.bytes_per_page(model.cache_specs(), page_size, dtype)
     if per_page == 0:
         return 0
