@@ -117,8 +117,8 @@ __device__ __forceinline__ uint32_t block_max2(uint32_t v) {
 
 // Places i * out_page .. of sequence s go to page s * width + i of the output, in the cache's order [kv head][offset][hd]; places behind
 // the sequence's last token are zeros, and so are those in pages it does not hold. A CTA takes one kv head's part of a page. With `cu_q` (attention
-// of portions) pages that no query of the step sees are left out; table_out says which are there, cu_out counts the portions' rows
-// from zero.
+// of portions) i counts from the page of the first place that a query of the step sees, and pages that none sees are left out; table_out
+// [table_width pages from place 0 on] says where which are, cu_out counts the portions' rows from zero.
 // vexp: the values are 16-bit numbers times a power of two a page and kv head (`value_word`). A value has 12 significant bits: half numbers hold 11
 // of them, bfloat16 8, but half numbers have few powers of two. So a page whose scales lie within 2^6 of each other is half numbers, its
 // largest scale between 1 and 2; any other is bfloat16, its smallest scale (but not less than 2^-40 of its largest) between 1 and 2. The power
@@ -131,18 +131,22 @@ template <typename T, int UNITS>
 __global__ void __launch_bounds__(THREADS)
 kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ kv_lens,
                 const int* __restrict__ cu_q, int window, int num_seqs, int width, int out_page, T* __restrict__ k, T* __restrict__ v,
-                int* __restrict__ table_out, int* __restrict__ cu_out, int* __restrict__ vexp) {
+                int table_width, int* __restrict__ table_out, int* __restrict__ cu_out, int* __restrict__ vexp) {
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x, s = blockIdx.y;
   const bool is_v = (int)blockIdx.z >= c.nkv;
   const int kvh = (int)blockIdx.z - (is_v ? c.nkv : 0);
-  const int n = kv_lens[s], j0 = i * out_page;
+  const int n = kv_lens[s];
   int first = 0;                                         // the first position that a query sees
   if (cu_q != nullptr && window > 0) first = max(0, n - (cu_q[s + 1] - cu_q[s]) - window + 1);
-  const bool left_out = table_out != nullptr && (j0 >= n || j0 + out_page <= first);
+  const int base = first > 0 ? first / out_page : 0, at = base + i, j0 = at * out_page;
+  const bool left_out = table_out != nullptr && (j0 >= n || at >= table_width);
+  if (table_out != nullptr && i == 0 && blockIdx.z == 0)
+    for (int t = threadIdx.x; t < table_width; t += THREADS)
+      if (t < base || t >= base + width) table_out[(size_t)s * table_width + t] = -1;
   if (threadIdx.x == 0 && blockIdx.z == 0) {
-    if (table_out != nullptr) table_out[(size_t)s * width + i] = left_out ? -1 : s * width + i;
+    if (table_out != nullptr && at < table_width) table_out[(size_t)s * table_width + at] = left_out ? -1 : s * width + i;
     if (cu_out != nullptr && i == 0) {
       cu_out[s] = cu_q[s] - cu_q[0];
       if (s == num_seqs - 1) cu_out[s + 1] = cu_q[s + 1] - cu_q[0];
@@ -250,18 +254,19 @@ RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk,
 }
 
 // The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, out_page, hd] float or bf16 (rounded once). kv_lens int32
-// [num_seqs], none above width * out_page; block_table int32 with an entry for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, width] and cu_out
+// [num_seqs], none above width * out_page (with cu_q and a window: no more places seen than `width` pages hold); block_table int32 with an entry
+// for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, table_width] and cu_out
 // [num_seqs + 1], and vexp [num_seqs * width, nkv] (bf16 only: v is then 16-bit numbers as `value_word` says; out_page * hd / 64 between 32 and 256) for attention of portions, or null.
 RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
                            const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, int out_page, void* k,
-                           void* v, int* table_out, int* cu_out, int* vexp, int nkv, int page_size, int hd, void* stream) {
+                           void* v, int table_width, int* table_out, int* cu_out, int* vexp, int nkv, int page_size, int hd, void* stream) {
   if (num_seqs <= 0 || width <= 0) return 0;
   if (out_page <= 0 || 2 * nkv > 65535) return ERR_BAD_SIZE;
   if (vexp != nullptr && (dt != DT_BF16 || (long long)out_page * (hd >> 6) > 8 * (THREADS / 8) || out_page * (hd >> 6) < THREADS / 8)) return ERR_BAD_SIZE;
   Pages c;
   const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
   if (rc) return rc;
-  if (num_seqs > 65535 || (cu_out != nullptr && cu_q == nullptr) || (long long)num_seqs * width > 2147483647LL || (long long)width * out_page > 2147483647LL) return ERR_TOO_LARGE;
+  if (num_seqs > 65535 || (cu_out != nullptr && cu_q == nullptr) || (long long)num_seqs * width > 2147483647LL || (long long)width * out_page > 2147483647LL || (long long)table_width * out_page > 2147483647LL) return ERR_TOO_LARGE;
   if (((uintptr_t)k | (uintptr_t)v) & 15) return ERR_BAD_ALIGN;
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid(width, num_seqs, 2 * nkv);
@@ -270,7 +275,7 @@ RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long 
   auto run = [&](auto type, auto kernel) {
     typedef decltype(type) T;
     return launch_ex(kernel, grid, dim3(THREADS), 0, s, 1, c, num_pages, shift, block_table, bt_stride, kv_lens, cu_q, window, num_seqs, width,
-                     out_page, (T*)k, (T*)v, table_out, cu_out, vexp);
+                     out_page, (T*)k, (T*)v, table_width, table_out, cu_out, vexp);
   };
   const long long each = ((long long)out_page * (hd >> 6) + THREADS / 8 - 1) / (THREADS / 8);
   if (dt == DT_F32) return each <= 1 ? run(float(), kv4_read_kernel<float, 1>) : each <= 4 ? run(float(), kv4_read_kernel<float, 4>) : run(float(), kv4_read_kernel<float, 8>);

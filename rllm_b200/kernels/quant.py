@@ -23,8 +23,8 @@ ops.register_signatures("quant", {
     "rllm_int8_linear": [c_int, c_int, c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int,
                          c_int, c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
-    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, c_int,
-                      c_int, _P],
+    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, c_int,
+                      c_int, c_int, _P],
     "rllm_kv4_decode": [_P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                         c_int, c_int, _P],
     "rllm_kv4_attention_simt": [c_int, _P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
@@ -267,7 +267,7 @@ def kv4_read(tensors: dict, block_table: torch.Tensor, kv_lens: torch.Tensor, ma
     k, v = torch.empty((2, S, width, nkv, page_size, hd), dtype=dtype, device=k4.device).unbind(0)
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops._dt(k, "k"), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr(),
-        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), None, None, None, nkv, page_size, hd,
+        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), 0, None, None, None, nkv, page_size, hd,
         ops._stream()), "kv4_read")
     return k, v
 
@@ -294,7 +294,7 @@ def attention_kv4_simt(q: torch.Tensor, tensors: dict, token_seq: torch.Tensor, 
     return out
 
 
-# Places of a key range's page in the scratch that portions are read into, and bytes of scratch a run of portions may take at once
+# Places of a page in the scratch that portions are read into, and bytes of it that several sequences may take at once (more: one by one)
 READ_PAGE, READ_BYTES = 128, 2 << 30
 
 
@@ -401,7 +401,10 @@ def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> 
     memory left does not hold the scratch."""
     s0, s1, r0, r1, _, longest, most = run
     k4, ks, v4, vs, pages, nkv, page_size, hd = kv
-    S, width, T = s1 - s0, -(-most // READ_PAGE), r1 - r0
+    S, T, entries = s1 - s0, r1 - r0, -(-most // READ_PAGE)
+    # pages of a sequence that its rows see any place of: `span` places, wherever in a page they begin
+    span = window + longest - 1 if window else most
+    width = min(entries, (span + READ_PAGE - 2) // READ_PAGE + 1)
     size = S * width * nkv * READ_PAGE * hd * 2
     if S > 1 and 2 * size > READ_BYTES:            # one by one, then
         row = r0
@@ -417,16 +420,16 @@ def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> 
         return False
     k, v = room.unbind(0)
     v = v.view(torch.float16)
-    table, vexp, cu = q.new_empty(S * width * (1 + nkv) + S + 1, dtype=torch.int32).split((S * width, S * width * nkv, S + 1))
+    table, vexp, cu = q.new_empty(S * (entries + width * nkv) + S + 1, dtype=torch.int32).split((S * entries, S * width * nkv, S + 1))
     whole = S == ctx.num_seqs                      # (a view costs the host as much as half a launch)
     kv_lens = ctx.kv_lens if whole else ctx.kv_lens[s0:s1]
     if not whole:
         q, out = q[r0:r1], out[r0:r1]
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr() + 4 * s0 * block_table.stride(0),
-        block_table.stride(0), kv_lens.data_ptr(), ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+        block_table.stride(0), kv_lens.data_ptr(), ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), entries, table.data_ptr(),
         cu.data_ptr(), vexp.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
-    a = (q, k, v, cu, kv_lens, table.view(S, width))
+    a = (q, k, v, cu, kv_lens, table.view(S, entries))
     if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(q, k):
         items = -(-longest * (nh // nkv) // 256) * nkv * S
         parts = portion_parts(items, min(most, window + longest) if window else most, hd, sm100.init(q.device).sm_count)

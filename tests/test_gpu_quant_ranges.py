@@ -149,3 +149,28 @@ def test_single_tokens_whose_weight_lies_on_few_keys(kind, hd):
     for splits in (1, 3, 8):
         y = quant().attention_kv4_decode(q, t, lens_d, table, nh, 16 / hd, None, 700, splits)
         check(y, q, held, lens, [1], nh, hd, 16 / hd, None, False)
+
+
+@pytest.mark.parametrize("kernel", ["short", "long"])
+@pytest.mark.parametrize("known", [True, False])
+def test_portions_in_a_window_take_scratch_for_what_they_see(known, kernel, monkeypatch):
+    """Long contexts of which a window leaves little, at every place of a page of the scratch: numbers of the pages that a row sees any place of."""
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if kernel == "long" else 1 << 30)
+    lens, q_lens, nh, nkv, hd, window = [9000, 4991, 600, 129], [65, 128, 40, 129], 8, 2, 64, 300
+    t, table, held = make("like", lens, nkv, hd, seed=8)
+    for s, (L, n) in enumerate(zip(lens, q_lens)):         # as the engine gives pages back
+        table[s, : max(0, L - n - window + 1) // 16] = -1
+    q = rnd(sum(q_lens), nh * hd, seed=6, dtype=torch.bfloat16, scale=1.5).to(DEV)
+    asked = []
+
+    def scratch(size, make):
+        asked.append(size)
+        return make()
+    _, (be, ctx, cache) = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, hd ** -0.5, window)
+    if not known:
+        ctx.kv_lens_host = None
+    ctx.per_forward.clear()
+    y = quant().attention_kv4(q, t, ctx, table, nh, hd ** -0.5, window, True, scratch)
+    check(y, q, held, lens, q_lens, nh, hd, hd ** -0.5, window, True)
+    # 129 + 299 places lie in five pages of 128 at most: k and v of 4 sequences, 2 bytes a number
+    assert asked and max(asked) <= 2 * 4 * 5 * nkv * 128 * hd * 2, asked
