@@ -84,14 +84,12 @@ kv4_attention_simt_kernel(const Kv4Params p) {
   float m = -INFINITY, l = 0.f;
   for (int base = start; base <= pos; base += 32) {
     const int j = base + lane;
-    bool valid = j <= pos;
-    float s = -INFINITY;
-    long long row = 0;
+    const bool valid = j <= pos;
+    float s = valid ? 0.f : -INFINITY;
+    long long row = -1;
     const int page = valid ? bt[j / p.page_size] : -1;
-    valid = valid && page >= 0 && page < p.num_pages;      // a table entry without a page: not read
-    if (valid) {
+    if (page >= 0 && page < p.num_pages) {                 // a table entry without a page reads as zeros
       row = ((long long)page * p.nkv + kvh) * p.page_size + j % p.page_size;
-      s = 0.f;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const uint4* kp = reinterpret_cast<const uint4*>(p.k4 + row * (HD / 2) + 32 * b);
@@ -122,7 +120,7 @@ kv4_attention_simt_kernel(const Kv4Params p) {
     for (int jj = 0; jj < cnt; ++jj) {
       const float pj = __shfl_sync(0xffffffffu, pr, jj);
       const long long rj = __shfl_sync(0xffffffffu, row, jj);
-      if (!__shfl_sync(0xffffffffu, (int)valid, jj)) continue;
+      if (rj < 0) continue;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const uint32_t two = __ldcg(reinterpret_cast<const uint32_t*>(p.vs + rj * (HD / 32)) + b);

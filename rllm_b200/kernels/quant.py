@@ -280,7 +280,8 @@ def _queries(q, nh, nkv, hd, T):
 
 def attention_kv4_simt(q: torch.Tensor, tensors: dict, token_seq: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
                        nh: int, scale: float, window: int | None = None) -> torch.Tensor:
-    """Attention over 4 bits on the CUDA cores, in float: any rows, both run types, every head size."""
+    """Attention over 4 bits on the CUDA cores, in float: any rows, both run types, every head size. In this and every other form a visible place on
+    a page that the table does not hold is a key and a value of zeros, as `kv4_read` gives it."""
     k4, ks, v4, vs, pages, nkv, page_size, hd = _kv4(tensors)
     T = q.shape[0]
     _queries(q, nh, nkv, hd, T)

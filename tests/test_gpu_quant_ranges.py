@@ -174,3 +174,29 @@ def test_portions_in_a_window_take_scratch_for_what_they_see(known, kernel, monk
     check(y, q, held, lens, q_lens, nh, hd, hd ** -0.5, window, True)
     # 129 + 299 places lie in five pages of 128 at most: k and v of 4 sequences, 2 bytes a number
     assert asked and max(asked) <= 2 * 4 * 5 * nkv * 128 * hd * 2, asked
+
+
+@pytest.mark.parametrize("entry", [-1, 1 << 20])
+@pytest.mark.parametrize("hd,q_lens,dtype", [(64, [1, 1], "bfloat16"), (128, [1, 1], "bfloat16"), (64, [40, 64], "bfloat16"), (128, [64, 1], "bfloat16"),
+                                             (64, [1, 40], "float32"), (256, [1, 9], "bfloat16")])
+def test_a_visible_place_on_a_page_that_is_not_held_reads_as_zeros(hd, q_lens, dtype, entry, monkeypatch):
+    """The engine makes no such call; every form answers it alike: a key and a value of zeros."""
+    lens, nh, nkv = [300, 700], 4, 2
+    t, table, held = make("like", lens, nkv, hd, seed=5)
+    dt = getattr(torch, dtype)
+    q = rnd(sum(q_lens), nh * hd, seed=6, dtype=dt, scale=1.5).to(DEV)
+    for s, pages in ((0, (3,)), (1, (0, 9, 20, 21, 22, 23, 24, 25, 26, 27, 28, 29, 30, 31, 32, 33))):
+        for p in pages:
+            table[s, p] = entry
+            for x in held[s]:
+                x[16 * p: 16 * p + 16] = 0.0
+    for least in (1, 1 << 30):
+        monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", least)
+        y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, hd ** -0.5, None)
+        row = 0
+        for s, n in enumerate(q_lens):
+            want, mag, big = Q.attention(q[row: row + n].cpu().view(n, nh, hd), held[s][0], held[s][1], hd ** -0.5)
+            got = y[row: row + n].cpu().double().view(n, nh, hd)
+            row += n
+            tol = bound(dt, want, mag, big, hd, lens[s], dt == torch.bfloat16 and n > 1)
+            assert ((got - want).abs() <= tol).all(), (s, float(((got - want).abs() / tol).max()))
