@@ -80,6 +80,7 @@ struct FaParams {
                          // tokens than the caller said) is skipped, never written
   // V16: values are half numbers, or bfloat16, times 2^e, a word per page and kv head (quant.cuh); a page is a multiple of BN keys
   const int* vexp;       // [page * nkv + kv head]
+  const uint32_t* vlost; // a bit a place of every group whose values are NaN, on pages whose word says that there are such
 };
 
 // V16: a value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
@@ -151,6 +152,7 @@ fa_paged_kernel(const FaParams p) {
 #pragma unroll
   for (int i = 0; i < DTILES; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
   float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+  int lostA = 0, lostB = 0;             // V16: groups of 32 values that a NaN is among
 
   // What the 16 rows of this warp can see (the same for all its lanes): a tile wholly inside is
   // taken without a mask, a tile wholly outside is not computed at all.
@@ -212,6 +214,17 @@ fa_paged_kernel(const FaParams p) {
       const int page_v = V16 ? bt[pshift >= 0 ? (j0 >> pshift) : j0 / p.page_size] : -1;
       const int word = V16 && page_v >= 0 ? p.vexp[page_v * p.nkv + kvh] : 0, ve = value_exponent(word);
       const bool halves = V16 && !value_wide(word);
+      if (V16 && value_lost(word)) {                       // (the values are zeros there, for the rows that do not see them)
+        const int words = p.page_size / 32;
+        const uint32_t* bits = p.vlost + (size_t)(page_v * p.nkv + kvh) * (HD / 32) * words + j0 % p.page_size / 32;
+#pragma unroll 1
+        for (int x = 0; x < HD / 32 * (BN / 32); ++x) {
+          const int j = j0 + 32 * (x % (BN / 32));
+          const uint32_t b = bits[x / (BN / 32) * words + x % (BN / 32)];
+          if (b & bits_below(posA + 1 - j) & ~bits_below(loA - j)) lostA |= 1 << (x / (BN / 32));
+          if (b & bits_below(posB + 1 - j) & ~bits_below(loB - j)) lostB |= 1 << (x / (BN / 32));
+        }
+      }
       const float vef = (float)ve, vback = V16 ? __int_as_float((127 - ve) << 23) : 1.f;
       // ---- scores S = Q K^T : 16 rows x 64 keys; the K fragments of a k-step are fetched together
       float s[BN / 8][4];
@@ -304,6 +317,13 @@ fa_paged_kernel(const FaParams p) {
     __syncthreads();       // everyone is done with this buffer before it is refilled
   }
   cp_async_wait<0>();
+  if (V16 && (lostA | lostB)) {
+#pragma unroll
+    for (int i = 0; i < DTILES; ++i) {
+      if (lostA >> (i / 4) & 1) o[i][0] = o[i][1] = __int_as_float(0x7fc00000);
+      if (lostB >> (i / 4) & 1) o[i][2] = o[i][3] = __int_as_float(0x7fc00000);
+    }
+  }
 
   lA += __shfl_xor_sync(0xffffffffu, lA, 1); lA += __shfl_xor_sync(0xffffffffu, lA, 2);
   lB += __shfl_xor_sync(0xffffffffu, lB, 1); lB += __shfl_xor_sync(0xffffffffu, lB, 2);
@@ -380,7 +400,7 @@ int run_fa(const void* q, int q_stride, const void* kcache, const void* vcache, 
            int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
            int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
            int hd, int page_size, float scale, int window, int splits, float* part_o,
-           float* part_ml, const int* vexp, void* stream) {
+           float* part_ml, const int* vexp, const uint32_t* vlost, void* stream) {
   if (num_seqs <= 0 || num_tokens <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh % nkv || page_size <= 0) return ERR_BAD_SIZE;
   if (q_stride % 2 || out_stride % 2 || ((uintptr_t)q & 3) || ((uintptr_t)out & 3) ||
@@ -394,7 +414,7 @@ int run_fa(const void* q, int q_stride, const void* kcache, const void* vcache, 
   p.window = window; p.splits = splits; p.scale_log2e = scale * 1.4426950408889634f;
   p.page_shift = -1;
   if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
-  p.part_o = part_o; p.part_ml = part_ml; p.vexp = vexp;
+  p.part_o = part_o; p.part_ml = part_ml; p.vexp = vexp; p.vlost = vlost;
   p.part_rows = (long long)num_tokens * nh * splits;
   cudaStream_t s = (cudaStream_t)stream;
   const int G = nh / nkv;
@@ -421,18 +441,18 @@ RLLM_API int rllm_attention_fa(const void* q, int q_stride, const void* kcache, 
                                int hd, int page_size, float scale, int window, int splits, float* part_o,
                                float* part_ml, void* stream) {
   return run_fa(q, q_stride, kcache, vcache, out, out_stride, cu_q, kv_lens, block_table, bt_stride, num_seqs, num_tokens, max_q_len,
-                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, nullptr, stream);
+                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, nullptr, nullptr, stream);
 }
 
-// The same with values of 16 bits times a power of two, vexp[page * nkv + kv head] (quant.cuh: value_word); pages of a multiple of 64 keys.
-RLLM_API int rllm_attention_fa_v16(const void* q, int q_stride, const void* kcache, const void* vcache, const int* vexp, void* out,
+// The same with values of 16 bits times a power of two, vexp[page * nkv + kv head], and the places of NaNs, vlost (quant.cuh: value_word); pages of a multiple of 64 keys.
+RLLM_API int rllm_attention_fa_v16(const void* q, int q_stride, const void* kcache, const void* vcache, const int* vexp, const uint32_t* vlost, void* out,
                                    int out_stride, const int* cu_q, const int* kv_lens, const int* block_table,
                                    int bt_stride, int num_seqs, int num_tokens, int max_q_len, int nh, int nkv,
                                    int hd, int page_size, float scale, int window, int splits, float* part_o,
                                    float* part_ml, void* stream) {
-  if (!vexp || page_size <= 0 || page_size % BN) return ERR_BAD_SIZE;
+  if (!vexp || !vlost || page_size <= 0 || page_size % BN) return ERR_BAD_SIZE;
   return run_fa(q, q_stride, kcache, vcache, out, out_stride, cu_q, kv_lens, block_table, bt_stride, num_seqs, num_tokens, max_q_len,
-                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, vexp, stream);
+                nh, nkv, hd, page_size, scale, window, splits, part_o, part_ml, vexp, vlost, stream);
 }
 
 // ------------------------------------------------------------------------------------------

@@ -136,6 +136,7 @@ struct PfParams {
   float scale_log2e;
   // HALF_V: values are 16-bit numbers times 2^e, a word per page and kv head (quant.cuh): [page * nkv + kv head]; a page is a multiple of a tile's keys
   const int* vexp;
+  const uint32_t* vlost; // and a bit a place of every group whose values are NaN, on pages whose word says that there are such
   int parts;             // HALF_V: CTAs of a cluster that share an item's keys; with more than one a CTA has one item
   int* err;
 };
@@ -166,7 +167,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // instruction descriptor: bf16 x bf16 -> f32, A K-major, B K-major or MN-major
 __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_mn_major) {
   return umma_idesc_bf16(M, N) | (b_mn_major ? (1u << 16) : 0u);
@@ -294,6 +294,23 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     fence_barrier_init();
   }
   __syncthreads();
+  int words = 0;                                        // HALF_V: what the words of a softmax thread's tiles say, and what of it asks for more
+  auto lost_groups = [&](int kvh_, int pos, int lo) {   // groups of 32 values of a row that a NaN is among: a bit each
+    asm volatile("" : "+r"(kvh_));                      // (nothing of this is worked out before it is wanted)
+    int lost = 0;
+    const int* bt = p.block_table + (size_t)seq * p.bt_stride;
+#pragma unroll 1
+    for (int j = (p.keep_first > 0 ? 0 : max(lo, 0)) & ~31; j <= pos; j += 32) {
+      const int page = bt[j >> p.page_shift];
+      if (page < 0 || !value_lost(p.vexp[page * p.nkv + kvh_])) continue;
+      const uint32_t seen = bits_below(pos + 1 - j) & (~bits_below(lo - j) | bits_below(p.keep_first - j));
+      const uint32_t* bits = p.vlost + ((size_t)(page * p.nkv + kvh_) * (VD / 32) << (p.page_shift - 5)) + ((j & (p.page_size - 1)) >> 5);
+#pragma unroll 1
+      for (int x = 0; x < VD / 32; ++x)
+        if (bits[x << (p.page_shift - 5)] & seen) lost |= 1 << x;
+    }
+    return lost;
+  };
   const bool shared = MODE == HALF_V && p.parts > 1;    // (its CTAs meet at the item's end, whatever happens before)
   if (abort_flag && !shared) break;                     // a wait ran out in an earlier item: the kernel's output is void anyway
 
@@ -605,6 +622,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (page >= 0) word = p.vexp[page * p.nkv + kvh];
       }
       const int ve = value_exponent(word);
+      if (MODE == HALF_V) words |= word;
       const uint32_t s_addr = lane_addr + C::S_COL + (uint32_t)sa * PN;          // this step's S accumulator
       const uint32_t p_addr = BESIDE ? lane_addr + C::P_COL + (uint32_t)g * (PN / 2) : s_addr;
       if (!wait_on(&s_full[sa], (uint32_t)(BESIDE ? t : k / SB) & 1u, 24, t)) { ok = false; break; }
@@ -805,6 +823,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
       }
       tc_fence_before();
+      if (MODE == HALF_V && value_lost(words) && valid) {
+        // Groups whose scale is NaN are zeros in the scratch, for the rows that do not see them. (Looked for tile by tile, or in front of the
+        // stores, 512 rows over 2,012 keys took 2 us more.)
+        const int lost = lost_groups(kvh, pos, lo);
+#pragma unroll 1
+        for (int i = 0; i < VD / 8; ++i)
+          if (lost >> (i / 4) & 1) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+      }
+      __syncwarp();
       }
     }
   } else if (TMA) {
@@ -825,12 +852,22 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + C::O_COL + (uint32_t)(x / PM) * VD;
         const int owner = x / rows, at = x % rows;
         const bool there = n_t[x / PM] > 0;                // the range has keys of this row tile
+        int lost = 0;
+        if (value_lost(words)) {
+          const int at = tile[x / PM] * PM + x % PM, pos = at < rows_total ? kv_len - q_len + at / G : -1;
+          lost = lost_groups(kvh, pos, p.window > 0 ? pos - p.window + 1 : 0);
+        }
+        __syncwarp();
         const uint32_t to = map_to_rank(k_s + (uint32_t)(((int)blockIdx.z * (VD / 4) * rows + at) * 16), owner);
 #pragma unroll
         for (int c = 0; c < VD / 32; ++c) {
           uint32_t ov[32];
-          if (there) { tmem_ld32(from + 32 * c, ov); tmem_ld_wait(); }
-          else {
+          if (there) {
+            tmem_ld32(from + 32 * c, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = lost >> c & 1 ? 0x7fc00000u : ov[i];
+          } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) ov[i] = 0u;
           }
@@ -996,7 +1033,7 @@ int multiprocessors(int asked, int& sms) {
 // max_q_len: the longest portion in the batch (sizes the list of work items). Head sizes 64 and 128.
 // chunk > 0: a query sees only the keys of its own block of `chunk` positions (blocks counted from position 0);
 // sinks: float [nh] or null; gate: float logits [T, gate_ld] or null (see PfParams); keep_first, sigmoid: see PfParams.
-// softcap > 0: bounded scores. cross, long_from, vexp (values of 16 bits times powers of two, pages of a power of two from 128 keys): see PfParams. parts: CTAs
+// softcap > 0: bounded scores. cross, long_from, vexp and vlost (values of 16 bits times powers of two, pages of a power of two from 128 keys): see PfParams. parts: CTAs
 // that may share an item's keys (1, 2 or 4, with vexp; taken where every item's then have an SM each, else 1). sm_count: CTAs to launch at most (0: asked from the device).
 RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* kcache, const void* vcache,
                                        void* out, int out_stride, const int* cu_q, const int* kv_lens,
@@ -1004,7 +1041,7 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
                                        int num_pages, int nh, int nkv, int hd, int page_size, float scale, int window,
                                        int chunk, const float* sinks, const float* gate, int gate_ld,
                                        int keep_first, int sigmoid, float softcap, int long_from, float* cross, const int* vexp,
-                                       int parts, int* err, int sm_count, void* stream) {
+                                       const uint32_t* vlost, int parts, int* err, int sm_count, void* stream) {
   if (num_seqs <= 0 || max_q_len <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh % nkv || page_size <= 0 || num_pages <= 0 || keep_first < 0 || scale <= 0.f)
     return ERR_BAD_SIZE;
@@ -1012,10 +1049,10 @@ RLLM_API int rllm_attention_prefill_tc(const void* q, int q_stride, const void* 
       ((uintptr_t)kcache & 15) || ((uintptr_t)vcache & 15)) return ERR_BAD_ALIGN;
   if (long_from > 0 && !cross) return ERR_BAD_SIZE;
   if (cross && (softcap > 0.f || sigmoid || gate || ((uintptr_t)cross & 15))) return ERR_BAD_SIZE;
-  if (vexp && (cross || softcap > 0.f || sigmoid || sinks || page_size % 128)) return ERR_BAD_SIZE;
+  if (vexp && (cross || softcap > 0.f || sigmoid || sinks || page_size % 128 || !vlost)) return ERR_BAD_SIZE;
   if (parts != 1 && ((parts != 2 && parts != 4) || !vexp || gate || keep_first)) return ERR_BAD_SIZE;
   PfParams p = {};
-  p.long_from = long_from; p.cross = cross; p.vexp = vexp;
+  p.long_from = long_from; p.cross = cross; p.vexp = vexp; p.vlost = vlost;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.kc = (const bf16*)kcache; p.vc = (const bf16*)vcache;
   p.out = (bf16*)out; p.out_stride = out_stride; p.cu_q = cu_q; p.kv_lens = kv_lens;
   p.block_table = block_table; p.bt_stride = bt_stride; p.nh = nh; p.nkv = nkv; p.page_size = page_size;

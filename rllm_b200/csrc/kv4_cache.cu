@@ -102,10 +102,10 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {       // of b
   asm("max.u16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
   return a;
 }
-__device__ __forceinline__ uint32_t block_max2(uint32_t v) {
+__device__ __forceinline__ uint32_t block_max2(uint32_t v) {              // eight neighbouring lanes have the same
   __shared__ uint32_t red[THREADS / 32];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max2(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 4; o >>= 1) v = max2(v, __shfl_xor_sync(0xffffffffu, v, o));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
@@ -124,14 +124,14 @@ __device__ __forceinline__ uint32_t block_max2(uint32_t v) {
 // largest scale between 1 and 2; any other is bfloat16, its smallest scale (but not less than 2^-40 of its largest) between 1 and 2. The power
 // joins the scores where the weights are made: with the smallest scale no group of such a page, be it one a row's weight lies
 // wholly on, raises a row's maximum by more than it adds to the sum, so that the other pages' weights, in half precision, keep their bits.
-// A page of zeros adds nothing and so has the lowest power.
+// A page of zeros adds nothing and so has the lowest power. vlost: the places of groups whose scale is NaN.
 // UNITS: pieces (place, block of 64 dimensions) that a thread has at once, eight lanes together: 8 are a page of 128 places of 128 dimensions.
 // (With place after place, each behind its page's number, 2,012 keys of 8 heads of 128 took 11.5 us to read, now 7.6.)
 template <typename T, int UNITS>
 __global__ void __launch_bounds__(THREADS)
 kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ kv_lens,
                 const int* __restrict__ cu_q, int window, int num_seqs, int width, int out_page, T* __restrict__ k, T* __restrict__ v,
-                int table_width, int* __restrict__ table_out, int* __restrict__ cu_out, int* __restrict__ vexp) {
+                int table_width, int* __restrict__ table_out, int* __restrict__ cu_out, int* __restrict__ vexp, uint32_t* __restrict__ vlost) {
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x, s = blockIdx.y;
@@ -158,7 +158,7 @@ kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restr
   const bf16* sc = is_v ? c.vs : c.ks;
   T* dst = (is_v ? v : k) + (((size_t)s * width + i) * c.nkv + kvh) * out_page * c.hd;
   const int* bt = block_table + (size_t)s * bt_stride;
-  const bool half = is_v && vexp != nullptr;
+  const bool half = sizeof(T) == 2 && is_v && vexp != nullptr;
 #pragma unroll 1
   for (int u0 = threadIdx.x >> 3; u0 < units; u0 += UNITS * (THREADS / 8)) {
     // a thread's units (place, block of 64 dimensions), all of its page numbers on their way at once, then all of its words
@@ -187,20 +187,48 @@ kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restr
     bool wide = false;
     if (half) {                                          // (the page is one turn of the loop)
       // the largest scale's bits, and 0x7fff less the smallest's, as two maxima in a word
-      uint32_t ends = 0u;
+      auto both_ends = [&]() {
+        uint32_t hi = 0u, lo = 0u;
 #pragma unroll
-      for (int e = 0; e < UNITS; ++e)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint32_t b = (g ? two[e] >> 16 : two[e]) & 0x7fffu;
-          if (there[e] && b < 0x7f80u) ends = max2(ends, b | (0x7fffu - b) << 16);        // (a NaN is one in any format)
+        for (int e = 0; e < UNITS; ++e) {
+          const uint32_t m = two[e] & 0x7fff7fffu;
+          hi = max2(hi, m);
+          lo = max2(lo, there[e] ? 0x7fff7fffu - m : 0u);
         }
-      ends = block_max2(ends);
+        return block_max2(max(hi & 0xffffu, hi >> 16) | max(lo & 0xffffu, lo >> 16) << 16);
+      };
+      uint32_t ends = both_ends();
+      const bool lost = (ends & 0xffffu) >= 0x7f80u;
+      if (lost) {                                        // a scale of NaN: zeros (a number times zero), a bit, and the ends of the others
+        __shared__ uint32_t bits[4 * 8];                 // [group][32 places]: at most 256 pieces of two groups
+        const int words = out_page / 32, all = 2 * blocks * words;
+        if (threadIdx.x < 32) bits[threadIdx.x] = 0u;
+        __syncthreads();
+        uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+        for (int e = 0; e < UNITS; ++e) {
+          int r, b;
+          place(e, r, b);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t m = two[e] >> (16 * g) & 0x7fffu;
+            if (m >= 0x7f80u) {
+              two[e] &= g ? 0xffffu : 0xffff0000u;
+              if (w == g) atomicOr(&bits[(2 * b + g) * words + (r >> 5)], 1u << (r & 31));
+            } else {
+              hi = max(hi, m);
+              lo = max(lo, there[e] ? 0x7fffu - m : 0u);
+            }
+          }
+        }
+        ends = block_max2(hi | lo << 16);
+        if ((int)threadIdx.x < all) vlost[(((size_t)s * width + i) * c.nkv + kvh) * all + threadIdx.x] = bits[threadIdx.x];
+      }
       const int top = (int)(ends >> 7 & 0xffu) - 127, low = (int)((0x7fffu - (ends >> 16)) >> 7 & 0xffu) - 127;
       const bool zeros = (ends & 0xffffu) == 0u;
       wide = !zeros && (low < top - 6 || top < -VALUE_EXPONENTS || top > VALUE_EXPONENTS);
       const int e = min(max(zeros ? -VALUE_EXPONENTS : wide ? max(low, top - 40) : top, -VALUE_EXPONENTS), VALUE_EXPONENTS);
-      if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = value_word(e, wide);
+      if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = value_word(e, wide, lost);
       down = __int_as_float((127 - e) << 23);
     }
 #pragma unroll
@@ -256,13 +284,15 @@ RLLM_API int rllm_kv4_store(int dt, const void* k, const void* v, long long ldk,
 // The sequences' keys and values as numbers: k, v [num_seqs * width, nkv, out_page, hd] float or bf16 (rounded once). kv_lens int32
 // [num_seqs], none above width * out_page (with cu_q and a window: no more places seen than `width` pages hold); block_table int32 with an entry
 // for each of their pages. cu_q (int32 [num_seqs + 1]), window, table_out [num_seqs, table_width] and cu_out
-// [num_seqs + 1], and vexp [num_seqs * width, nkv] (bf16 only: v is then 16-bit numbers as `value_word` says; out_page * hd / 64 between 32 and 256) for attention of portions, or null.
+// [num_seqs + 1], and vexp [num_seqs * width, nkv] with vlost [num_seqs * width, nkv, hd / 32, out_page / 32] (bf16 only: v is then 16-bit
+// numbers as `value_word` says; pages of a multiple of 32 places, out_page * hd / 64 between 32 and 256) for attention of portions, or null.
 RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long long num_pages, const int* block_table, int bt_stride,
                            const int* kv_lens, const int* cu_q, int window, int num_seqs, int width, int out_page, void* k,
-                           void* v, int table_width, int* table_out, int* cu_out, int* vexp, int nkv, int page_size, int hd, void* stream) {
+                           void* v, int table_width, int* table_out, int* cu_out, int* vexp, uint32_t* vlost,
+                           int nkv, int page_size, int hd, void* stream) {
   if (num_seqs <= 0 || width <= 0) return 0;
   if (out_page <= 0 || 2 * nkv > 65535) return ERR_BAD_SIZE;
-  if (vexp != nullptr && (dt != DT_BF16 || (long long)out_page * (hd >> 6) > 8 * (THREADS / 8) || out_page * (hd >> 6) < THREADS / 8)) return ERR_BAD_SIZE;
+  if (vexp != nullptr && (dt != DT_BF16 || (long long)out_page * (hd >> 6) > 8 * (THREADS / 8) || out_page * (hd >> 6) < THREADS / 8 || out_page % 32 || !vlost)) return ERR_BAD_SIZE;
   Pages c;
   const int rc = make_pages(c, k4, ks, v4, vs, nkv, page_size, hd);
   if (rc) return rc;
@@ -275,7 +305,7 @@ RLLM_API int rllm_kv4_read(int dt, void* k4, void* ks, void* v4, void* vs, long 
   auto run = [&](auto type, auto kernel) {
     typedef decltype(type) T;
     return launch_ex(kernel, grid, dim3(THREADS), 0, s, 1, c, num_pages, shift, block_table, bt_stride, kv_lens, cu_q, window, num_seqs, width,
-                     out_page, (T*)k, (T*)v, table_width, table_out, cu_out, vexp);
+                     out_page, (T*)k, (T*)v, table_width, table_out, cu_out, vexp, vlost);
   };
   const long long each = ((long long)out_page * (hd >> 6) + THREADS / 8 - 1) / (THREADS / 8);
   if (dt == DT_F32) return each <= 1 ? run(float(), kv4_read_kernel<float, 1>) : each <= 4 ? run(float(), kv4_read_kernel<float, 4>) : run(float(), kv4_read_kernel<float, 8>);

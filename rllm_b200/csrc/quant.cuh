@@ -73,10 +73,14 @@ __device__ __forceinline__ float bf16_lo(uint32_t two) { return __uint_as_float(
 __device__ __forceinline__ float bf16_hi(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
 
 // How a page of values is held in the scratch of portions (kv4_read_kernel writes it, the portions' kernels read it): 16-bit numbers times
-// 2^e, half numbers or, `wide`, bfloat16. One word a page and kv head.
-__host__ __device__ __forceinline__ int value_word(int e, bool wide) { return 2 * e + (wide ? 1 : 0); }
-__host__ __device__ __forceinline__ int value_exponent(int word) { return word >> 1; }
+// 2^e, half numbers or, `wide`, bfloat16. One word a page and kv head. A group whose scale is NaN holds zeros there, so that the products of rows
+// that do not see it stay as they are; the word says that there are such (`lost`), and a bit a place in [page][kv head][group][page
+// size / 32] words which.
+__host__ __device__ __forceinline__ int value_word(int e, bool wide, bool lost) { return 4 * e + (lost ? 2 : 0) + (wide ? 1 : 0); }
+__host__ __device__ __forceinline__ int value_exponent(int word) { return word >> 2; }
+__host__ __device__ __forceinline__ bool value_lost(int word) { return word & 2; }
 __host__ __device__ __forceinline__ bool value_wide(int word) { return word & 1; }
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 constexpr int VALUE_EXPONENTS = 48;           // e lies between -48 and 48
 
 }  // namespace rllm

@@ -23,8 +23,8 @@ ops.register_signatures("quant", {
     "rllm_int8_linear": [c_int, c_int, c_int, _P, c_longlong, _P, _P, c_int, c_float, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int,
                          c_int, c_int, _P, c_int, _P],
     "rllm_kv4_store": [c_int, _P, _P, c_longlong, c_longlong, _P, _P, _P, _P, _P, c_longlong, c_int, c_int, c_int, c_int, _P],
-    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, c_int,
-                      c_int, c_int, _P],
+    "rllm_kv4_read": [c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P,
+                      c_int, c_int, c_int, _P],
     "rllm_kv4_decode": [_P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                         c_int, c_int, _P],
     "rllm_kv4_attention_simt": [c_int, _P, c_int, _P, _P, _P, _P, c_longlong, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
@@ -267,7 +267,7 @@ def kv4_read(tensors: dict, block_table: torch.Tensor, kv_lens: torch.Tensor, ma
     k, v = torch.empty((2, S, width, nkv, page_size, hd), dtype=dtype, device=k4.device).unbind(0)
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops._dt(k, "k"), k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr(),
-        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), 0, None, None, None, nkv, page_size, hd,
+        block_table.stride(0), kv_lens.data_ptr(), None, 0, S, width, page_size, k.data_ptr(), v.data_ptr(), 0, None, None, None, None, nkv, page_size, hd,
         ops._stream()), "kv4_read")
     return k, v
 
@@ -421,7 +421,9 @@ def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> 
         return False
     k, v = room.unbind(0)
     v = v.view(torch.float16)
-    table, vexp, cu = q.new_empty(S * (entries + width * nkv) + S + 1, dtype=torch.int32).split((S * entries, S * width * nkv, S + 1))
+    heads = S * width * nkv
+    lost = heads * (hd // 32) * (READ_PAGE // 32)
+    table, vexp, vlost, cu = q.new_empty(S * entries + heads + lost + S + 1, dtype=torch.int32).split((S * entries, heads, lost, S + 1))
     whole = S == ctx.num_seqs                      # (a view costs the host as much as half a launch)
     kv_lens = ctx.kv_lens if whole else ctx.kv_lens[s0:s1]
     if not whole:
@@ -429,14 +431,14 @@ def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> 
     ops._check(ops._fn("quant", "rllm_kv4_read")(
         ops.DT_BF16, k4.data_ptr(), ks.data_ptr(), v4.data_ptr(), vs.data_ptr(), pages, block_table.data_ptr() + 4 * s0 * block_table.stride(0),
         block_table.stride(0), kv_lens.data_ptr(), ctx.cu_q.data_ptr() + 4 * s0, int(window or 0), S, width, READ_PAGE, k.data_ptr(), v.data_ptr(), entries, table.data_ptr(),
-        cu.data_ptr(), vexp.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
+        cu.data_ptr(), vexp.data_ptr(), vlost.data_ptr(), nkv, page_size, hd, ops._stream()), "kv4_read")
     a = (q, k, v, cu, kv_lens, table.view(S, entries))
     if longest * (nh // nkv) >= 128 and most >= sm100.TC_ATTENTION_MIN_KEYS and sm100.prefill_tc_supported(q, k):
         items = -(-longest * (nh // nkv) // 256) * nkv * S
         parts = portion_parts(items, min(most, window + longest) if window else most, hd, sm100.init(q.device).sm_count)
-        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out, vexp=vexp, parts=parts)
+        sm100.attention_prefill_tc(*a, longest, nh, scale, window, out=out, vexp=vexp, vlost=vlost, parts=parts)
     else:
-        sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out, vexp=vexp)
+        sm100.attention_fa(*a, T, longest, most, nh, scale, window, out=out, vexp=vexp, vlost=vlost)
     return True
 
 

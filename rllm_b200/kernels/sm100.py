@@ -30,10 +30,10 @@ ops.register_signatures("sm100", {
     "rllm_wait_probe": [_P, c_longlong, c_int, _P],
     "rllm_attention_fa": [_P, c_int, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                           c_int, c_int, c_float, c_int, c_int, _P, _P, _P],
-    "rllm_attention_fa_v16": [_P, c_int, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
+    "rllm_attention_fa_v16": [_P, c_int, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                               c_int, c_int, c_float, c_int, c_int, _P, _P, _P],
     "rllm_attention_prefill_tc": [_P, c_int, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
-                                  c_int, c_int, c_float, c_int, c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, _P, c_int, _P, c_int, _P],
+                                  c_int, c_int, c_float, c_int, c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, _P, _P, c_int, _P, c_int, _P],
     "rllm_attention_prefill_dense": [_P, c_int, c_int, _P, c_longlong, c_int, _P, _P, c_longlong, c_int, c_int, _P, c_int, c_longlong, _P,
                                      c_int, _P, _P, c_int, c_int, c_int, c_float, c_int, _P, c_int, c_int, c_int, _P, c_int, _P],
     "rllm_attention_decode_per_sm": [c_int, c_int, c_int],
@@ -377,12 +377,13 @@ def attention_splits(num_seqs: int, nkv: int, max_rows: int, max_kv_len: int, sm
 
 
 def attention_fa(q, kcache, vcache, cu_q, kv_lens, block_table, num_tokens, max_q_len, max_kv_len, nh,
-                 scale, window, splits=None, out=None, vexp=None):
+                 scale, window, splits=None, out=None, vexp=None, vlost=None):
     """Tiled tensor-core attention over the paged cache (bf16, head size 64 or 128). `vexp` int32 [pages, kv heads]: the values
-    are half numbers times 2^(vexp >> 1), or with vexp odd bfloat16 ones (float16 vcache, pages of a multiple of 64 keys)."""
+    are half numbers times 2^(vexp >> 2), or with vexp odd bfloat16 ones (float16 vcache, pages of a multiple of 64 keys); with bit 1 of vexp set, `vlost` int32
+    [pages, kv heads, hd / 32, page size / 32] has a bit for each place whose group of values is NaN."""
     st = init(q.device)
     _, nkv, page_size, hd = kcache.shape
-    _check_vexp(vexp, kcache, vcache, 64)
+    _check_vexp(vexp, vlost, kcache, vcache, 64)
     S = kv_lens.numel()
     G = nh // nkv
     if splits is None:
@@ -395,7 +396,7 @@ def attention_fa(q, kcache, vcache, cu_q, kv_lens, block_table, num_tokens, max_
         part_o = torch.empty(need * hd, dtype=torch.float32, device=q.device)
         part_ml = torch.empty(need * 2, dtype=torch.float32, device=q.device)
     rc = ops._fn("sm100", "rllm_attention_fa" if vexp is None else "rllm_attention_fa_v16")(
-        q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), *(() if vexp is None else (vexp.data_ptr(),)),
+        q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), *(() if vexp is None else (vexp.data_ptr(), vlost.data_ptr())),
         out.data_ptr(), out.stride(0),
         cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), S, num_tokens,
         max_q_len, nh, nkv, hd, page_size, float(scale), int(window or 0), splits,
@@ -405,12 +406,16 @@ def attention_fa(q, kcache, vcache, cu_q, kv_lens, block_table, num_tokens, max_
     return out
 
 
-def _check_vexp(vexp, kcache, vcache, keys):
+def _check_vexp(vexp, vlost, kcache, vcache, keys):
     if (vexp is None) != (vcache.dtype == torch.bfloat16):
         raise ops.KernelError("attention: values are bfloat16, or float16 with their powers of two")
-    if vexp is not None and (vcache.dtype != torch.float16 or vexp.dtype != torch.int32 or not vexp.is_contiguous() or not vexp.is_cuda
-                             or vexp.numel() != kcache.shape[0] * kcache.shape[1] or kcache.shape[2] % keys):
-        raise ops.KernelError(f"attention: float16 values need an int32 [pages, kv heads] of powers of two and pages of a multiple of {keys}")
+    if vexp is None:
+        return
+    pages, nkv, page_size, hd = kcache.shape
+    whole = lambda t, n: t is not None and t.dtype == torch.int32 and t.is_contiguous() and t.is_cuda and t.numel() == n
+    if vcache.dtype != torch.float16 or page_size % keys or not whole(vexp, pages * nkv) or not whole(vlost, pages * nkv * (hd // 32) * (page_size // 32)):
+        raise ops.KernelError(f"attention: float16 values need an int32 [pages, kv heads] of powers of two, an int32 [pages, kv heads, groups of 32, words "
+                              f"of 32 places] of the places of NaNs, and pages of a multiple of {keys}")
 
 
 TC_ATTENTION_MIN_KEYS = int(os.environ.get("RLLM_B200_TC_ATTENTION_MIN_KEYS", "512"))
@@ -435,7 +440,7 @@ def _extras(chunk, sinks, gate, nh, rows):
 
 def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_len, nh, scale, window, out=None,
                          chunk=None, sinks=None, gate=None, keep_first=0, sigmoid=False, softcap=None, long_from=0,
-                         cross=None, vexp=None, parts=1):
+                         cross=None, vexp=None, vlost=None, parts=1):
     """Prefill attention on the tcgen05 tensor cores (bf16, head size 64 or 128): tiles of 128 rows x
     128 (64) keys, both products with their accumulators in TMEM. `chunk`: a query sees only the keys of its
     own block of that many positions; `sinks` float [nh]: exp(sink) joins a row's denominator; `gate` float
@@ -444,11 +449,11 @@ def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_le
     bounded, softcap * tanh(score / softcap). `cross` float32 [T, nh, nkv, hd]: every query head meets every kv head's
     values and the float outputs go there (pages of a power of two from 8 keys on; no gate, bound or sigmoid); sequences with
     fewer than `long_from` rows are then left out. `vexp` int32 [pages, kv heads]: the values are half numbers times
-    2^(vexp >> 1), or with vexp odd bfloat16 ones (float16 vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid); `parts`: that many CTAs (1, 2 or 4) may then share a
+    2^(vexp >> 2), or with vexp odd bfloat16 ones, `vlost` as for `attention_fa` (float16 vcache, pages of a power of two from 128 keys on; no sink, bound or sigmoid); `parts`: that many CTAs (1, 2 or 4) may then share a
     work item's keys, where all of them find an SM."""
     if not prefill_tc_supported(q, kcache):
         raise ops.KernelError("attention_prefill_tc: bfloat16, head size 64 or 128, rows 16-byte aligned")
-    _check_vexp(vexp, kcache, vcache, 128)
+    _check_vexp(vexp, vlost, kcache, vcache, 128)
     st = init(q.device)
     _, nkv, page_size, hd = kcache.shape
     if cross is not None:
@@ -462,7 +467,7 @@ def attention_prefill_tc(q, kcache, vcache, cu_q, kv_lens, block_table, max_q_le
         cu_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.numel(),
         max_q_len, kcache.shape[0], nh, nkv, hd, page_size, float(scale), int(window or 0),
         *_extras(chunk, sinks, gate, nh, q.shape[0]), int(keep_first or 0), int(bool(sigmoid)), float(softcap or 0.0), int(long_from),
-        None if cross is None else cross.data_ptr(), None if vexp is None else vexp.data_ptr(), int(parts), st.err.data_ptr(), st.sm_count, ops._stream())
+        None if cross is None else cross.data_ptr(), None if vexp is None else vexp.data_ptr(), None if vexp is None else vlost.data_ptr(), int(parts), st.err.data_ptr(), st.sm_count, ops._stream())
     ops._check(rc, "attention_prefill_tc")
     return out if cross is None else cross
 

@@ -200,3 +200,36 @@ def test_a_visible_place_on_a_page_that_is_not_held_reads_as_zeros(hd, q_lens, d
             row += n
             tol = bound(dt, want, mag, big, hd, lens[s], dt == torch.bfloat16 and n > 1)
             assert ((got - want).abs() <= tol).all(), (s, float(((got - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("window", [None, 150])
+@pytest.mark.parametrize("hd,dtype,q_lens", [(64, "bfloat16", [200, 60]), (128, "bfloat16", [200, 60]), (64, "float32", [200, 60]), (64, "bfloat16", [1, 1]),
+                                             (128, "bfloat16", [1, 1]), (192, "bfloat16", [60, 1])])
+@pytest.mark.parametrize("parts", [0, 1, 2, 4])
+def test_values_that_are_not_finite_are_seen_where_they_are_visible_only(hd, dtype, q_lens, window, parts, monkeypatch):
+    """A group of a value with a scale of NaN: the group's dimensions are NaN in rows that see the place, and in no other row or dimension."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: max(parts, 1))
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if parts else 1 << 30)
+    lens, nh, nkv = [700, 260], 4, 2
+    dt = getattr(torch, dtype)
+    t, table, held = make("places", lens, nkv, hd, seed=11)
+    gone = [[(3, 0, 1), (540, 1, 0), (600, 0, hd // 32 - 1), (601, 0, 0), (699, 1, 1)], [(100, 1, 1), (259, 0, 0)]]
+    for s, places in enumerate(gone):
+        for j, head, grp in places:
+            t["vs"][int(table[s, j // 16]), head, j % 16, grp] = math.nan
+            held[s][1][j, head, 32 * grp: 32 * grp + 32] = 0.0
+    q = rnd(sum(q_lens), nh * hd, seed=6, dtype=dt, scale=1.5).to(DEV)
+    y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, hd ** -0.5, window)
+    row = 0
+    for s, n in enumerate(q_lens):
+        want, mag, big = Q.attention(q[row: row + n].cpu().view(n, nh, hd), held[s][0], held[s][1], hd ** -0.5, window)
+        got = y[row: row + n].cpu().double().view(n, nh, hd)
+        row += n
+        nan = torch.zeros(n, nh, hd, dtype=torch.bool)
+        for j, head, grp in gone[s]:
+            pos = torch.arange(lens[s] - n, lens[s])
+            sees = (j <= pos) & (j > pos - window if window else j >= 0)
+            nan[:, head * 2: head * 2 + 2, 32 * grp: 32 * grp + 32] |= sees[:, None, None]
+        assert torch.equal(torch.isnan(got), nan), s
+        tol = bound(dt, want, mag, big, hd, lens[s], dt == torch.bfloat16 and n > 1)
+        assert ((got - want).abs() <= tol)[~nan].all(), (s, float(((got - want).abs() / tol)[~nan].max()))
