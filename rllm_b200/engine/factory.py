@@ -47,7 +47,7 @@ def set_kv_quant(model, kv_quant: str) -> list:
     if kv_quant not in KV_QUANT:
         raise ValueError(f"kv_quant must be one of {KV_QUANT}, got {kv_quant!r}")
     able = [p for p in model.parts() if hasattr(p, "use_kv4")]
-    if not _may_change(model, "kv_quant", kv_quant, "int4" if any(p.kv4 for p in able) else "none"):
+    if not _may_change(model, "kv_quant", kv_quant, "int4" if any(getattr(p, "kv4", False) for p in able) else "none"):
         return []
     specs = [s for s in model.cache_specs() if s is not None and cache_kind_of(s).paged]
     if not able:

@@ -62,20 +62,22 @@ class MetaLayout:
         return buf[o: o + n]
 
 
+# model -> the engines that run it (beside the models, whose copies have none)
+_engines: weakref.WeakKeyDictionary = weakref.WeakKeyDictionary()
+
+
 def any_engine(model) -> bool:
     """Is there an engine that runs this model?"""
-    if not getattr(model, "engines", None):
+    if not _engines.get(model):
         return False
     gc.collect()                      # (an engine and its captured steps refer to one another)
-    return bool(model.engines)
+    return bool(_engines.get(model))
 
 
 class Engine:
     def __init__(self, model, backend, cache: CacheManager, use_graphs: bool | None = None):
         self.model, self.backend, self.cache = model, backend, cache
-        if not hasattr(model, "engines"):
-            model.engines = weakref.WeakSet()
-        model.engines.add(self)
+        _engines.setdefault(model, weakref.WeakSet()).add(self)
         self.device = backend.device
         self.vocab = model.vocab_size
         # device words: [0] a kernel's bounded wait ran out, [1] a token id outside the table,

@@ -1,4 +1,5 @@
 """Quantising a model changes its parts, which every engine of the model runs: what is refused, and that a refused model is as it was. No GPU."""
+import copy
 import gc
 import weakref
 
@@ -7,7 +8,7 @@ import torch
 
 import tiny
 from rllm_b200.config import config_from_dict
-from rllm_b200.engine import factory
+from rllm_b200.engine import factory, step
 from rllm_b200.engine.factory import set_kv_quant, set_weight_quant
 from rllm_b200.kernels import quant
 from rllm_b200.parts import KV4CacheSpec, Part
@@ -50,10 +51,10 @@ def kinds(m):
 
 def test_a_model_that_an_engine_runs_is_not_changed(on_cpu):
     m = bound()
-    m.engines = weakref.WeakSet()
     e = AnEngine()
     e.me = e                                               # (as an engine and its captured steps do)
-    m.engines.add(e)
+    step._engines[m] = weakref.WeakSet([e])
+    twin = copy.deepcopy(m)                                # parts of its own, which no engine runs
     before = kinds(m), [getattr(p, n) for p in m.parts() for n in p.int8_params]
     with pytest.raises(ValueError, match="another engine"):
         set_kv_quant(m, "int4")
@@ -63,15 +64,17 @@ def test_a_model_that_an_engine_runs_is_not_changed(on_cpu):
     set_weight_quant(m, "none")
     after = kinds(m), [getattr(p, n) for p in m.parts() for n in p.int8_params]
     assert before[0] == after[0] and all(a is b for a, b in zip(before[1], after[1])) and not on_cpu
+    set_kv_quant(twin, "int4")
+    assert all(k is KV4CacheSpec for k in kinds(twin)) and kinds(m) == before[0]
     del e                                                  # nothing runs it any more
     set_kv_quant(m, "int4")
     set_weight_quant(m, "int8")
     assert all(k is KV4CacheSpec for k in kinds(m)) and on_cpu
     n = len(on_cpu)
-    m.engines.add(e := AnEngine())
+    step._engines[m].add(e := AnEngine())
     set_kv_quant(m, "int4")                                # a second engine of the same kind
     set_weight_quant(m, "int8")
-    assert len(on_cpu) == n and e in m.engines
+    assert len(on_cpu) == n and e in step._engines[m]
 
 
 def test_a_quantised_model_does_not_turn_back_in_silence(on_cpu):
@@ -115,7 +118,7 @@ def test_an_engine_is_known_while_it_lives():
     m = NoModel()
     assert not any_engine(m)
     a, b = (Engine(m, NoBackend(), None, use_graphs=False) for _ in range(2))
-    assert any_engine(m) and len(m.engines) == 2
+    assert any_engine(m) and len(step._engines[m]) == 2
     del a, b
     gc.collect()
     assert not any_engine(m)
