@@ -232,7 +232,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __shared__ __align__(8) uint64_t kv_full[KVS], kv_empty[KVS], s_full[SB], s_free[SB], p_full[RT], pv_full[RT], q_full;
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
-  __shared__ int tile_wide[RT];        // HALF_V: is P of the row tile's step bfloat16? Written in front of `p_full`, when the PV before is complete
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* smem = (uint8_t*)(((uintptr_t)pf_smem_raw + 1023) & ~(uintptr_t)1023);
@@ -404,12 +403,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   auto issue_pv = [&](int k, bool& ok) {                // PV of step k, added to the row tile's output (one thread)
     int g, t;
     step(k, g, t);
+    // HALF_V: the tile's type, on its way while P is waited for
+    int word = 0;
+    if (MODE == HALF_V) {
+      const int page = p.block_table[(size_t)seq * p.bt_stride + (tile_first(t) >> p.page_shift)];
+      if (page >= 0) word = p.vexp[page * p.nkv + kvh];
+    }
     // P of this step is written (and the row tile's PV before is complete: its threads waited for it)
     if (!mbar_wait(&p_full[g], (uint32_t)t & 1u, &abort_flag)) {
       abort_flag = 1; record_failure(p.err, 23, t); ok = false; return;
     }
     tc_fence_after();
-    const uint32_t id_pv = MODE == HALF_V && !*(volatile int*)&tile_wide[g] ? id_half : id_bf16;
+    const uint32_t id_pv = MODE == HALF_V && !value_wide(word) ? id_half : id_bf16;
     const uint64_t dv = dv0 + (uint64_t)((t % NST) * (C::V_BYTES >> 4));
     const uint32_t acc = tmem_base + C::O_COL + (uint32_t)g * VD, pa = tmem_base + (BESIDE ? C::P_COL + (uint32_t)g * (PN / 2) : C::S_COL + (uint32_t)(k % SB) * PN);
 #pragma unroll
@@ -761,10 +766,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if (!BESIDE && !moves && !pv_before()) { ok = false; break; }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (MODE == HALF_V) *(volatile int*)&tile_wide[g] = value_wide(word);
-        mbar_arrive(&p_full[g]);
-      }
+      if (lane == 0) mbar_arrive(&p_full[g]);
       float ls[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(lq[i], ls[2 * i], ls[2 * i + 1]);
