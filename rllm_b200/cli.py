@@ -28,9 +28,11 @@ def _model_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--tp", type=int, default=0, help="Tensor parallelism; this engine runs on one GPU (0 or 1).")
     p.add_argument("--stream-experts", action="store_true", help="(not built) MoE expert streaming")
     p.add_argument("--image", default=None, help="(not built) image input")
-    p.add_argument("--kv-quant", default="none", help='KV cache quantization: "none" or "int4" (4 bits, a scale per 32 numbers).')
+    p.add_argument("--kv-quant", default="none", help='KV cache quantization: "none" or "int4" (4 bits, a scale per 32 numbers): 9/32 of the cache; '
+                   'faster from some sequences of some thousand tokens on, slower for one.')
     p.add_argument("--weight-quant", default="none", choices=["none", "int8"],
-                   help="Layers' matrices in 8 bits with a scale per output channel, quantised at load.")
+                   help="Layers' matrices in 8 bits with a scale per output channel, quantised at load: half of their memory; prompts and wide layers are "
+                   "faster, one to eight sequences on layers of 2,048 slower.")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     p.add_argument("--seed", type=int, default=None, help="Seed of the sampling random numbers.")
     p.add_argument("--page-size", type=int, default=16, help="Positions per cache page (reference: 16).")

@@ -45,9 +45,9 @@
 // the window's, as one list. With `sigmoid` a visible key's weight is sigmoid(score + bias[head]) in place of the
 // softmax's: no maximum, no rescaling, no denominator.
 //
-// Values in half precision (HALF_V, the numbers of a cache held in 4 bits) may be shared: the CTAs of a cluster each take a range of a work item's
-// keys where the items leave SMs idle, and their sums meet in shared memory at the end. 64 rows over 4,000 keys (32 / 8 heads of
-// 64) 67 -> 32 us with four, 512 over 8,000 122 -> 75 with two.
+// Over the numbers of a cache held in 4 bits (HALF_V) a work item may be shared: the CTAs of a cluster each take a range of its keys
+// where the items leave SMs idle, and their sums meet in shared memory at the end. 64 rows over 4,000 keys (32 / 8 heads of
+// 64) 65 -> 30 us with four, 512 over 8,000 116 -> 71 with two.
 //
 // Formulas: src/gpu/cuda/shaders/attention.cu:573-618 and :328-388 of the reference (scale,
 // softmax with the maximum subtracted, weighted V, head h -> kv head h / G, window); unlike the
@@ -216,8 +216,8 @@ __device__ __forceinline__ void softcap_poly2(uint32_t& x0, uint32_t& x1, float 
 // MODE PLAIN: pages. CROSS: pages, every head over every kv head's values, float outputs (PfParams). DENSE: keys and values in
 // rows, by tensor copies of whole tiles.
 // HALF_V: pages whose values are half numbers, or bfloat16 where half's range is too small, times a power of two a page (PfParams); the weights
-// that meet them are of the same type. A value's power of two joins its key's score as far as the running maximum and the weight are concerned, so that the weights
-// are those of the sum itself and stay within half's range; the denominator's part is given it back.
+// that meet them are of the same type. A value's power of two joins its key's score as far as the running maximum and the weight are
+// concerned, so that the weights are those of the sum itself and stay within half's range; the denominator's part is given it back.
 enum : int { PLAIN = 0, CROSS = 1, DENSE_ROWS = 2, HALF_V = 3 };
 template <int KD, int VD, bool TMA, bool CAP, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)

@@ -10,8 +10,8 @@
 //     lane multiplies by one group's scale; the two groups' sums meet by one shuffle.
 //   * Fragments hold codes, exact half numbers: nibbles 0 and 1 of a half word are the last four bits of 1024 + n and four higher ones of 64 + n
 //     by one AND-OR each for two numbers, nibbles 2 and 3 the same after a shift by 8; less 1032 and 72 they are the codes. (In bfloat16, with 7 bits
-//     behind the first, three of the four nibbles would want a shift; the pipe of shifts, ANDs and permutations is what bounds this
-//     kernel: with those and with pairs put together from two words, 64 sequences of 4,096 keys, 8 x 128, took 115 us.) Queries are half numbers
+//     behind the first, three of the four nibbles would want a shift; shifts, ANDs and permutations share the kernel's busiest pipe: with
+//     those and with pairs put together from two words, 64 sequences of 4,096 keys, 8 x 128, took 115 us, now 85.) Queries are half numbers
 //     times a power of two a row, which is exact down to 2^-14 of the row's largest. A group's sum is as exact as float; it is multiplied
 //     by the group's scale as a float number. No dequantised key exists.
 //   * O^T = V^T P^T, dimensions within a group on the rows; the contraction is over (key, group) pairs, so that a register is again a word's
@@ -24,8 +24,8 @@
 //     shared memory meet a bank twice.
 //   * The running maximum moves only when a score passes it by 8 (in the log2 domain): weights reach 256 then, which is as good as 1, and
 //     the lanes' maxima meet once in a while instead of in every tile.
-// 64 sequences of 2,048 keys, 32 / 8 heads of 128: 50 us, 3.0 TB/s, the pipe of shifts, ANDs and permutations busy 46 %, an instruction issued in
-// 56 % of the cycles. One sequence of 300 keys 4.0 us, eight of 4,096 (32 / 8 heads of 64) 12.
+// 64 sequences of 2,048 keys, 32 / 8 heads of 128: 52 us, 2.9 TB/s, an instruction issued in 60 % of the cycles, the pipe of shifts, ANDs and permutations
+// busy 47 %: nothing is full, 14 of 64 warps wait for their own chains. One sequence of 300 keys 4.1 us, eight of 4,096 (32 / 8 heads of 64) 12.
 //
 // On the CUDA cores, for any mix of prompt portions and single tokens, both run types and head sizes of 64, 128, 192 and 256: one
 // warp per (query token, query head), keys 32 at a time in position order with a running maximum and sum, all arithmetic in
@@ -619,7 +619,7 @@ int launch_decode(const Kv4Params& p, int sm_count, cudaStream_t s) {
   const dim3 grid(p.nkv * ((G + 4 * NQ - 1) / (4 * NQ)), p.rows, p.splits);
   if (grid.y > 65535) return ERR_TOO_LARGE;
   // While every CTA can have an SM of its own it takes one: the CTAs of a cluster are otherwise put on SMs in pairs (8 sequences of 4,096
-  // keys, 8 kv heads of 64, 2 ranges: 16.1 us, alone 12.4). Not so clusters of 16, for which too few GPCs have 16 SMs (41 us for one
+  // keys, 8 kv heads of 64, 2 ranges: 16.1 us, alone 12.8; the 4 ranges that the rule takes, two CTAs an SM, 11.9). Not so clusters of 16, for which too few GPCs have 16 SMs (41 us for one
   // sequence of 60,000 keys of 128, 57 alone).
   const long long ctas = (long long)grid.x * grid.y * grid.z;
   return launch_ex(kv4_decode_kernel<HD, NQ>, grid, dim3(C::THREADS), ctas <= sm_count && p.splits <= 8 ? C::ALONE : C::RING, s, p.splits, p);

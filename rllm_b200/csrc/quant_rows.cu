@@ -3,9 +3,10 @@
 // step and, once at load, the rows of a weight.
 //
 // The row has to be read before its scale is known, so a CTA holds it: 256 threads with up to VPT groups of 8 numbers in registers
-// each (16,384 numbers with eight groups), longer rows are read twice, the second time out of the caches. The bound is the
+// each (16,384 numbers with eight groups), longer rows are read twice, the second time out of the caches. What it has to do is the
 // read of x and the write of the codes; a quotient is a multiplication by 1 / s except next to a border (`codes8`), since
-// a division for every number took as long as the memory.
+// a division for every number took as long as the memory. 2,048 bfloat16 rows of 8,192 take 13 us (50 MB, floor 7.7): an
+// instruction is issued in 63 % of the cycles, the integer pipe busy 57 %.
 // Codes lie in rows of a multiple of 16 bytes (`ldc`), the numbers behind K are zeros: the products' copies are whole pieces.
 #include "quant.cuh"
 

@@ -382,8 +382,8 @@ def _runs(ctx) -> list:
 def portion_parts(items: int, keys: int, hd: int, sm_count: int) -> int:
     """CTAs that share a work item's keys (256 rows of a kv head, 1, 2 or 4 CTAs) where the items leave SMs idle: by the time in us, 0.0139 a
     key at heads of 64 and 0.0185 at 128, and 4 + 1/16 a CTA for where the ranges meet, 4 more for many clusters of 4. One | two | four, us with the
-    keys' reading: 512 rows over 2,012 keys (32 / 8 heads of 128) 54.5 | 50.7; 512 over 600 25.4 | 28.5; 128 over 4,000 92 | 63 | 48; 64 over
-    4,000 (heads of 64) 67 | 43 | 32; 512 over 8,000 122 | 74."""
+    keys' reading: 512 rows over 2,012 keys (32 / 8 heads of 128) 51 | 42; 512 over 600 24.6 | 27.6; 128 over 4,000 84 | 57 | 41; 64 over
+    4,000 (heads of 64) 65 | 42 | 30; 512 over 8,000 116 | 71."""
     best, cost = 1, keys * (0.0139 if hd == 64 else 0.0185)
     for z in (2, 4):
         n = items * z
@@ -396,10 +396,11 @@ def portion_parts(items: int, keys: int, hd: int, sm_count: int) -> int:
 def _portions(q, kv, ctx, block_table, nh, scale, window, run, out, scratch) -> bool:
     """Attention of a run of portions (bfloat16, heads of 64 or 128): the keys and values that they see are read into scratch, in pages of
     READ_PAGE places, and the kernels of the cache of whole numbers attend over those. A portion's rows share the keys, so the
-    numbers are made once instead of in every row tile. Keys are rounded to bfloat16, what the queries' product takes; values (12
-    significant bits) and the weights that meet them to half precision with a power of two a page: with both in bfloat16 the result was
-    0.0026 of its norm from the exact one, with half precision 0.0018, of which 0.0017 is the output's own rounding. False where the
-    memory left does not hold the scratch."""
+    numbers are made once instead of in every row tile. Keys are rounded to bfloat16, what the queries' product takes (single tokens
+    multiply the codes, which is exact); values (12 significant bits) and the weights that meet them to half precision with a power of two a
+    page, or to bfloat16 on a page whose scales are too far apart for that (kv4_cache.cu): with both in bfloat16 the result was 0.0026 of
+    its norm from the exact one, with half precision 0.0018, of which 0.0017 is the output's own rounding. False where the memory left does
+    not hold the scratch."""
     s0, s1, r0, r1, _, longest, most = run
     k4, ks, v4, vs, pages, nkv, page_size, hd = kv
     S, T, entries = s1 - s0, r1 - r0, -(-most // READ_PAGE)
