@@ -125,7 +125,8 @@ __device__ __forceinline__ uint32_t block_max2(uint32_t v) {              // eig
 // largest scale between 1 and 2; any other is bfloat16, its smallest scale (but not less than 2^-40 of its largest) between 1 and 2. The power
 // joins the scores where the weights are made: with the smallest scale no group of such a page, be it one a row's weight lies
 // wholly on, raises a row's maximum by more than it adds to the sum, so that the other pages' weights, in half precision, keep their bits.
-// A page of zeros adds nothing and so has the lowest power. vlost: the places of groups whose scale is NaN.
+// A page of zeros adds nothing and so has the lowest power; not a lower one still, since its weights, times that power beside
+// others', have to stay float numbers for the denominator. vlost: the places of groups whose scale is NaN.
 // UNITS: pieces (place, block of 64 dimensions) that a thread has at once, eight lanes together: 8 are a page of 128 places of 128 dimensions.
 // (With place after place, each behind its page's number, 2,012 keys of 8 heads of 128 took 11.5 us to read, now 7.6.)
 template <typename T, int UNITS>
@@ -228,7 +229,7 @@ kv4_read_kernel(Pages c, long long num_pages, int page_shift, const int* __restr
       const int top = (int)(ends >> 7 & 0xffu) - 127, low = (int)((0x7fffu - (ends >> 16)) >> 7 & 0xffu) - 127;
       const bool zeros = (ends & 0xffffu) == 0u;
       wide = !zeros && (low < top - 6 || top < -VALUE_EXPONENTS || top > VALUE_EXPONENTS);
-      const int e = min(max(zeros ? -VALUE_EXPONENTS : wide ? max(low, top - 40) : top, -VALUE_EXPONENTS), VALUE_EXPONENTS);
+      const int e = zeros ? ZEROS_EXPONENT : min(max(wide ? max(low, top - 40) : top, -VALUE_EXPONENTS), VALUE_EXPONENTS);
       if (threadIdx.x == 0) vexp[((size_t)s * width + i) * c.nkv + kvh] = value_word(e, wide, lost);
       down = __int_as_float((127 - e) << 23);
     }

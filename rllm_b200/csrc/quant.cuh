@@ -81,6 +81,7 @@ __host__ __device__ __forceinline__ int value_exponent(int word) { return word >
 __host__ __device__ __forceinline__ bool value_lost(int word) { return word & 2; }
 __host__ __device__ __forceinline__ bool value_wide(int word) { return word & 1; }
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-constexpr int VALUE_EXPONENTS = 48;           // e lies between -48 and 48
+constexpr int VALUE_EXPONENTS = 48;           // e lies between -48 and 48,
+constexpr int ZEROS_EXPONENT = -70;           // that of a page of zeros below
 
 }  // namespace rllm

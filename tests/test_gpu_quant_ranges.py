@@ -233,3 +233,16 @@ def test_values_that_are_not_finite_are_seen_where_they_are_visible_only(hd, dty
         assert torch.equal(torch.isnan(got), nan), s
         tol = bound(dt, want, mag, big, hd, lens[s], dt == torch.bfloat16 and n > 1)
         assert ((got - want).abs() <= tol)[~nan].all(), (s, float(((got - want).abs() / tol)[~nan].max()))
+
+
+@pytest.mark.parametrize("parts", [0, 1, 2])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_keys_of_zeros_that_outweigh_small_values(hd, parts, monkeypatch):
+    """Nearly all of the weight on keys in pages of zeros, values of 2^-30 elsewhere: what is left of the sum is theirs."""
+    monkeypatch.setattr(quant(), "portion_parts", lambda *a: max(parts, 1))
+    monkeypatch.setattr(quant().sm100, "TC_ATTENTION_MIN_KEYS", 1 if parts else 1 << 30)
+    lens, q_lens, nh, nkv = [700], [64], 4, 1
+    t, table, held = make("zero_pages", lens, nkv, hd, seed=7 * hd + parts, sink=(0, 1, 2))
+    q = (0.5 + 0.1 * rnd(64, nh * hd, seed=6)).bfloat16().to(DEV)
+    y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, 20 / hd, None)
+    check(y, q, held, lens, q_lens, nh, hd, 20 / hd, None, True)
