@@ -246,3 +246,21 @@ def test_keys_of_zeros_that_outweigh_small_values(hd, parts, monkeypatch):
     q = (0.5 + 0.1 * rnd(64, nh * hd, seed=6)).bfloat16().to(DEV)
     y, _ = run_attention(q, t, table, lens, q_lens, nh, nkv, hd, 16, 20 / hd, None)
     check(y, q, held, lens, q_lens, nh, hd, 20 / hd, None, True)
+
+
+def test_values_of_16_bits_are_refused_without_their_words():
+    from rllm_b200.kernels import ops, sm100
+    z = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=DEV)
+    k, v, q = z(2, 1, 128, 64, dt=torch.bfloat16), z(2, 1, 128, 64, dt=torch.float16), z(4, 64, dt=torch.bfloat16)
+    cu, lens, table = torch.tensor([0, 4], dtype=torch.int32, device=DEV), torch.tensor([100], dtype=torch.int32, device=DEV), z(1, 1)
+    vexp, vlost = z(2, 1), z(2, 1, 2, 4)
+    fa = lambda v_, **kw: sm100.attention_fa(q, k, v_, cu, lens, table, 4, 4, 100, 1, 0.125, None, **kw)
+    tc = lambda v_, **kw: sm100.attention_prefill_tc(q, k, v_, cu, lens, table, 4, 1, 0.125, None, **kw)
+    for call in (fa, tc):
+        assert not call(v, vexp=vexp, vlost=vlost).any()
+        for bad in ({}, {"vexp": vexp}, {"vexp": vexp[:1], "vlost": vlost}, {"vexp": vexp, "vlost": vlost[:1]}, {"vexp": vexp.long(), "vlost": vlost},
+                    {"vexp": vexp, "vlost": vlost.cpu()}, {"vexp": vexp, "vlost": vlost.float()}):
+            with pytest.raises(ops.KernelError):
+                call(v, **bad)
+        with pytest.raises(ops.KernelError):
+            call(v.bfloat16(), vexp=vexp, vlost=vlost)
